@@ -360,6 +360,57 @@ MABA_API int maba_decode_dgda_mix(const maba_tensor* w, const maba_tensor* x, co
                                   void* workspace, size_t workspace_bytes, void* stream);
 MABA_API size_t maba_decode_dgda_mix_workspace_size(int32_t n_heads);
 
+/* ---- Dense operators ------------------------------------------------------
+ * The linear map with its epilogue and the gated feed-forward block (the dense
+ * half of MabaBlock: model.py:28-37 SwiGLUFFN, :107-108 / :126-127 the gated
+ * residual adds; the projections of layers/dgda.py and layers/sparse_attention.py),
+ * with the gradients that the reference takes from torch's autograd.
+ *
+ * x [M,K], weight [N,K]: float32 / float16 / bfloat16, one type, any strides.
+ * activation: 0 none, 1 relu, 2 silu, 3 gelu (0.5 z (1 + erf(z / sqrt 2))).
+ * bias, scale [N] (float32 or x's type, any stride), residual and grad [M,N]
+ * (float32 or x's type, any strides, 0 included); outputs have unit column stride
+ * and rows that do not overlap.  Optional tensors are NULL.  Sums are float32 and
+ * each result is rounded once; nothing depends on the order in which CTAs run.
+ * Workspace: 256-byte aligned, of the size that the matching call reports for the
+ * same tensors; one workspace serves one call at a time.
+ *
+ * maba_linear: out = residual + scale * act(x weight^T + bias), out [M,N] float32 or
+ *   x's type; out may be the residual itself, and no other input.
+ * maba_linear_backward: with z = x weight^T + bias (computed again) and
+ *   dz = grad * scale * act'(z): dx = dz weight, dw = dz^T x (x's type),
+ *   dbias = column sums of dz, dscale = column sums of grad * act(z); only the
+ *   outputs given are computed.  dz is rounded to x's type between the products.
+ * maba_gated_ffn: out [M,I] = act(x w_gate^T) * (x w_up^T), activation 1..3, x's type.
+ * maba_gated_ffn_backward: dx, dw_gate, dw_up for grad [M,I] (x's type); the gradients
+ *   of the two projections are rounded to x's type between the products. */
+MABA_API int maba_linear(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* bias, int32_t activation,
+                         const maba_tensor* scale, const maba_tensor* residual, const maba_tensor* out,
+                         void* workspace, size_t workspace_bytes, void* stream);
+MABA_API size_t maba_linear_workspace_size(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* out);
+MABA_API int maba_linear_backward(const maba_tensor* grad, const maba_tensor* x, const maba_tensor* weight,
+                                  const maba_tensor* bias, int32_t activation, const maba_tensor* scale,
+                                  const maba_tensor* dx, const maba_tensor* dw, const maba_tensor* dbias,
+                                  const maba_tensor* dscale, void* workspace, size_t workspace_bytes, void* stream);
+MABA_API size_t maba_linear_backward_workspace_size(const maba_tensor* grad, const maba_tensor* x,
+                                                    const maba_tensor* weight, const maba_tensor* bias,
+                                                    int32_t activation, const maba_tensor* scale,
+                                                    const maba_tensor* dx, const maba_tensor* dw,
+                                                    const maba_tensor* dbias, const maba_tensor* dscale);
+MABA_API int maba_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up,
+                            int32_t activation, const maba_tensor* out, void* workspace, size_t workspace_bytes,
+                            void* stream);
+MABA_API size_t maba_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up,
+                                              const maba_tensor* out);
+MABA_API int maba_gated_ffn_backward(const maba_tensor* grad, const maba_tensor* x, const maba_tensor* w_gate,
+                                     const maba_tensor* w_up, int32_t activation, const maba_tensor* dx,
+                                     const maba_tensor* dw_gate, const maba_tensor* dw_up, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+MABA_API size_t maba_gated_ffn_backward_workspace_size(const maba_tensor* grad, const maba_tensor* x,
+                                                       const maba_tensor* w_gate, const maba_tensor* w_up,
+                                                       const maba_tensor* dx, const maba_tensor* dw_gate,
+                                                       const maba_tensor* dw_up);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ CUDA kernels behind a C ABI (include/maba_b200.h, libmaba_b200.so), exposed
 with the reference project's op, registry and layer interfaces.
 """
 from .config import MabaSparseConfig, MabaConfig, get_101m_config
+from .dense import b200_gated_ffn, b200_gated_ffn_backward, b200_linear, b200_linear_backward
 from .dispatcher import (
     clear_dispatcher_cache,
     clear_fallback_warnings,

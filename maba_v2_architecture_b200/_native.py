@@ -31,13 +31,16 @@ DTYPE_CODES = {
 OK, ERR_INVALID, ERR_DTYPE, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA = range(6)
 
 
+_DIMS = ctypes.c_int64 * MAX_DIMS
+
+
 class MabaTensor(ctypes.Structure):
     _fields_ = [
         ("data", ctypes.c_void_p),
         ("dtype", ctypes.c_int32),
         ("ndim", ctypes.c_int32),
-        ("shape", ctypes.c_int64 * MAX_DIMS),
-        ("stride", ctypes.c_int64 * MAX_DIMS),
+        ("shape", _DIMS),
+        ("stride", _DIMS),
     ]
 
 
@@ -57,6 +60,14 @@ SIGNATURES = {
     "maba_dgda_frontend": (ctypes.c_int, [T_P] * 5 + [_i32, _f32, _vp]),
     "maba_rmsnorm_residual": (ctypes.c_int, [T_P, T_P, T_P, T_P, _f32, T_P, _vp]),
     "maba_swiglu": (ctypes.c_int, [T_P, T_P, _vp]),
+    "maba_linear": (ctypes.c_int, [T_P] * 3 + [_i32] + [T_P] * 3 + [_vp, _sz, _vp]),
+    "maba_linear_workspace_size": (_sz, [T_P] * 3),
+    "maba_linear_backward": (ctypes.c_int, [T_P] * 4 + [_i32] + [T_P] * 5 + [_vp, _sz, _vp]),
+    "maba_linear_backward_workspace_size": (_sz, [T_P] * 4 + [_i32] + [T_P] * 5),
+    "maba_gated_ffn": (ctypes.c_int, [T_P] * 3 + [_i32, T_P, _vp, _sz, _vp]),
+    "maba_gated_ffn_workspace_size": (_sz, [T_P] * 4),
+    "maba_gated_ffn_backward": (ctypes.c_int, [T_P] * 4 + [_i32] + [T_P] * 3 + [_vp, _sz, _vp]),
+    "maba_gated_ffn_backward_workspace_size": (_sz, [T_P] * 7),
     "maba_decode_gemv": (ctypes.c_int, [T_P, _i32, T_P, T_P, _f32, T_P, _i32, T_P, T_P, T_P, T_P, T_P, _i32, _i32,
                                         T_P, _vp, _vp, _sz, _vp]),
     "maba_decode_gemv_workspace_size": (_sz, [_i64]),
@@ -124,14 +135,7 @@ def desc(t: Optional[torch.Tensor]) -> Optional[MabaTensor]:
     code = DTYPE_CODES.get(t.dtype)
     if code is None:
         raise TypeError(f"maba_b200: unsupported dtype {t.dtype}")
-    d = MabaTensor()
-    d.data = t.data_ptr() if t.numel() > 0 else None
-    d.dtype = code
-    d.ndim = t.dim()
-    for i, (s, st) in enumerate(zip(t.shape, t.stride())):
-        d.shape[i] = s
-        d.stride[i] = st
-    return d
+    return MabaTensor(t.data_ptr() if t.numel() > 0 else None, code, t.dim(), _DIMS(*t.shape), _DIMS(*t.stride()))
 
 
 def ref(d: Optional[MabaTensor]):

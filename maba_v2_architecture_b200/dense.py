@@ -1,0 +1,338 @@
+"""Dense operators of the model's blocks: the linear map with its epilogue and the gated
+feed-forward block, with their gradients (maba_linear*, maba_gated_ffn* of the C ABI).
+
+    b200_linear      out = residual + scale * act(x weight^T + bias)
+    b200_gated_ffn   out = act(x w_gate^T) * (x w_up^T)
+
+The reference computes these with torch modules and autograd: SwiGLUFFN (maba_sparse/model.py:
+28-37), the gated residual adds (:107-108, :126-127) and the layers' projections.
+
+Inputs are float32, float16 or bfloat16 CUDA tensors of one type with any strides; leading
+dimensions of ``x`` are rows.  Sums are float32 and a result is rounded once; results do not
+depend on the order in which the GPU runs the work.  Inputs are never written, except that
+``out`` may be ``residual``.  Work is enqueued on the current stream of the tensors' device.
+Scratch memory comes from torch's allocator for each call (not from the per-stream buffer that
+the other ops keep): two captured graphs, or a graph and an eager call, then never share it.
+
+With gradients enabled and an input that requires one, both functions record themselves for
+autograd; ``*_backward`` are the same gradients as plain calls, for training loops that are
+captured into a CUDA graph or keep their own tape.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+DENSE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------
+# argument checks
+# ---------------------------------------------------------------------------
+def _check_operands(x: torch.Tensor, weights: Sequence[Tuple[str, torch.Tensor]]) -> None:
+    if x.dtype not in DENSE_DTYPES:
+        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {DENSE_DTYPES}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    n = weights[0][1].shape[0] if weights[0][1].dim() else 0
+    for name, w in weights:
+        if w.device != x.device:
+            raise RuntimeError(
+                f"Expected all tensors to be on the same device, but got {x.device} and {w.device} for {name}"
+            )
+        if w.dtype != x.dtype:
+            raise TypeError(f"Tensor dtypes must match, but got {x.dtype} for x and {w.dtype} for {name}")
+        if w.dim() != 2 or w.shape[0] != n or w.shape[1] != x.shape[-1]:
+            raise ValueError(f"{name} shape {list(w.shape)} must be [{n}, {x.shape[-1]}]")
+    if n == 0 or x.shape[-1] == 0:
+        raise ValueError(f"no features: x {list(x.shape)}, {weights[0][0]} {list(weights[0][1].shape)}")
+
+
+def _check_side(t: Optional[torch.Tensor], name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
+    if t is None:
+        return
+    if t.device != x.device:
+        raise RuntimeError(
+            f"Expected all tensors to be on the same device, but got {x.device} and {t.device} for {name}"
+        )
+    if t.dtype != x.dtype and not (f32 and t.dtype == torch.float32):
+        raise TypeError(f"{name} must be {x.dtype}{' or torch.float32' if f32 else ''}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} shape {list(t.shape)} must be {list(shape)}")
+
+
+def _activation(name: str, plain: bool) -> int:
+    code = ACTIVATIONS.get(name)
+    if code is None or (code == 0 and not plain):
+        names = [a for a, c in ACTIVATIONS.items() if plain or c]
+        raise ValueError(f"Unknown activation {name!r}. Supported: {names}")
+    return code
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_out(out: torch.Tensor, x: torch.Tensor, shape, inputs, residual) -> None:
+    _check_side(out, "out", x, shape)
+    if not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]):
+        raise ValueError(f"out must be contiguous or have contiguous rows, got strides {list(out.stride())}")
+    if out.numel() == 0:
+        return
+    lo, hi = _span(out)
+    for name, t in inputs:
+        if t is not None and t.numel() > 0:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError(f"out shares memory with {name}")
+    if residual is not None:
+        a, b = _span(residual)
+        same = (a == lo and residual.dtype == out.dtype and residual.stride() == out.stride())
+        if a < hi and lo < b and not same:
+            raise ValueError("out overlaps residual without being the same tensor")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+class _Device:
+    """Makes a tensor's device current (only where it is not): the C entries launch on the current device."""
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _call(fn, size, head, size_args, x) -> None:
+    """Runs one entry with scratch of the size it asks for."""
+    with _Device(x):
+        nbytes = size(*size_args)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, N.stream_of(x))
+    if rc != N.OK:
+        N.check(rc, fn.__name__)
+
+
+def _refs(*tensors):
+    return [None if t is None else N.ref(N.desc(t)) for t in tensors]
+
+
+# ---------------------------------------------------------------------------
+# the linear map
+# ---------------------------------------------------------------------------
+def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
+    if out is None:
+        out = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype or x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    rx, rw, rb, rs, rr, ro = _refs(_rows(x), weight, bias, scale, None if residual is None else _rows(residual),
+                                   out if out.dim() == 2 else out.view(-1, out.shape[-1]))
+    lib = N.lib()
+    _call(lib.maba_linear, lib.maba_linear_workspace_size, (rx, rw, rb, act, rs, rr, ro), (rx, rw, ro), x)
+    return out
+
+
+def _linear_backward(grad_out, x, weight, bias, act, scale, needs):
+    need_x, need_w, need_b, need_s = needs
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need_b else None
+    ds = torch.empty(scale.shape, dtype=scale.dtype, device=dev) if need_s else None
+    if any(needs):
+        rg, rx, rw, rb, rs, ox, ow, ob, os_ = _refs(_rows(grad_out), _rows(x), weight, bias, scale,
+                                                    None if dx is None else dx.view(-1, x.shape[-1]), dw, db, ds)
+        args = (rg, rx, rw, rb, act, rs, ox, ow, ob, os_)
+        lib = N.lib()
+        _call(lib.maba_linear_backward, lib.maba_linear_backward_workspace_size, args, args, x)
+    return dx, dw, db, ds
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, scale, residual, act, out_dtype):
+        ctx.save_for_backward(x, weight, bias, scale)
+        ctx.act, ctx.res_dtype = act, None if residual is None else residual.dtype
+        return _linear(x, weight, bias, act, scale, residual, None, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, weight, bias, scale = ctx.saved_tensors
+        dx, dw, db, ds = _linear_backward(grad_out, x, weight, bias, ctx.act, scale, ctx.needs_input_grad[:4])
+        dr = grad_out.to(ctx.res_dtype) if ctx.needs_input_grad[4] else None
+        return dx, dw, db, ds, dr, None, None
+
+
+def b200_linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    activation: str = "none",
+    scale: Optional[torch.Tensor] = None,
+    residual: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    """``residual + scale * act(x weight^T + bias)`` in one kernel.
+
+    x [..., K], weight [N, K] (nn.Linear's layout), bias and scale [N] and residual [..., N] in x's
+    dtype or float32; ``activation`` one of ``none``, ``relu``, ``silu``, ``gelu`` (the erf form).
+    The result [..., N] has x's dtype, or ``out_dtype=torch.float32``; ``out`` receives it in
+    place and may be ``residual`` (a residual stream updated where it is), not another input.
+    With the residual gates of MabaBlock as ``scale``: maba_sparse/model.py:107-108, 126-127.
+    """
+    act = _activation(activation, True)
+    _check_operands(x, (("weight", weight),))
+    n = weight.shape[0]
+    shape = (*x.shape[:-1], n)
+    _check_side(bias, "bias", x, (n,))
+    _check_side(scale, "scale", x, (n,))
+    _check_side(residual, "residual", x, shape)
+    if out_dtype is not None and out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
+    N.require_cuda(x, op="linear")
+    tracked = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias, scale, residual))
+    if out is not None:
+        if tracked or out.requires_grad:
+            raise RuntimeError("linear: out= does not support automatic differentiation")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError(f"out must be {out_dtype}, got {out.dtype}")
+        _check_out(out, x, shape, (("x", x), ("weight", weight), ("bias", bias), ("scale", scale)), residual)
+    if tracked:
+        return _LinearFunction.apply(x, weight, bias, scale, residual, act, out_dtype)
+    return _linear(x, weight, bias, act, scale, residual, out, out_dtype)
+
+
+def b200_linear_backward(
+    grad_out: torch.Tensor,
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    activation: str = "none",
+    scale: Optional[torch.Tensor] = None,
+    needs: Tuple[bool, bool, bool, bool] = (True, True, True, True),
+) -> Tuple[Optional[torch.Tensor], ...]:
+    """Gradients ``(dx, dweight, dbias, dscale)`` of ``b200_linear`` for its output's gradient
+    ``grad_out`` [..., N] (x's dtype or float32); the residual's is grad_out itself.  ``needs``
+    says which are computed (dbias / dscale only where bias / scale are given); the rest are None.
+
+    z = x weight^T + bias is computed again where act' or dscale needs it, so the forward pass
+    keeps nothing but its inputs.  grad_out * scale * act'(z) is rounded to x's dtype between the
+    products; the column sums of dbias and dscale are taken before that rounding.
+    """
+    act = _activation(activation, True)
+    _check_operands(x, (("weight", weight),))
+    n = weight.shape[0]
+    _check_side(bias, "bias", x, (n,))
+    _check_side(scale, "scale", x, (n,))
+    _check_side(grad_out, "grad_out", x, (*x.shape[:-1], n))
+    N.require_cuda(x, op="linear_backward")
+    needs = (bool(needs[0]), bool(needs[1]), bool(needs[2]) and bias is not None, bool(needs[3]) and scale is not None)
+    return _linear_backward(grad_out, x, weight, bias, act, scale, needs)
+
+
+# ---------------------------------------------------------------------------
+# the gated feed-forward block
+# ---------------------------------------------------------------------------
+def _gated_ffn(x, w_gate, w_up, act, out):
+    if out is None:
+        out = torch.empty((*x.shape[:-1], w_gate.shape[0]), dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    rx, rg, ru, ro = _refs(_rows(x), w_gate, w_up, out if out.dim() == 2 else out.view(-1, out.shape[-1]))
+    lib = N.lib()
+    _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, (rx, rg, ru, act, ro), (rx, rg, ru, ro), x)
+    return out
+
+
+def _gated_ffn_backward(grad_out, x, w_gate, w_up, act, needs):
+    need_x, need_g, need_u = needs
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dg = torch.empty(w_gate.shape, dtype=w_gate.dtype, device=dev) if need_g else None
+    du = torch.empty(w_up.shape, dtype=w_up.dtype, device=dev) if need_u else None
+    if any(needs):
+        rd, rx, rg, ru, ox, og, ou = _refs(_rows(grad_out), _rows(x), w_gate, w_up,
+                                           None if dx is None else dx.view(-1, x.shape[-1]), dg, du)
+        lib = N.lib()
+        _call(lib.maba_gated_ffn_backward, lib.maba_gated_ffn_backward_workspace_size,
+              (rd, rx, rg, ru, act, ox, og, ou), (rd, rx, rg, ru, ox, og, ou), x)
+    return dx, dg, du
+
+
+class _GatedFFNFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, act):
+        ctx.save_for_backward(x, w_gate, w_up)
+        ctx.act = act
+        return _gated_ffn(x, w_gate, w_up, act, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        return (*_gated_ffn_backward(grad_out, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad[:3]), None)
+
+
+def b200_gated_ffn(
+    x: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    activation: str = "silu",
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``act(x w_gate^T) * (x w_up^T)``: both projections, the activation and the product in one
+    kernel; the two projections are never stored.
+
+    x [..., K], w_gate and w_up [I, K]; ``activation`` one of ``silu``, ``gelu`` (the erf form),
+    ``relu``.  The result is [..., I] in x's dtype.  Reference: maba_sparse/model.py:28-37
+    (SwiGLUFFN without its down projection, which is ``b200_linear``).
+    """
+    act = _activation(activation, False)
+    _check_operands(x, (("w_gate", w_gate), ("w_up", w_up)))
+    N.require_cuda(x, op="gated_ffn")
+    tracked = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
+    if out is not None:
+        if tracked or out.requires_grad:
+            raise RuntimeError("gated_ffn: out= does not support automatic differentiation")
+        _check_side(out, "out", x, (*x.shape[:-1], w_gate.shape[0]), f32=False)
+        _check_out(out, x, out.shape, (("x", x), ("w_gate", w_gate), ("w_up", w_up)), None)
+    if tracked:
+        return _GatedFFNFunction.apply(x, w_gate, w_up, act)
+    return _gated_ffn(x, w_gate, w_up, act, out)
+
+
+def b200_gated_ffn_backward(
+    grad_out: torch.Tensor,
+    x: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    activation: str = "silu",
+    needs: Tuple[bool, bool, bool] = (True, True, True),
+) -> Tuple[Optional[torch.Tensor], ...]:
+    """Gradients ``(dx, dw_gate, dw_up)`` of ``b200_gated_ffn`` for ``grad_out`` [..., I] (x's dtype);
+    ``needs`` says which are computed.  The projections are computed again from the inputs; their
+    gradients are rounded to x's dtype between the products."""
+    act = _activation(activation, False)
+    _check_operands(x, (("w_gate", w_gate), ("w_up", w_up)))
+    _check_side(grad_out, "grad_out", x, (*x.shape[:-1], w_gate.shape[0]), f32=False)
+    N.require_cuda(x, op="gated_ffn_backward")
+    return _gated_ffn_backward(grad_out, x, w_gate, w_up, act, tuple(bool(n) for n in needs))
+
+
+__all__ = ["b200_linear", "b200_linear_backward", "b200_gated_ffn", "b200_gated_ffn_backward"]
