@@ -1,6 +1,7 @@
 // Library-wide pieces of the C ABI: version, per-thread error message,
 // descriptor validation helpers.
 #include "common.cuh"
+#include "dense.cuh"
 #include "sa_attention.cuh"
 
 #include <string.h>
@@ -75,7 +76,9 @@ extern "C" int maba_selftest_wait_timeout(int64_t limit_cycles, void* stream) {
 extern "C" int maba_device_error(int32_t* out, void* stream) {
     if (out == nullptr) return maba::set_error(MABA_ERR_INVALID, "device_error: out is null");
     int v = 0;
+    int dense = 0;
     MABA_TRY(maba::device_error_take(static_cast<cudaStream_t>(stream), &v));
-    *out = v;
+    MABA_TRY(maba::dense::device_error_take(static_cast<cudaStream_t>(stream), &dense));
+    *out = v != 0 ? v : dense;
     return MABA_OK;
 }

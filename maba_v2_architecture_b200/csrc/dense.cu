@@ -52,16 +52,16 @@ __global__ void __launch_bounds__(256) copy_kernel(Side src, int64_t rows, int64
     }
 }
 
-// out = sum over splits of partial [splits][rows][cols]; rows past `half` go to out2
+// out = sum over splits of partial [splits][rows][ldp]; rows from `half` on go to out2
 template <typename T>
 __global__ void __launch_bounds__(256)
-    sum_splits_kernel(const float* __restrict__ partial, int splits, int64_t rows, int64_t cols, T* out, T* out2,
-                      int64_t half, int64_t ld) {
+    sum_splits_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t rows, int64_t cols, T* out,
+                      T* out2, int64_t half, int64_t ld) {
     const int64_t n = rows * cols;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float z = 0.f;
-        for (int q = 0; q < splits; ++q) z += partial[q * n + i];
         const int64_t r = i / cols, c = i - r * cols;
+        float z = 0.f;
+        for (int q = 0; q < splits; ++q) z += partial[(q * rows + r) * ldp + c];
         T* o = r < half ? out + r * ld : out2 + (r - half) * ld;
         o[c] = Cvt<T>::from_f(z);
     }
@@ -117,7 +117,7 @@ inline unsigned grid1d(int64_t n) {
 // ---------------------------------------------------------------------------
 // Contraction splits of a plain product whose tiles do not fill the GPU; the partial sums
 // are float32 and added in split order.
-int splits_of(const Product& p) {
+int simt_splits(const Product& p) {
     if (p.e.kind != E_STORE) return 1;
     const int64_t tiles = ceil_div(p.M, SIMT_ROWS) * ceil_div(p.N, 128) * (p.form == F_PAIR ? 2 : 1);
     const int64_t steps = ceil_div(p.K, 16) * (p.form == F_SUM ? 2 : 1);
@@ -127,14 +127,15 @@ int splits_of(const Product& p) {
 }
 
 int run(Ctx& c, const Product& p) {
-    const int splits = splits_of(p);
-    const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M;
-    float* partial = splits > 1 ? static_cast<float*>(c.ws.take((size_t)splits * rows * p.N * 4)) : nullptr;
+    const int splits = c.dt == MABA_F32 ? simt_splits(p) : tc_splits(p);
+    const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
+    float* partial = splits > 1 ? static_cast<float*>(c.ws.take((size_t)splits * rows * ldp * 4)) : nullptr;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        MABA_TRY(simt_product<T>(p, splits, partial, c.s));
+        if constexpr (sizeof(T) == 4) MABA_TRY(simt_product<T>(p, splits, partial, ldp, c.s));
+        else MABA_TRY(tc_product<T>(p, partial, ldp, c.s));
         if (splits == 1) return (int)MABA_OK;
-        sum_splits_kernel<T><<<grid1d(rows * p.N), 256, 0, c.s>>>(partial, splits, rows, p.N, static_cast<T*>(p.e.out),
+        sum_splits_kernel<T><<<grid1d(rows * p.N), 256, 0, c.s>>>(partial, ldp, splits, rows, p.N, static_cast<T*>(p.e.out),
                                                                   static_cast<T*>(p.e.out2), p.M, p.e.ldo);
         return check_launch("dense(split sums)");
     });
@@ -215,8 +216,6 @@ int want_operands(const maba_tensor* x, const maba_tensor* w, const char* wname,
     return MABA_OK;
 }
 
-Matrix rows_of(const maba_tensor* t) { return Matrix{t->data, t->stride[0], t->stride[1]}; }   // [rows, contraction]
-Matrix cols_of(const maba_tensor* t) { return Matrix{t->data, t->stride[1], t->stride[0]}; }   // its transpose
 Side side2(const maba_tensor* t) {
     return given(t) ? Side{t->data, t->stride[0], t->stride[1], t->dtype == MABA_F32} : Side{};
 }
@@ -225,6 +224,21 @@ Side side1(const maba_tensor* t) { return given(t) ? Side{t->data, 0, t->stride[
 // ---------------------------------------------------------------------------
 // the operators
 // ---------------------------------------------------------------------------
+// A matrix as an operand.  The tensor-memory loads of the 16-bit products want rows on
+// 16-byte boundaries; what is not laid out so is copied once per call.  One copy serves
+// both directions of a matrix: K-major along its rows, MN-major across them.
+int operand(Ctx& c, const maba_tensor* t, Matrix& m) {
+    m = Matrix{t->data, t->stride[0], t->stride[1]};
+    if (c.dt == MABA_F32) return MABA_OK;
+    const int64_t rows = t->shape[0], cols = t->shape[1];
+    if (t->dtype == c.dt && tc_readable(t->data, rows, cols, t->stride[0], t->stride[1])) return MABA_OK;
+    const int64_t ld = (cols + 7) / 8 * 8;
+    void* to = c.ws.take((size_t)rows * ld * 2);
+    m = Matrix{to, ld, 1};
+    return copy_matrix(c, side2(t), rows, cols, to, ld);
+}
+Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr}; }
+
 struct LinearArgs {
     const maba_tensor *x, *w, *bias, *scale, *res, *out;              // forward
     const maba_tensor *g, *dx, *dw, *dbias, *dscale;                  // backward
@@ -233,10 +247,10 @@ struct LinearArgs {
 
 int linear_forward(Ctx& c, const LinearArgs& a) {
     Product p;
-    p.a[0] = rows_of(a.x);
-    p.b[0] = rows_of(a.w);
     p.M = a.x->shape[0], p.K = a.x->shape[1], p.N = a.w->shape[0];
     if (p.M == 0) return MABA_OK;
+    MABA_TRY(operand(c, a.x, p.a[0]));
+    MABA_TRY(operand(c, a.w, p.b[0]));
     p.e.kind = E_LINEAR;
     p.e.act = a.act;
     p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.res);
@@ -255,20 +269,21 @@ int zero_rows(Ctx& c, const maba_tensor* t) {
 }
 
 // dx = sum of d_i W_i and dW_i = d_i^T x for one or two (d, W)
-int dx_product(Ctx& c, int64_t M, int n, const Matrix* d, const maba_tensor* const* w, const maba_tensor* dx) {
+int dx_product(Ctx& c, int64_t M, int64_t N, int n, const Matrix* d, const Matrix* w, const maba_tensor* dx) {
     Product p;
     p.form = n == 2 ? F_SUM : F_SINGLE;
-    p.M = M, p.N = w[0]->shape[1], p.K = w[0]->shape[0];
-    for (int i = 0; i < n; ++i) p.a[i] = d[i], p.b[i] = cols_of(w[i]);
+    p.M = M, p.N = dx->shape[1], p.K = N;
+    for (int i = 0; i < n; ++i) p.a[i] = d[i], p.b[i] = transposed(w[i]);
     p.e.out = dx->data, p.e.ldo = dx->stride[0];
     return run(c, p);
 }
-int dw_product(Ctx& c, int64_t M, int n, const Matrix* d, const maba_tensor* x, const maba_tensor* const* dw) {
+int dw_product(Ctx& c, int64_t M, int n, const Matrix* d, const Matrix& x, const maba_tensor* const* dw) {
     Product p;
     p.form = n == 2 ? F_PAIR : F_SINGLE;
-    p.M = dw[0]->shape[0], p.N = x->shape[1], p.K = M;
-    for (int i = 0; i < n; ++i) p.a[i] = Matrix{d[i].p, d[i].sk, d[i].sr};
-    p.b[0] = cols_of(x);
+    p.M = dw[0]->shape[0], p.N = dw[0]->shape[1], p.K = M;
+    for (int i = 0; i < n; ++i) p.a[i] = transposed(d[i]);
+    p.b[0] = transposed(x);
+    p.a_mn = true;
     p.e.out = dw[0]->data, p.e.ldo = dw[0]->stride[0];
     if (n == 2) p.e.out2 = dw[1]->data;
     return run(c, p);
@@ -283,18 +298,20 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         return zero_rows(c, a.dscale);
     }
     if (!need_dx && !need_dw && !need_db && !need_ds) return MABA_OK;
-    const int64_t blocks = ceil_div(M, SIMT_ROWS);
+    const bool through = a.act == ACT_NONE && !given(a.scale);  // dz = g
+    const int64_t blocks = ceil_div(M, through ? CS_ROWS : (c.dt == MABA_F32 ? SIMT_ROWS : TC_ROWS));
     float* pb = need_db ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     float* ps = need_ds ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
-    Matrix d = rows_of(a.g);
-    const int64_t ld = (N + 7) / 8 * 8;
-    const bool through = a.act == ACT_NONE && !given(a.scale);  // dz = g
+    Matrix x, w, d;
+    if (!through || need_dw) MABA_TRY(operand(c, a.x, x));
+    if (!through || need_dx) MABA_TRY(operand(c, a.w, w));
     if (!through) {
         // z again, rather than a copy kept by the forward pass: a 16-bit z would add its own
         // rounding to phi'(z), and a float32 one costs more traffic than the product
+        const int64_t ld = (N + 7) / 8 * 8;
         Product p;
         p.M = M, p.N = N, p.K = K;
-        p.a[0] = rows_of(a.x), p.b[0] = rows_of(a.w);
+        p.a[0] = x, p.b[0] = w;
         p.e.kind = E_LINEAR_BWD;
         p.e.act = a.act;
         p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.g);
@@ -304,16 +321,13 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         d = Matrix{p.e.out, ld, 1};
     } else {
         if (need_db) MABA_TRY(column_sums(c, side2(a.g), M, N, pb));
-        if (a.g->dtype != c.dt && (need_dx || need_dw)) {  // the products take one type: g rounded to it
-            void* t = c.ws.take((size_t)M * ld * esize(c.dt));
-            MABA_TRY(copy_matrix(c, side2(a.g), M, N, t, ld));
-            d = Matrix{t, ld, 1};
-        }
+        // the products take one type: a float32 gradient is rounded to x's here
+        if (need_dx || need_dw) MABA_TRY(operand(c, a.g, d));
     }
     if (need_db) MABA_TRY(finish_columns(c, pb, blocks, N, a.dbias));
     if (need_ds) MABA_TRY(finish_columns(c, ps, blocks, N, a.dscale));
-    if (need_dx) MABA_TRY(dx_product(c, M, 1, &d, &a.w, a.dx));
-    if (need_dw) MABA_TRY(dw_product(c, M, 1, &d, a.x, &a.dw));
+    if (need_dx) MABA_TRY(dx_product(c, M, N, 1, &d, &w, a.dx));
+    if (need_dw) MABA_TRY(dw_product(c, M, 1, &d, x, &a.dw));
     return MABA_OK;
 }
 
@@ -323,17 +337,19 @@ struct FfnArgs {
     int act;
 };
 
-Product ffn_product(const FfnArgs& a) {
-    Product p;
+int ffn_product(Ctx& c, const FfnArgs& a, Product& p) {
     p.form = F_DUAL;
     p.M = a.x->shape[0], p.K = a.x->shape[1], p.N = a.wg->shape[0];
-    p.a[0] = rows_of(a.x), p.b[0] = rows_of(a.wg), p.b[1] = rows_of(a.wu);
     p.e.act = a.act;
-    return p;
+    if (p.M == 0) return MABA_OK;
+    MABA_TRY(operand(c, a.x, p.a[0]));
+    MABA_TRY(operand(c, a.wg, p.b[0]));
+    return operand(c, a.wu, p.b[1]);
 }
 
 int ffn_forward(Ctx& c, const FfnArgs& a) {
-    Product p = ffn_product(a);
+    Product p;
+    MABA_TRY(ffn_product(c, a, p));
     if (p.M == 0) return MABA_OK;
     p.e.kind = E_GLU;
     if (a.out) p.e.out = a.out->data, p.e.ldo = a.out->stride[0];
@@ -341,13 +357,15 @@ int ffn_forward(Ctx& c, const FfnArgs& a) {
 }
 
 int ffn_backward(Ctx& c, const FfnArgs& a) {
-    Product p = ffn_product(a);
-    const int64_t M = p.M, ld = (p.N + 7) / 8 * 8;
+    const int64_t M = a.x->shape[0];
     if (M == 0) {
         MABA_TRY(zero_rows(c, a.dwg));
         return zero_rows(c, a.dwu);
     }
     if (!given(a.dx) && !given(a.dwg) && !given(a.dwu)) return MABA_OK;
+    Product p;
+    MABA_TRY(ffn_product(c, a, p));
+    const int64_t ld = (p.N + 7) / 8 * 8;
     // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
     // the one rounding between the two passes
     p.e.kind = E_GLU_BWD;
@@ -356,12 +374,12 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     p.e.out2 = c.ws.take((size_t)M * ld * esize(c.dt));
     MABA_TRY(run(c, p));
     const Matrix d[2] = {{p.e.out, ld, 1}, {p.e.out2, ld, 1}};
-    const maba_tensor* w[2] = {a.wg, a.wu};
-    if (given(a.dx)) MABA_TRY(dx_product(c, M, 2, d, w, a.dx));
+    if (given(a.dx)) MABA_TRY(dx_product(c, M, p.N, 2, d, p.b, a.dx));
     const maba_tensor* dw[2] = {a.dwg, a.dwu};
-    if (given(a.dwg) && given(a.dwu) && a.dwg->stride[0] == a.dwu->stride[0]) return dw_product(c, M, 2, d, a.x, dw);
+    if (given(a.dwg) && given(a.dwu) && a.dwg->stride[0] == a.dwu->stride[0])
+        return dw_product(c, M, 2, d, p.a[0], dw);
     for (int i = 0; i < 2; ++i)
-        if (given(dw[i])) MABA_TRY(dw_product(c, M, 1, d + i, a.x, dw + i));
+        if (given(dw[i])) MABA_TRY(dw_product(c, M, 1, d + i, p.a[0], dw + i));
     return MABA_OK;
 }
 

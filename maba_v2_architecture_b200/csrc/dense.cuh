@@ -60,6 +60,7 @@ struct Product {
     int form = F_SINGLE;
     Matrix a[2], b[2];
     int64_t M = 0, N = 0, K = 0;
+    bool a_mn = false;  // E_STORE: A's rows (not its contraction) are contiguous; B's rows always are
     Epilogue e;
 };
 
@@ -95,9 +96,18 @@ template <typename T> __device__ __forceinline__ float side_at(const Side& s, in
     return s.f32 ? static_cast<const float*>(s.p)[i] : Cvt<T>::to_f(static_cast<const T*>(s.p)[i]);
 }
 
-// dense_simt.cu: any type and any strides, CUDA cores.  Row tiles of SIMT_ROWS rows.
+// Partial sums of a split product: float32 [split][rows][ldp], rows = M (2 M of F_PAIR).
+
+// dense_simt.cu: any type and any strides, CUDA cores; column sums per 128 rows.
 constexpr int SIMT_ROWS = 128;
-template <typename T> int simt_product(const Product& p, int splits, float* partial, cudaStream_t s);
+template <typename T> int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s);
+
+// dense_tc.cu: 16-bit operands that tc_readable() accepts, tensor cores; column sums per 32 rows.
+constexpr int TC_ROWS = 32;
+bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
+int tc_splits(const Product& p);
+template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s);
+int device_error_take(cudaStream_t s, int* out);
 
 }  // namespace dense
 }  // namespace maba

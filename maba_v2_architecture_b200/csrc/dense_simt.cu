@@ -69,7 +69,7 @@ template <typename T> __device__ __forceinline__ bool vec_ok(const Matrix& m) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NTHR) simt_kernel(const Product p, int tiles_n, int splits, float* partial) {
+__global__ void __launch_bounds__(NTHR) simt_kernel(const Product p, int tiles_n, int splits, float* partial, int64_t ldp) {
     __shared__ float As[2][BK * LD], Bs[2][BK * LD];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const bool dual = p.form == F_DUAL;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(NTHR) simt_kernel(const Product p, int tiles_n
             if (e.kind == E_STORE) {
                 if (n >= p.N) continue;
                 const int64_t mo = m + pair * p.M;
-                if (splits > 1) partial[((int64_t)blockIdx.y * rows_out + mo) * p.N + n] = z;
+                if (splits > 1) partial[((int64_t)blockIdx.y * rows_out + mo) * ldp + n] = z;
                 else static_cast<T*>(pair ? e.out2 : e.out)[m * e.ldo + n] = Cvt<T>::from_f(z);
             } else if (e.kind == E_LINEAR) {
                 if (n >= p.N) continue;
@@ -209,17 +209,15 @@ __global__ void __launch_bounds__(NTHR) simt_kernel(const Product p, int tiles_n
 
 }  // namespace
 
-template <typename T> int simt_product(const Product& p, int splits, float* partial, cudaStream_t s) {
+template <typename T> int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s) {
     const int bn = p.form == F_DUAL ? 64 : BN;
     const int64_t tn = ceil_div(p.N, bn), tm = ceil_div(p.M, BM);
     if (tm * tn > 0x7fffffff) return set_error(MABA_ERR_UNSUPPORTED, "dense: %lld tiles", (long long)(tm * tn));
     dim3 grid((unsigned)(tm * tn), (unsigned)splits, p.form == F_PAIR ? 2 : 1);
-    simt_kernel<T><<<grid, NTHR, 0, s>>>(p, (int)tn, splits, partial);
+    simt_kernel<T><<<grid, NTHR, 0, s>>>(p, (int)tn, splits, partial, ldp);
     return check_launch("dense(simt)");
 }
-template int simt_product<float>(const Product&, int, float*, cudaStream_t);
-template int simt_product<__half>(const Product&, int, float*, cudaStream_t);
-template int simt_product<__nv_bfloat16>(const Product&, int, float*, cudaStream_t);
+template int simt_product<float>(const Product&, int, float*, int64_t, cudaStream_t);
 
 }  // namespace dense
 }  // namespace maba

@@ -41,8 +41,8 @@
 // read by maba_device_error() is set.
 #include "sa_attention.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.cuh"
 
-#include <cudaTypedefs.h>
 #include <type_traits>
 
 namespace maba {
@@ -930,46 +930,6 @@ __global__ void __launch_bounds__(NTHR, 1)
 }
 
 // ------------------------------------------------------------------ host side
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_fn() {
-    static EncodeTiled fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) !=
-                cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
-    return fn;
-}
-
-// rank-R tiled map of 16-bit elements, 128-byte swizzle; strides in elements (R-1 of them)
-bool make_map(CUtensorMap* m, int dtype, const void* ptr, int rank, const int64_t* dims, const int64_t* strides,
-              const uint32_t* box) {
-    EncodeTiled fn = encode_fn();
-    if (fn == nullptr) return false;
-    cuuint64_t gd[5], gs[4];
-    cuuint32_t bx[5], es[5];
-    for (int i = 0; i < rank; ++i) {
-        gd[i] = (cuuint64_t)dims[i];
-        bx[i] = box[i];
-        es[i] = 1;
-        if (i + 1 < rank) gs[i] = (cuuint64_t)strides[i] * 2;
-    }
-    const CUresult r =
-        fn(m, dtype == MABA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
-           const_cast<void*>(ptr), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
-}
-
-inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline bool s16(int64_t stride_elems) { return ((stride_elems * 2) % 16) == 0 && stride_elems > 0; }
-
 // Largest L2 norm of the rows of each 64-row tile of c_kv [B, L, 128] (tiles
 // 0..ntc-1) and of the pooled HCA entries [B, NC, 128] (tiles ntc..ntc+nth-1),
 // scaled by 1 + 1e-3 so that |q| * norm bounds every score of the tile.
