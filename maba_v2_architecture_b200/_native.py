@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 from typing import Optional
@@ -60,14 +61,15 @@ SIGNATURES = {
     "maba_dgda_frontend": (ctypes.c_int, [T_P] * 5 + [_i32, _f32, _vp]),
     "maba_rmsnorm_residual": (ctypes.c_int, [T_P, T_P, T_P, T_P, _f32, T_P, _vp]),
     "maba_swiglu": (ctypes.c_int, [T_P, T_P, _vp]),
-    "maba_linear": (ctypes.c_int, [T_P] * 3 + [_i32] + [T_P] * 3 + [_vp, _sz, _vp]),
-    "maba_linear_workspace_size": (_sz, [T_P] * 3),
-    "maba_linear_backward": (ctypes.c_int, [T_P] * 4 + [_i32] + [T_P] * 5 + [_vp, _sz, _vp]),
-    "maba_linear_backward_workspace_size": (_sz, [T_P] * 4 + [_i32] + [T_P] * 5),
-    "maba_gated_ffn": (ctypes.c_int, [T_P] * 3 + [_i32, T_P, _vp, _sz, _vp]),
-    "maba_gated_ffn_workspace_size": (_sz, [T_P] * 4),
-    "maba_gated_ffn_backward": (ctypes.c_int, [T_P] * 4 + [_i32] + [T_P] * 3 + [_vp, _sz, _vp]),
-    "maba_gated_ffn_backward_workspace_size": (_sz, [T_P] * 7),
+    # the dense entries take their descriptors as addresses of packed bytes (pack_matrix / pack_vector)
+    "maba_linear": (ctypes.c_int, [_vp] * 3 + [_i32] + [_vp] * 3 + [_vp, _sz, _vp]),
+    "maba_linear_workspace_size": (_sz, [_vp] * 3),
+    "maba_linear_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 5 + [_vp, _sz, _vp]),
+    "maba_linear_backward_workspace_size": (_sz, [_vp] * 4 + [_i32] + [_vp] * 5),
+    "maba_gated_ffn": (ctypes.c_int, [_vp] * 3 + [_i32, _vp, _vp, _sz, _vp]),
+    "maba_gated_ffn_workspace_size": (_sz, [_vp] * 4),
+    "maba_gated_ffn_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 3 + [_vp, _sz, _vp]),
+    "maba_gated_ffn_backward_workspace_size": (_sz, [_vp] * 7),
     "maba_decode_gemv": (ctypes.c_int, [T_P, _i32, T_P, T_P, _f32, T_P, _i32, T_P, T_P, T_P, T_P, T_P, _i32, _i32,
                                         T_P, _vp, _vp, _sz, _vp]),
     "maba_decode_gemv_workspace_size": (_sz, [_i64]),
@@ -138,6 +140,19 @@ def desc(t: Optional[torch.Tensor]) -> Optional[MabaTensor]:
     return MabaTensor(t.data_ptr() if t.numel() > 0 else None, code, t.dim(), _DIMS(*t.shape), _DIMS(*t.stride()))
 
 
+_pack = struct.Struct("@Pii12q").pack  # a MabaTensor
+
+
+def pack_matrix(t: torch.Tensor) -> bytes:
+    """Descriptor of a 2-D device tensor as bytes (a third of a MabaTensor's cost to make)."""
+    (rows, cols), (sr, sc) = t.shape, t.stride()
+    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 2, rows, cols, 0, 0, 0, 0, sr, sc, 0, 0, 0, 0)
+
+
+def pack_vector(t: torch.Tensor) -> bytes:
+    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 1, t.shape[0], 0, 0, 0, 0, 0, t.stride(0), 0, 0, 0, 0, 0)
+
+
 def ref(d: Optional[MabaTensor]):
     return ctypes.byref(d) if d is not None else None
 
@@ -153,7 +168,8 @@ def desc_array(tensors) -> ctypes.Array:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # torch.cuda.current_stream(t.device).cuda_stream without the Stream object
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def check(rc: int, what: str) -> None:

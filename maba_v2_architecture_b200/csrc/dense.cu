@@ -127,6 +127,10 @@ int simt_splits(const Product& p) {
 }
 
 int run(Ctx& c, const Product& p) {
+    if (skinny_takes(p, c.dt)) {
+        if (c.dry) return MABA_OK;
+        return DENSE_DISPATCH(c.dt, [&] { return skinny_product<T>(p, c.s); });
+    }
     const int splits = c.dt == MABA_F32 ? simt_splits(p) : tc_splits(p);
     const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
     float* partial = splits > 1 ? static_cast<float*>(c.ws.take((size_t)splits * rows * ldp * 4)) : nullptr;
@@ -227,9 +231,9 @@ Side side1(const maba_tensor* t) { return given(t) ? Side{t->data, 0, t->stride[
 // A matrix as an operand.  The tensor-memory loads of the 16-bit products want rows on
 // 16-byte boundaries; what is not laid out so is copied once per call.  One copy serves
 // both directions of a matrix: K-major along its rows, MN-major across them.
-int operand(Ctx& c, const maba_tensor* t, Matrix& m) {
+int operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
     m = Matrix{t->data, t->stride[0], t->stride[1]};
-    if (c.dt == MABA_F32) return MABA_OK;
+    if (c.dt == MABA_F32 || as_is) return MABA_OK;
     const int64_t rows = t->shape[0], cols = t->shape[1];
     if (t->dtype == c.dt && tc_readable(t->data, rows, cols, t->stride[0], t->stride[1])) return MABA_OK;
     const int64_t ld = (cols + 7) / 8 * 8;
@@ -249,9 +253,10 @@ int linear_forward(Ctx& c, const LinearArgs& a) {
     Product p;
     p.M = a.x->shape[0], p.K = a.x->shape[1], p.N = a.w->shape[0];
     if (p.M == 0) return MABA_OK;
-    MABA_TRY(operand(c, a.x, p.a[0]));
-    MABA_TRY(operand(c, a.w, p.b[0]));
     p.e.kind = E_LINEAR;
+    const bool as_is = skinny_takes(p, c.dt);
+    MABA_TRY(operand(c, a.x, p.a[0], as_is));
+    MABA_TRY(operand(c, a.w, p.b[0], as_is));
     p.e.act = a.act;
     p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.res);
     if (a.out) p.e.out = a.out->data, p.e.ldo = a.out->stride[0], p.e.out_f32 = a.out->dtype == MABA_F32;
@@ -341,17 +346,18 @@ int ffn_product(Ctx& c, const FfnArgs& a, Product& p) {
     p.form = F_DUAL;
     p.M = a.x->shape[0], p.K = a.x->shape[1], p.N = a.wg->shape[0];
     p.e.act = a.act;
+    p.e.kind = given(a.g) ? E_GLU_BWD : E_GLU;
     if (p.M == 0) return MABA_OK;
-    MABA_TRY(operand(c, a.x, p.a[0]));
-    MABA_TRY(operand(c, a.wg, p.b[0]));
-    return operand(c, a.wu, p.b[1]);
+    const bool as_is = skinny_takes(p, c.dt);
+    MABA_TRY(operand(c, a.x, p.a[0], as_is));
+    MABA_TRY(operand(c, a.wg, p.b[0], as_is));
+    return operand(c, a.wu, p.b[1], as_is);
 }
 
 int ffn_forward(Ctx& c, const FfnArgs& a) {
     Product p;
     MABA_TRY(ffn_product(c, a, p));
     if (p.M == 0) return MABA_OK;
-    p.e.kind = E_GLU;
     if (a.out) p.e.out = a.out->data, p.e.ldo = a.out->stride[0];
     return run(c, p);
 }
@@ -368,7 +374,6 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     const int64_t ld = (p.N + 7) / 8 * 8;
     // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
     // the one rounding between the two passes
-    p.e.kind = E_GLU_BWD;
     p.e.res = side2(a.g);
     p.e.out = c.ws.take((size_t)M * ld * esize(c.dt)), p.e.ldo = ld;
     p.e.out2 = c.ws.take((size_t)M * ld * esize(c.dt));

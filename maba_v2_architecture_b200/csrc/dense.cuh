@@ -102,6 +102,10 @@ template <typename T> __device__ __forceinline__ float side_at(const Side& s, in
 constexpr int SIMT_ROWS = 128;
 template <typename T> int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s);
 
+// dense_skinny.cu: forward products of few rows, any strides.
+bool skinny_takes(const Product& p, int dt);
+template <typename T> int skinny_product(const Product& p, cudaStream_t s);
+
 // dense_tc.cu: 16-bit operands that tc_readable() accepts, tensor cores; column sums per 32 rows.
 constexpr int TC_ROWS = 32;
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);

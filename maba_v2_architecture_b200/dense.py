@@ -34,35 +34,40 @@ DENSE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 # ---------------------------------------------------------------------------
 # argument checks
 # ---------------------------------------------------------------------------
-def _check_operands(x: torch.Tensor, weights: Sequence[Tuple[str, torch.Tensor]]) -> None:
-    if x.dtype not in DENSE_DTYPES:
-        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {DENSE_DTYPES}")
-    if x.dim() < 1:
-        raise ValueError("x must have at least one dimension")
-    n = weights[0][1].shape[0] if weights[0][1].dim() else 0
-    for name, w in weights:
-        if w.device != x.device:
-            raise RuntimeError(
-                f"Expected all tensors to be on the same device, but got {x.device} and {w.device} for {name}"
-            )
-        if w.dtype != x.dtype:
-            raise TypeError(f"Tensor dtypes must match, but got {x.dtype} for x and {w.dtype} for {name}")
-        if w.dim() != 2 or w.shape[0] != n or w.shape[1] != x.shape[-1]:
-            raise ValueError(f"{name} shape {list(w.shape)} must be [{n}, {x.shape[-1]}]")
-    if n == 0 or x.shape[-1] == 0:
-        raise ValueError(f"no features: x {list(x.shape)}, {weights[0][0]} {list(weights[0][1].shape)}")
-
-
-def _check_side(t: Optional[torch.Tensor], name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
-    if t is None:
-        return
+def _check_device(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
     if t.device != x.device:
         raise RuntimeError(
             f"Expected all tensors to be on the same device, but got {x.device} and {t.device} for {name}"
         )
-    if t.dtype != x.dtype and not (f32 and t.dtype == torch.float32):
+
+
+def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, n: int, k: int) -> None:
+    _check_device(w, name, x)
+    if w.dtype is not x.dtype:
+        raise TypeError(f"Tensor dtypes must match, but got {x.dtype} for x and {w.dtype} for {name}")
+    if w.shape != (n, k):
+        raise ValueError(f"{name} shape {list(w.shape)} must be [{n}, {k}]")
+
+
+def _check_x(x: torch.Tensor, w: torch.Tensor, name: str) -> Tuple[int, int]:
+    """Output and input features."""
+    if x.dtype not in DENSE_DTYPES:
+        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {DENSE_DTYPES}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    k = x.shape[-1]
+    n = w.shape[0] if w.dim() else 0
+    _check_weight(w, name, x, n, k)
+    if n == 0 or k == 0:
+        raise ValueError(f"no features: x {list(x.shape)}, {name} {list(w.shape)}")
+    return n, k
+
+
+def _check_side(t: torch.Tensor, name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
+    _check_device(t, name, x)
+    if t.dtype is not x.dtype and not (f32 and t.dtype is torch.float32):
         raise TypeError(f"{name} must be {x.dtype}{' or torch.float32' if f32 else ''}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} shape {list(t.shape)} must be {list(shape)}")
 
 
@@ -98,37 +103,35 @@ def _check_out(out: torch.Tensor, x: torch.Tensor, shape, inputs, residual) -> N
             raise ValueError("out overlaps residual without being the same tensor")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-
-
-class _Device:
-    """Makes a tensor's device current (only where it is not): the C entries launch on the current device."""
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _call(fn, size, head, size_args, x) -> None:
-    """Runs one entry with scratch of the size it asks for."""
-    with _Device(x):
-        nbytes = size(*size_args)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, N.stream_of(x))
+def _call(fn, size, x: torch.Tensor, head, size_args) -> None:
+    """Runs one entry on x's device (made current where it is not: the C entries launch on the current
+    device).  ``size_args`` None: most calls of the entry need no scratch memory, so it is tried
+    without; it refuses before it launches anything."""
+    index = x.device.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _call(fn, size, x, head, size_args)
+    stream = N.stream_of(x)
+    if size_args is None:
+        rc = fn(*head, None, 0, stream)
+        if rc != N.ERR_WORKSPACE:
+            return None if rc == N.OK else N.check(rc, fn.__name__)
+        size_args = (*head[:len(size.argtypes) - 1], head[-1])
+    nbytes = size(*size_args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, stream)
     if rc != N.OK:
         N.check(rc, fn.__name__)
 
 
-def _refs(*tensors):
-    return [None if t is None else N.ref(N.desc(t)) for t in tensors]
+def _mat(t: Optional[torch.Tensor]) -> Optional[bytes]:
+    if t is None:
+        return None
+    return N.pack_matrix(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+
+
+def _vec(t: Optional[torch.Tensor]) -> Optional[bytes]:
+    return None if t is None else N.pack_vector(t)
 
 
 # ---------------------------------------------------------------------------
@@ -139,26 +142,22 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
         out = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype or x.dtype, device=x.device)
     if out.numel() == 0:
         return out
-    rx, rw, rb, rs, rr, ro = _refs(_rows(x), weight, bias, scale, None if residual is None else _rows(residual),
-                                   out if out.dim() == 2 else out.view(-1, out.shape[-1]))
     lib = N.lib()
-    _call(lib.maba_linear, lib.maba_linear_workspace_size, (rx, rw, rb, act, rs, rr, ro), (rx, rw, ro), x)
+    _call(lib.maba_linear, lib.maba_linear_workspace_size, x,
+          (_mat(x), _mat(weight), _vec(bias), act, _vec(scale), _mat(residual), _mat(out)), None)
     return out
 
 
 def _linear_backward(grad_out, x, weight, bias, act, scale, needs):
     need_x, need_w, need_b, need_s = needs
-    dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need_b else None
-    ds = torch.empty(scale.shape, dtype=scale.dtype, device=dev) if need_s else None
-    if any(needs):
-        rg, rx, rw, rb, rs, ox, ow, ob, os_ = _refs(_rows(grad_out), _rows(x), weight, bias, scale,
-                                                    None if dx is None else dx.view(-1, x.shape[-1]), dw, db, ds)
-        args = (rg, rx, rw, rb, act, rs, ox, ow, ob, os_)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if need_w else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if need_b else None
+    ds = torch.empty(scale.shape, dtype=scale.dtype, device=x.device) if need_s else None
+    if need_x or need_w or need_b or need_s:
         lib = N.lib()
-        _call(lib.maba_linear_backward, lib.maba_linear_backward_workspace_size, args, args, x)
+        args = (_mat(grad_out), _mat(x), _mat(weight), _vec(bias), act, _vec(scale), _mat(dx), _mat(dw), _vec(db), _vec(ds))
+        _call(lib.maba_linear_backward, lib.maba_linear_backward_workspace_size, x, args, args)
     return dx, dw, db, ds
 
 
@@ -197,17 +196,21 @@ def b200_linear(
     With the residual gates of MabaBlock as ``scale``: maba_sparse/model.py:107-108, 126-127.
     """
     act = _activation(activation, True)
-    _check_operands(x, (("weight", weight),))
-    n = weight.shape[0]
+    n, _ = _check_x(x, weight, "weight")
     shape = (*x.shape[:-1], n)
-    _check_side(bias, "bias", x, (n,))
-    _check_side(scale, "scale", x, (n,))
-    _check_side(residual, "residual", x, shape)
+    if bias is not None:
+        _check_side(bias, "bias", x, (n,))
+    if scale is not None:
+        _check_side(scale, "scale", x, (n,))
+    if residual is not None:
+        _check_side(residual, "residual", x, shape)
     if out_dtype is not None and out_dtype not in (x.dtype, torch.float32):
         raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
-    N.require_cuda(x, op="linear")
-    tracked = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias, scale, residual))
+    if not x.is_cuda:
+        N.require_cuda(x, op="linear")
+    tracked = torch.is_grad_enabled() and (
+        x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+        or (scale is not None and scale.requires_grad) or (residual is not None and residual.requires_grad))
     if out is not None:
         if tracked or out.requires_grad:
             raise RuntimeError("linear: out= does not support automatic differentiation")
@@ -237,10 +240,11 @@ def b200_linear_backward(
     products; the column sums of dbias and dscale are taken before that rounding.
     """
     act = _activation(activation, True)
-    _check_operands(x, (("weight", weight),))
-    n = weight.shape[0]
-    _check_side(bias, "bias", x, (n,))
-    _check_side(scale, "scale", x, (n,))
+    n, _ = _check_x(x, weight, "weight")
+    if bias is not None:
+        _check_side(bias, "bias", x, (n,))
+    if scale is not None:
+        _check_side(scale, "scale", x, (n,))
     _check_side(grad_out, "grad_out", x, (*x.shape[:-1], n))
     N.require_cuda(x, op="linear_backward")
     needs = (bool(needs[0]), bool(needs[1]), bool(needs[2]) and bias is not None, bool(needs[3]) and scale is not None)
@@ -255,24 +259,22 @@ def _gated_ffn(x, w_gate, w_up, act, out):
         out = torch.empty((*x.shape[:-1], w_gate.shape[0]), dtype=x.dtype, device=x.device)
     if out.numel() == 0:
         return out
-    rx, rg, ru, ro = _refs(_rows(x), w_gate, w_up, out if out.dim() == 2 else out.view(-1, out.shape[-1]))
     lib = N.lib()
-    _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, (rx, rg, ru, act, ro), (rx, rg, ru, ro), x)
+    _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, x, (_mat(x), _mat(w_gate), _mat(w_up), act, _mat(out)),
+          None)
     return out
 
 
 def _gated_ffn_backward(grad_out, x, w_gate, w_up, act, needs):
     need_x, need_g, need_u = needs
-    dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dg = torch.empty(w_gate.shape, dtype=w_gate.dtype, device=dev) if need_g else None
-    du = torch.empty(w_up.shape, dtype=w_up.dtype, device=dev) if need_u else None
-    if any(needs):
-        rd, rx, rg, ru, ox, og, ou = _refs(_rows(grad_out), _rows(x), w_gate, w_up,
-                                           None if dx is None else dx.view(-1, x.shape[-1]), dg, du)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    dg = torch.empty(w_gate.shape, dtype=x.dtype, device=x.device) if need_g else None
+    du = torch.empty(w_up.shape, dtype=x.dtype, device=x.device) if need_u else None
+    if need_x or need_g or need_u:
         lib = N.lib()
-        _call(lib.maba_gated_ffn_backward, lib.maba_gated_ffn_backward_workspace_size,
-              (rd, rx, rg, ru, act, ox, og, ou), (rd, rx, rg, ru, ox, og, ou), x)
+        ins, outs = (_mat(grad_out), _mat(x), _mat(w_gate), _mat(w_up)), (_mat(dx), _mat(dg), _mat(du))
+        _call(lib.maba_gated_ffn_backward, lib.maba_gated_ffn_backward_workspace_size, x, (*ins, act, *outs),
+              (*ins, *outs))
     return dx, dg, du
 
 
@@ -304,13 +306,15 @@ def b200_gated_ffn(
     (SwiGLUFFN without its down projection, which is ``b200_linear``).
     """
     act = _activation(activation, False)
-    _check_operands(x, (("w_gate", w_gate), ("w_up", w_up)))
-    N.require_cuda(x, op="gated_ffn")
+    n, k = _check_x(x, w_gate, "w_gate")
+    _check_weight(w_up, "w_up", x, n, k)
+    if not x.is_cuda:
+        N.require_cuda(x, op="gated_ffn")
     tracked = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
     if out is not None:
         if tracked or out.requires_grad:
             raise RuntimeError("gated_ffn: out= does not support automatic differentiation")
-        _check_side(out, "out", x, (*x.shape[:-1], w_gate.shape[0]), f32=False)
+        _check_side(out, "out", x, (*x.shape[:-1], n), f32=False)
         _check_out(out, x, out.shape, (("x", x), ("w_gate", w_gate), ("w_up", w_up)), None)
     if tracked:
         return _GatedFFNFunction.apply(x, w_gate, w_up, act)
@@ -329,8 +333,9 @@ def b200_gated_ffn_backward(
     ``needs`` says which are computed.  The projections are computed again from the inputs; their
     gradients are rounded to x's dtype between the products."""
     act = _activation(activation, False)
-    _check_operands(x, (("w_gate", w_gate), ("w_up", w_up)))
-    _check_side(grad_out, "grad_out", x, (*x.shape[:-1], w_gate.shape[0]), f32=False)
+    n, k = _check_x(x, w_gate, "w_gate")
+    _check_weight(w_up, "w_up", x, n, k)
+    _check_side(grad_out, "grad_out", x, (*x.shape[:-1], n), f32=False)
     N.require_cuda(x, op="gated_ffn_backward")
     return _gated_ffn_backward(grad_out, x, w_gate, w_up, act, tuple(bool(n) for n in needs))
 
