@@ -491,7 +491,11 @@ __global__ void __launch_bounds__(NTHR, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync();
+    if (CG == 2) {
+        // the last arrival that rank 0's products make on this CTA's barriers
+        if (rank == 1 && warp == W_MMA) mbar_wait_warp(&bars[B_DRAIN], 0, nullptr);
+        cluster_sync();
+    }
     if (warp == W_MMA) {
         tc_fence_after();
         if (CG == 2) tmem_dealloc_pair<TMEM_COLS>(tmem);
@@ -523,7 +527,7 @@ Plan plan_of(const Product& p) {
     const int64_t pairs = p.form == F_PAIR ? 2 : 1;
     Plan best;
     double least = 1e300;
-    for (int cg = 1; cg <= 1; ++cg) {
+    for (int cg = 1; cg <= 2; ++cg) {
         for (int bn = dual ? 64 : 32; bn <= (cg == 2 ? 256 : 192); bn += dual ? 64 : 32) {
             const int64_t tiles = ceil_div(p.M, 128 * cg) * ceil_div(p.N, dual ? bn / 2 : bn) * pairs;
             const int64_t slots = sm_count() / cg;
@@ -612,7 +616,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.ldp = ldp;
     // (before the maps: this call binds the device's context to the thread, which encoding a
     // map needs and autograd's threads may not have)
-    const Kernel kern = kernel_of<T, 1>(p);
+    const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p) : kernel_of<T, 1>(p);
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     CUtensorMap m[4];

@@ -42,12 +42,13 @@ def linear_case(m, k, n, dt, bias, scale, residual, seed=0, grad=None):
 SHAPES = [(1, 1, 1), (1, 64, 64), (1, 1248, 640), (3, 7, 5), (8, 640, 1544), (16, 33, 100), (17, 640, 1544), (33, 72, 24),
           (64, 1248, 640), (65, 130, 72), (128, 64, 128), (129, 641, 257), (300, 640, 1003), (513, 96, 2000),
           (1000, 2048, 136)]
+LARGE = [(2000, 264, 2056), (5003, 328, 520), (9001, 72, 250)]  # several tiles of a CTA pair per SM, ragged edges
 EPILOGUES = [("none", "none", "none", "none", None), ("silu", "f32", "none", "none", None),
              ("gelu", "same", "f32", "same", None), ("relu", "none", "same", "f32", F32), ("none", "none", "f32", "f32", F32)]
 
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
-@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("m,k,n", SHAPES + LARGE)
 def test_linear(m, k, n, dt):
     for i, (act, bias, scale, residual, out_dtype) in enumerate(EPILOGUES):
         t = linear_case(m, k, n, dt, bias, scale, residual, seed=i)
@@ -59,7 +60,7 @@ def test_linear(m, k, n, dt):
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 64, 64), (3, 7, 5), (40, 136, 72), (65, 130, 72), (129, 641, 257),
-                                   (300, 96, 1003), (2100, 200, 136)])
+                                   (300, 96, 1003), (2100, 200, 136)] + LARGE)
 def test_linear_backward(m, k, n, dt):
     for i, (act, bias, scale, _, out_dtype) in enumerate(EPILOGUES + [("none", "f32", "none", "none", F32)]):
         t = linear_case(m, k, n, dt, bias, scale, "none", seed=i, grad=out_dtype or dt)
@@ -72,7 +73,7 @@ def test_linear_backward(m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
-@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("m,k,n", SHAPES + LARGE)
 def test_gated_ffn(m, k, n, dt):
     g = gen(5)
     x, wg, wu = randn(g, m, k, dt=dt), randn(g, n, k, dt=dt, std=k ** -0.5), randn(g, n, k, dt=dt, std=k ** -0.5)
@@ -82,7 +83,7 @@ def test_gated_ffn(m, k, n, dt):
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 64, 64), (3, 7, 5), (40, 136, 72), (65, 130, 72), (129, 641, 257),
-                                   (300, 96, 1003), (2100, 200, 136)])
+                                   (300, 96, 1003), (2100, 200, 136)] + LARGE)
 def test_gated_ffn_backward(m, k, n, dt):
     g = gen(6)
     x, wg, wu = randn(g, m, k, dt=dt), randn(g, n, k, dt=dt, std=k ** -0.5), randn(g, n, k, dt=dt, std=k ** -0.5)
