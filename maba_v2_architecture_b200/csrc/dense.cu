@@ -52,6 +52,28 @@ __global__ void __launch_bounds__(256) copy_kernel(Side src, int64_t rows, int64
     }
 }
 
+// dst [3][rows][ld] (bf16) = x1, x2, x3 with x = x1 + x2 + x3: each the nearest bf16 of what
+// the ones before left, so the three hold all 24 bits of x (the largest finite float32 would
+// round to infinity: it is truncated).  An infinity or NaN is x1 alone.
+__global__ void __launch_bounds__(256)
+    planes_kernel(const float* __restrict__ src, int64_t sr, int64_t sc, int64_t rows, int64_t cols, __nv_bfloat16* dst,
+                  int64_t ld, int64_t plane) {
+    const int64_t n = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / cols, c = i - r * cols;
+        const float x = src[r * sr + c * sc];
+        __nv_bfloat16 x1 = __float2bfloat16_rn(x), x2 = __float2bfloat16_rn(0.f), x3 = x2;
+        if (isfinite(x)) {
+            if (!isfinite(__bfloat162float(x1))) x1 = __float2bfloat16_rz(x);
+            const float r1 = x - __bfloat162float(x1);
+            x2 = __float2bfloat16_rn(r1);
+            x3 = __float2bfloat16_rn(r1 - __bfloat162float(x2));
+        }
+        __nv_bfloat16* d = dst + r * ld + c;
+        d[0] = x1, d[plane] = x2, d[2 * plane] = x3;
+    }
+}
+
 // out = sum over splits of partial [splits][rows][ldp]; rows from `half` on go to out2
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -115,29 +137,19 @@ inline unsigned grid1d(int64_t n) {
 // ---------------------------------------------------------------------------
 // products
 // ---------------------------------------------------------------------------
-// Contraction splits of a plain product whose tiles do not fill the GPU; the partial sums
-// are float32 and added in split order.
-int simt_splits(const Product& p) {
-    if (p.e.kind != E_STORE) return 1;
-    const int64_t tiles = ceil_div(p.M, SIMT_ROWS) * ceil_div(p.N, 128) * (p.form == F_PAIR ? 2 : 1);
-    const int64_t steps = ceil_div(p.K, 16) * (p.form == F_SUM ? 2 : 1);
-    int64_t s = 2 * (int64_t)sm_count() / tiles;
-    if (s > steps / 16) s = steps / 16;
-    return (int)(s < 1 ? 1 : (s > 16 ? 16 : s));
-}
-
 int run(Ctx& c, const Product& p) {
     if (skinny_takes(p, c.dt)) {
         if (c.dry) return MABA_OK;
         return DENSE_DISPATCH(c.dt, [&] { return skinny_product<T>(p, c.s); });
     }
-    const int splits = c.dt == MABA_F32 ? simt_splits(p) : tc_splits(p);
+    // a plain product whose tiles do not fill the GPU splits its contraction; the partial
+    // sums are float32 and added in split order
+    const int splits = tc_splits(p, c.dt);
     const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
     float* partial = splits > 1 ? static_cast<float*>(c.ws.take((size_t)splits * rows * ldp * 4)) : nullptr;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        if constexpr (sizeof(T) == 4) MABA_TRY(simt_product<T>(p, splits, partial, ldp, c.s));
-        else MABA_TRY(tc_product<T>(p, partial, ldp, c.s));
+        MABA_TRY(tc_product<T>(p, partial, ldp, c.s));
         if (splits == 1) return (int)MABA_OK;
         sum_splits_kernel<T><<<grid1d(rows * p.N), 256, 0, c.s>>>(partial, ldp, splits, rows, p.N, static_cast<T*>(p.e.out),
                                                                   static_cast<T*>(p.e.out2), p.M, p.e.ldo);
@@ -229,19 +241,30 @@ Side side1(const maba_tensor* t) { return given(t) ? Side{t->data, 0, t->stride[
 // the operators
 // ---------------------------------------------------------------------------
 // A matrix as an operand.  The tensor-memory loads of the 16-bit products want rows on
-// 16-byte boundaries; what is not laid out so is copied once per call.  One copy serves
-// both directions of a matrix: K-major along its rows, MN-major across them.
-int operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
-    m = Matrix{t->data, t->stride[0], t->stride[1]};
-    if (c.dt == MABA_F32 || as_is) return MABA_OK;
-    const int64_t rows = t->shape[0], cols = t->shape[1];
-    if (t->dtype == c.dt && tc_readable(t->data, rows, cols, t->stride[0], t->stride[1])) return MABA_OK;
-    const int64_t ld = (cols + 7) / 8 * 8;
-    void* to = c.ws.take((size_t)rows * ld * 2);
-    m = Matrix{to, ld, 1};
-    return copy_matrix(c, side2(t), rows, cols, to, ld);
+// 16-byte boundaries; what is not laid out so is copied once per call, and a float32 matrix
+// is split into its planes.  One copy serves both directions of a matrix: K-major along its
+// rows, MN-major across them.
+int operand(Ctx& c, const Side& t, int64_t rows, int64_t cols, Matrix& m) {
+    m = Matrix{t.p, t.sr, t.sc, 0};
+    if (!t.f32 && tc_readable(t.p, rows, cols, t.sr, t.sc)) return MABA_OK;
+    const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
+    void* to = c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2);
+    m = Matrix{to, ld, 1, plane};
+    if (c.dt != MABA_F32) return copy_matrix(c, t, rows, cols, to, ld);
+    if (c.dry) return MABA_OK;
+    planes_kernel<<<grid1d(rows * cols), 256, 0, c.s>>>(static_cast<const float*>(t.p), t.sr, t.sc, rows, cols,
+                                                        static_cast<__nv_bfloat16*>(to), ld, plane);
+    return check_launch("dense(planes)");
 }
-Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr}; }
+int operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
+    m = Matrix{t->data, t->stride[0], t->stride[1], 0};
+    return as_is ? (int)MABA_OK : operand(c, side2(t), t->shape[0], t->shape[1], m);
+}
+// What an epilogue of this call wrote, [rows][ld] in the operands' type.
+int own_operand(Ctx& c, void* p, int64_t ld, int64_t rows, int64_t cols, Matrix& m) {
+    return operand(c, Side{p, ld, 1, c.dt == MABA_F32}, rows, cols, m);
+}
+Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr, m.sp}; }
 
 struct LinearArgs {
     const maba_tensor *x, *w, *bias, *scale, *res, *out;              // forward
@@ -304,7 +327,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
     }
     if (!need_dx && !need_dw && !need_db && !need_ds) return MABA_OK;
     const bool through = a.act == ACT_NONE && !given(a.scale);  // dz = g
-    const int64_t blocks = ceil_div(M, through ? CS_ROWS : (c.dt == MABA_F32 ? SIMT_ROWS : TC_ROWS));
+    const int64_t blocks = ceil_div(M, through ? CS_ROWS : TC_ROWS);
     float* pb = need_db ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     float* ps = need_ds ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     Matrix x, w, d;
@@ -323,7 +346,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         p.e.out = c.ws.take((size_t)M * ld * esize(c.dt)), p.e.ldo = ld;
         p.e.part_bias = pb, p.e.part_scale = ps;
         MABA_TRY(run(c, p));
-        d = Matrix{p.e.out, ld, 1};
+        if (need_dx || need_dw) MABA_TRY(own_operand(c, p.e.out, ld, M, N, d));
     } else {
         if (need_db) MABA_TRY(column_sums(c, side2(a.g), M, N, pb));
         // the products take one type: a float32 gradient is rounded to x's here
@@ -378,7 +401,9 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     p.e.out = c.ws.take((size_t)M * ld * esize(c.dt)), p.e.ldo = ld;
     p.e.out2 = c.ws.take((size_t)M * ld * esize(c.dt));
     MABA_TRY(run(c, p));
-    const Matrix d[2] = {{p.e.out, ld, 1}, {p.e.out2, ld, 1}};
+    Matrix d[2];
+    MABA_TRY(own_operand(c, p.e.out, ld, M, p.N, d[0]));
+    MABA_TRY(own_operand(c, p.e.out2, ld, M, p.N, d[1]));
     if (given(a.dx)) MABA_TRY(dx_product(c, M, p.N, 2, d, p.b, a.dx));
     const maba_tensor* dw[2] = {a.dwg, a.dwu};
     if (given(a.dwg) && given(a.dwu) && a.dwg->stride[0] == a.dwu->stride[0])

@@ -7,9 +7,7 @@
 //            dg = da * u * phi'(g);  du = da * phi(g);  dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x
 //
 // Every product of both operators is one Product: C[M,N] = A B^T summed in float32 over
-// the contraction index, with an epilogue on the float32 sums.  A and B are addressed by
-// two strides each (rows, contraction), so the transposed products of the backward pass
-// read x, W and dz where they are.
+// the contraction index, with an epilogue on the float32 sums.
 #pragma once
 #include "common.cuh"
 
@@ -34,9 +32,13 @@ enum EpiKind {
     E_STORE = 4,       // out = z, or float32 partial sums [split][M (2 M of F_PAIR)][N]
 };
 
+// An operand of a Product: 16-bit elements, or a float32 matrix as three bf16 planes
+// x = x1 + x2 + x3 (dense_tc.cu) that lie sp elements apart.  The few-row kernels read the
+// caller's float32 matrix itself.
 struct Matrix {
     const void* p = nullptr;
     int64_t sr = 0, sk = 0;  // element strides along the rows and along the contraction
+    int64_t sp = 0;
 };
 
 // A vector or a matrix that an epilogue reads: float32 or the operands' type, any strides.
@@ -98,18 +100,15 @@ template <typename T> __device__ __forceinline__ float side_at(const Side& s, in
 
 // Partial sums of a split product: float32 [split][rows][ldp], rows = M (2 M of F_PAIR).
 
-// dense_simt.cu: any type and any strides, CUDA cores; column sums per 128 rows.
-constexpr int SIMT_ROWS = 128;
-template <typename T> int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s);
-
 // dense_skinny.cu: forward products of few rows, any strides.
 bool skinny_takes(const Product& p, int dt);
 template <typename T> int skinny_product(const Product& p, cudaStream_t s);
 
-// dense_tc.cu: 16-bit operands that tc_readable() accepts, tensor cores; column sums per 32 rows.
+// dense_tc.cu: tensor cores.  Operands as tc_readable() accepts them (float32: as planes);
+// column sums per TC_ROWS rows; T is the type of what the epilogue reads and writes.
 constexpr int TC_ROWS = 32;
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
-int tc_splits(const Product& p);
+int tc_splits(const Product& p, int dt);
 template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);
 

@@ -1,4 +1,17 @@
-// Products of 16-bit operands on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
+// Products on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
+//
+// 16-bit operands are multiplied as they are.  A float32 operand is three bf16 planes,
+// x = x1 + x2 + x3 exactly, |x2| <= 2^-8 |x|, |x3| <= 2^-16 |x|; of the nine products the
+// six down to 2^-16 are taken, x1 w1 into one accumulator, x1 w2 + x2 w1 + x2 w2 + x1 w3 +
+// x3 w1 into a second, and what is left out is below 2^-23 of |x w|: float32's own rounding,
+// at six tensor products instead of the CUDA cores' one (where main is an infinity or NaN the
+// second sum, which may hold inf * 0, is not added).
+//
+// The tensor cores truncate when they add to their float32 accumulator, once per 16
+// contraction indices: a sum over K loses about K 5.6e-10 of itself toward zero (measured
+// 6e-7 relative at K = 640, 4.4e-6 at 4,096).  That is far below a 16-bit result's rounding,
+// but not below a float32 result's, so sums that end in float32 (MODE 1 and 2) leave TMEM
+// every 512 (256) indices and are added, rounded to nearest, in the epilogue's registers.
 //
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
@@ -39,7 +52,7 @@ constexpr int MAX_STAGES = 8;
 constexpr uint32_t STAGING = 32 * 128;  // one warp's 32 x 32 float32 chunk
 constexpr uint32_t TAIL = EPI_WARPS * STAGING + EPI_WARPS * 2 * 32 * 4 + 256;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
-constexpr int TMEM_COLS = 512, ACC_COLS = 256;
+constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
 
 enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2, N_BARS };
 static_assert(N_BARS * 8 + 8 <= 256, "barrier area");
@@ -49,8 +62,9 @@ struct TcArgs {
     int kblocks, kseg;  // contraction blocks over all segments, and of one
     int tiles_n, splits, pairs, units, dual;
     int bn, b_rows;  // columns of the MMA, rows of B per CTA
+    int flush;       // contraction blocks between two readings of the accumulator
     int stages;
-    uint32_t stage_bytes, load_bytes;  // load_bytes: what one stage's barrier receives
+    uint32_t stage_bytes, b_at, b_bytes, load_bytes;  // B's place in a stage, one plane of it, bytes per stage
     uint32_t idesc;
     int side_vec, out_vec;
     Epilogue e;
@@ -75,14 +89,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// phi and phi' on the SFU's exponential and reciprocal: a few float32 ulp, and the results
-// are rounded to 16 bits or come from sums of 16-bit products.
-template <int ACT> __device__ __forceinline__ float act16(float z) {
-    if (ACT == ACT_SILU) return silu_f(z);
+// phi and phi' of 16-bit operands on the SFU's exponential and reciprocal (a few float32
+// ulp); of float32 ones (EXACT) as dense.cuh has them.
+template <int ACT, bool EXACT> __device__ __forceinline__ float act16(float z) {
+    if (ACT == ACT_SILU && !EXACT) return silu_f(z);
     return act_f(z, ACT);
 }
-template <int ACT> __device__ __forceinline__ void act_grad16(float z, float& y, float& d) {
-    if (ACT == ACT_SILU) {
+template <int ACT, bool EXACT> __device__ __forceinline__ void act_grad16(float z, float& y, float& d) {
+    if (ACT == ACT_SILU && !EXACT) {
         const float s = sigmoid_f(z);
         y = z * s;
         d = s * (1.f + z * (1.f - s));
@@ -100,61 +114,66 @@ template <typename F> __device__ __forceinline__ void with_act(int act, F f) {
 // --------------------------------------------------------------------------
 // 32 x 32 chunks between global memory (a warp's lanes along the rows) and registers (lane
 // = row), through the warp's staging area; 16-byte pieces are swizzled so that both
-// directions are free of bank conflicts.
+// directions are free of bank conflicts.  A chunk that lies inside the matrix and on 16-byte
+// boundaries moves in 16-byte pieces with one address and constant steps (the epilogue is
+// bound by its instruction count); the others go element by element, out of line.
 // --------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void fetch_chunk(uint4* v, const Side& s, bool vec, int64_t row0, int64_t col0, int64_t M,
-                                            int64_t N, int lane) {
-    if (s.f32) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t r = row0 + i * 4 + (lane >> 3), c = col0 + (lane & 7) * 4;
-            float t[4] = {0.f, 0.f, 0.f, 0.f};
-            const float* p = static_cast<const float*>(s.p) + r * s.sr + c * s.sc;
-            if (r < M) {
-                if (vec && c + 4 <= N) *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(p);
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c + e < N) t[e] = p[e * s.sc];
-            }
-            v[i] = *reinterpret_cast<uint4*>(t);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
-            uint32_t t[4] = {0u, 0u, 0u, 0u};
-            const uint16_t* p = static_cast<const uint16_t*>(s.p) + r * s.sr + c * s.sc;
-            if (r < M) {
-                if (vec && c + 8 <= N) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < N) t[e >> 1] |= (uint32_t)p[e * s.sc] << (16 * (e & 1));
-            }
-            v[i] = *reinterpret_cast<uint4*>(t);
-        }
-    }
-}
 __device__ __forceinline__ uint4* at32(unsigned char* st, int row, int piece) {
     return reinterpret_cast<uint4*>(st + row * 128 + ((piece ^ (row & 7)) << 4));
 }
 __device__ __forceinline__ uint4* at16(unsigned char* st, int row, int piece) {
     return reinterpret_cast<uint4*>(st + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
 }
-template <typename T>
-__device__ __forceinline__ void chunk_to_rows(float* x, const uint4* v, bool f32, unsigned char* st, int lane) {
-    __syncwarp();
-    if (f32) {
+struct Chunk {
+    int64_t row0, col0;
+    int rows, cols;  // of 32, inside the matrix
+};
+
+template <typename E> __device__ __forceinline__ E* element(unsigned char* st, int r, int c) {
+    return sizeof(E) == 4 ? reinterpret_cast<E*>(at32(st, r, c >> 2)) + (c & 3)
+                          : reinterpret_cast<E*>(at16(st, r, c >> 3)) + (c & 7);
+}
+// (src, dst: the chunk's first element)
+template <typename E>
+__device__ __noinline__ void stage_in(unsigned char* st, const E* src, int64_t sr, int64_t sc, int rows, int cols, int lane) {
+    for (int r = 0; r < 32; ++r) *element<E>(st, r, lane) = r < rows && lane < cols ? src[r * sr + lane * sc] : E(0);
+}
+template <typename E>
+__device__ __noinline__ void stage_out(unsigned char* st, E* dst, int64_t ld, int rows, int cols, int lane) {
+    for (int r = 0; r < rows; ++r)
+        if (lane < cols) dst[r * ld + lane] = *element<E>(st, r, lane);
+}
+
+// The pieces of a whole chunk, in flight in registers (8 of float32, 4 of 16 bits).
+template <int EL> __device__ __forceinline__ void fetch_pieces(uint4* v, const Side& s, const Chunk& k, int lane) {
+    constexpr int PER = 32 * EL / 16, N = 32 * PER / 32;  // pieces per row, pieces per lane
+    const unsigned char* p = static_cast<const unsigned char*>(s.p) +
+                             ((k.row0 + lane / PER) * s.sr + k.col0) * EL + (lane % PER) * 16;
+    const int64_t step = s.sr * (EL * (32 / PER));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *at32(st, i * 4 + (lane >> 3), lane & 7) = v[i];
+    for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * step);
+}
+template <typename T>
+__device__ __forceinline__ void pieces_to_rows(float* x, const uint4* v, bool f32, bool whole, const Side& s, const Chunk& k,
+                                               unsigned char* st, int lane) {
+    __syncwarp();
+    if (sizeof(T) == 4 || f32) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *at32(st, i * 4 + (lane >> 3), lane & 7) = v[i];
+        } else {
+            stage_in<float>(st, static_cast<const float*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols, lane);
+        }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(x + 4 * i) = *at32(st, lane, i);
-    } else {
+    } else if constexpr (sizeof(T) == 2) {
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *at16(st, i * 8 + (lane >> 2), lane & 3) = v[i];
+            for (int i = 0; i < 4; ++i) *at16(st, i * 8 + (lane >> 2), lane & 3) = v[i];
+        } else {
+            stage_in<uint16_t>(st, static_cast<const uint16_t*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols, lane);
+        }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -168,49 +187,44 @@ __device__ __forceinline__ void chunk_to_rows(float* x, const uint4* v, bool f32
         }
     }
 }
+template <int EL>
+__device__ __forceinline__ void store_pieces(unsigned char* st, void* out, int64_t ld, const Chunk& k, int lane) {
+    constexpr int PER = 32 * EL / 16, N = 32 * PER / 32, RS = 32 / PER;
+    unsigned char* p = static_cast<unsigned char*>(out) + ((k.row0 + lane / PER) * ld + k.col0) * EL + (lane % PER) * 16;
+    const int64_t step = ld * (EL * RS);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        *reinterpret_cast<uint4*>(p + i * step) =
+            EL == 4 ? *at32(st, i * RS + lane / PER, lane % PER) : *at16(st, i * RS + lane / PER, lane % PER);
+}
 template <typename T>
-__device__ __forceinline__ void store_rows(const float* x, void* out, bool f32, int64_t ld, bool vec, int64_t row0,
-                                           int64_t col0, int64_t M, int64_t N, unsigned char* st, int lane) {
+__device__ __forceinline__ void store_rows(const float* x, void* out, bool f32, int64_t ld, bool vec, const Chunk& k,
+                                           unsigned char* st, int lane) {
+    const bool whole = vec && k.rows == 32 && k.cols == 32;
     __syncwarp();
-    if (f32) {
+    if (sizeof(T) == 4 || f32) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             *reinterpret_cast<float4*>(at32(st, lane, i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t r = row0 + i * 4 + (lane >> 3), c = col0 + (lane & 7) * 4;
-            const uint4 q = *at32(st, i * 4 + (lane >> 3), lane & 7);
-            if (r >= M) continue;
-            float* p = static_cast<float*>(out) + r * ld + c;
-            if (vec && c + 4 <= N) *reinterpret_cast<uint4*>(p) = q;
-            else {
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < N) p[e] = __uint_as_float(w[e]);
-            }
-        }
-    } else {
+        if (whole) store_pieces<4>(st, out, ld, k, lane);
+        else stage_out<float>(st, static_cast<float*>(out) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *at16(st, lane, i) = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]),
                                             pack2<T>(x[8 * i + 4], x[8 * i + 5]), pack2<T>(x[8 * i + 6], x[8 * i + 7]));
         __syncwarp();
+        if (whole) store_pieces<2>(st, out, ld, k, lane);
+        else stage_out<uint16_t>(st, static_cast<uint16_t*>(out) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
+    }
+}
+// x op= the 32 values of a shared vector
+template <typename F> __device__ __forceinline__ void with_vector(float* x, const float* v, F f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
-            const uint4 q = *at16(st, i * 8 + (lane >> 2), lane & 3);
-            if (r >= M) continue;
-            uint16_t* p = static_cast<uint16_t*>(out) + r * ld + c;
-            if (vec && c + 8 <= N) *reinterpret_cast<uint4*>(p) = q;
-            else {
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < N) p[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-            }
-        }
+    for (int j = 0; j < 32; j += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(v + j);
+        f(x[j], q.x), f(x[j + 1], q.y), f(x[j + 2], q.z), f(x[j + 3], q.w);
     }
 }
 // Sums of 32 columns over the warp's 32 rows, in a fixed tree; lane l returns column l's.
@@ -227,7 +241,7 @@ __device__ __forceinline__ float column_sum(float* v, int lane) {
     return v[0];
 }
 
-template <typename T, int CG, bool A_MN, bool B_MN, int KIND>
+template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE>
 __global__ void __launch_bounds__(NTHR, 1)
     tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap ta0, const __grid_constant__ CUtensorMap ta1,
               const __grid_constant__ CUtensorMap tb0, const __grid_constant__ CUtensorMap tb1) {
@@ -240,6 +254,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* abort_f = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+    constexpr int PLANES = MODE == 2 ? 3 : 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
@@ -294,35 +309,38 @@ __global__ void __launch_bounds__(NTHR, 1)
                 const int seg = kb >= a.kseg ? 1 : 0, k0 = (kb - seg * a.kseg) * BK;
                 const CUtensorMap* ma = (a.pairs == 2 ? t.pair : seg) ? &ta1 : &ta0;
                 unsigned char* sa = base + st * a.stage_bytes;
-                unsigned char* sb = sa + A_BYTES;
                 if (elect_one()) {
                     uint64_t* full = &bars[B_FULL + st];
                     const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : 0u;
-                    auto load = [&](unsigned char* dst, const CUtensorMap* m, int x, int y) {
-                        if (CG == 2) tma_load_2d_pair(dst, m, full0, x, y);
-                        else tma_load_2d(dst, m, full, x, y);
+                    auto load = [&](unsigned char* dst, const CUtensorMap* m, int x, int y, int plane) {
+                        if (CG == 2) tma_load_3d_pair(dst, m, full0, x, y, plane);
+                        else tma_load_3d(dst, m, full, x, y, plane);
                     };
                     if (rank == 0) mbar_arrive_expect_tx(full, a.load_bytes);
-                    if (A_MN) {
-                        load(sa, ma, (int)t.m0, k0);
-                        load(sa + A_BYTES / 2, ma, (int)t.m0 + 64, k0);
-                    } else {
-                        load(sa, ma, k0, (int)t.m0);
-                    }
-                    if (KIND == E_GLU || KIND == E_GLU_BWD) {
-                        if (CG == 2) {
-                            load(sb, rank ? &tb1 : &tb0, k0, (int)t.n0);
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; ++pl, sa += A_BYTES) {
+                        unsigned char* sb = base + st * a.stage_bytes + a.b_at + pl * a.b_bytes;
+                        if (A_MN) {
+                            load(sa, ma, (int)t.m0, k0, pl);
+                            load(sa + A_BYTES / 2, ma, (int)t.m0 + 64, k0, pl);
                         } else {
-                            load(sb, &tb0, k0, (int)t.n0);
-                            load(sb + a.bn / 2 * 128, &tb1, k0, (int)t.n0);
+                            load(sa, ma, k0, (int)t.m0, pl);
                         }
-                    } else {
-                        const CUtensorMap* mb = seg ? &tb1 : &tb0;
-                        const int y = (int)t.n0 + (int)rank * a.b_rows;
-                        if (B_MN) {
-                            for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0);
+                        if (KIND == E_GLU || KIND == E_GLU_BWD) {
+                            if (CG == 2) {
+                                load(sb, rank ? &tb1 : &tb0, k0, (int)t.n0, pl);
+                            } else {
+                                load(sb, &tb0, k0, (int)t.n0, pl);
+                                load(sb + a.bn / 2 * 128, &tb1, k0, (int)t.n0, pl);
+                            }
                         } else {
-                            load(sb, mb, k0, y);
+                            const CUtensorMap* mb = seg ? &tb1 : &tb0;
+                            const int y = (int)t.n0 + (int)rank * a.b_rows;
+                            if (B_MN) {
+                                for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0, pl);
+                            } else {
+                                load(sb, mb, k0, y, pl);
+                            }
                         }
                     }
                 }
@@ -337,36 +355,50 @@ __global__ void __launch_bounds__(NTHR, 1)
         // ============================ MMA issuer ==============================
         if (rank == 0) {
             const uint64_t ad0 = sdesc_sw128(smem_addr(base), A_MN ? A_BYTES / 2 : 16, 1024);
-            const uint64_t bd0 = sdesc_sw128(smem_addr(base + A_BYTES), B_MN ? 8192 : 16, 1024);
+            const uint64_t bd0 = sdesc_sw128(smem_addr(base + a.b_at), B_MN ? 8192 : 16, 1024);
             constexpr uint32_t ak = A_MN ? 2048 >> 4 : 32 >> 4, bk = B_MN ? 2048 >> 4 : 32 >> 4;
-            int it = 0, i = 0;
+            auto mma = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t acc) {
+                if (CG == 2) umma_f16_ss_pair_elect(d, ad, bd, a.idesc, acc);
+                else umma_f16_ss_elect(d, ad, bd, a.idesc, acc);
+            };
+            int it = 0, i = 0;  // i: accumulations begun
             bool ok = true;
-            for (int u = worker; u < a.units && ok; u += workers, ++i) {
+            for (int u = worker; u < a.units && ok; u += workers) {
                 const Unit t = unit_of(u);
-                const int buf = i & 1;
-                if (i >= 2) ok = mbar_wait_warp(&bars[B_TEMPTY + buf], ((i >> 1) - 1) & 1, abort_f);
-                if (!ok) break;
-                tc_fence_after();
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    const int st = it % a.stages;
-                    ok = mbar_wait_warp(&bars[B_FULL + st], (it / a.stages) & 1, abort_f);
+                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush, ++i) {
+                    const int buf = i & 1, f1 = f0 + a.flush < t.kb1 ? f0 + a.flush : t.kb1;
+                    const uint32_t d = tmem + buf * ACC_COLS;
+                    if (i >= 2) ok = mbar_wait_warp(&bars[B_TEMPTY + buf], ((i >> 1) - 1) & 1, abort_f);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t so = (uint64_t)(st * (a.stage_bytes >> 4));
+                    for (int kb = f0; kb < f1; ++kb, ++it) {
+                        const int st = it % a.stages;
+                        ok = mbar_wait_warp(&bars[B_FULL + st], (it / a.stages) & 1, abort_f);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t so = (uint64_t)(st * (a.stage_bytes >> 4));
+                        const uint64_t ad = ad0 + so, bd = bd0 + so;
+                        const uint64_t bp = a.b_bytes >> 4;  // from one plane of B to the next
+                        constexpr uint64_t ap = A_BYTES >> 4;
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k) {
-                        const uint32_t acc = kb > t.kb0 || k > 0 ? 1u : 0u;
-                        if (CG == 2)
-                            umma_f16_ss_pair_elect(tmem + buf * ACC_COLS, ad0 + so + k * ak, bd0 + so + k * bk, a.idesc, acc);
-                        else
-                            umma_f16_ss_elect(tmem + buf * ACC_COLS, ad0 + so + k * ak, bd0 + so + k * bk, a.idesc, acc);
+                        for (int k = 0; k < BK / 16; ++k) {
+                            const uint32_t acc = kb > f0 || k > 0 ? 1u : 0u;
+                            mma(d, ad + k * ak, bd + k * bk, acc);
+                            if (PLANES == 3) {
+                                mma(d + MINOR, ad + k * ak, bd + k * bk + 2 * bp, acc);
+                                mma(d + MINOR, ad + k * ak + 2 * ap, bd + k * bk, 1u);
+                                mma(d + MINOR, ad + k * ak + ap, bd + k * bk + bp, 1u);
+                                mma(d + MINOR, ad + k * ak, bd + k * bk + bp, 1u);
+                                mma(d + MINOR, ad + k * ak + ap, bd + k * bk, 1u);
+                            }
+                        }
+                        if (CG == 2) umma_commit_pair_elect(&bars[B_EMPTY + st]);
+                        else umma_commit_elect(&bars[B_EMPTY + st]);
                     }
-                    if (CG == 2) umma_commit_pair_elect(&bars[B_EMPTY + st]);
-                    else umma_commit_elect(&bars[B_EMPTY + st]);
+                    if (!ok) break;
+                    if (CG == 2) umma_commit_pair_elect(&bars[B_TFULL + buf]);
+                    else umma_commit_elect(&bars[B_TFULL + buf]);
                 }
-                if (!ok) break;
-                if (CG == 2) umma_commit_pair_elect(&bars[B_TFULL + buf]);
-                else umma_commit_elect(&bars[B_TFULL + buf]);
             }
             // every product has completed before TMEM is freed
             if (CG == 2) umma_commit_pair_elect(&bars[B_DRAIN]);
@@ -375,7 +407,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         }
     } else {
         // ============================== epilogue ==============================
-        constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD;
+        constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
+        constexpr int CH = MODE == 0 ? 1 : (DUAL ? 1 : 2);  // chunks whose sums a warp of MODE 1, 2 holds
         const int q = warp & 3, h = warp >> 2;
         unsigned char* st = tail + warp * STAGING;
         float* vscale = vecs + warp * 64;
@@ -383,37 +416,92 @@ __global__ void __launch_bounds__(NTHR, 1)
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
         const bool has_side = KIND != E_STORE && KIND != E_GLU && e.res.p != nullptr;
-        int i = 0;
-        for (int u = worker; u < a.units; u += workers, ++i) {
+        int i = 0;  // accumulations read
+        auto released = [&](int buf) {  // this warp has read its part of the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 2) mbar_arrive_cluster(cluster_addr(&bars[B_TEMPTY + buf], 0));
+                else mbar_arrive(&bars[B_TEMPTY + buf]);
+            }
+        };
+        bool ok = true;
+        for (int u = worker; u < a.units; u += workers) {
             const Unit t = unit_of(u);
-            const int buf = i & 1;
             const int64_t row0 = t.m0 + q * 32;
             const bool live = row0 < a.M;
             uint4 side[8];
             float ps = 0.f, pb = 0.f;  // this lane's column of scale and bias
+            auto place = [&](int c) {
+                Chunk k;
+                k.row0 = row0, k.col0 = t.n0 + c * 32;
+                k.rows = a.M - row0 < 32 ? (int)(a.M - row0) : 32;
+                k.cols = a.N - k.col0 < 32 ? (int)(a.N - k.col0) : 32;
+                return k;
+            };
+            auto side_whole = [&](const Chunk& k) { return a.side_vec && k.rows == 32 && k.cols == 32; };
             auto fetch = [&](int c) {
-                const int64_t col0 = t.n0 + c * 32;
-                if (has_side) fetch_chunk<T>(side, e.res, a.side_vec, row0, col0, a.M, a.N, lane);
+                const Chunk k = place(c);
+                if (has_side && side_whole(k)) {
+                    if (sizeof(T) == 4 || e.res.f32) fetch_pieces<4>(side, e.res, k, lane);
+                    else fetch_pieces<2>(side, e.res, k, lane);
+                }
                 if (KIND == E_LINEAR || KIND == E_LINEAR_BWD) {
-                    const bool in = col0 + lane < a.N;
-                    ps = in && e.scale.p ? side_at<T>(e.scale, 0, col0 + lane) : 1.f;
-                    pb = in && e.bias.p ? side_at<T>(e.bias, 0, col0 + lane) : 0.f;
+                    if (e.scale.p) ps = lane < k.cols ? side_at<T>(e.scale, 0, k.col0 + lane) : 1.f;
+                    if (e.bias.p) pb = lane < k.cols ? side_at<T>(e.bias, 0, k.col0 + lane) : 0.f;
                 }
             };
-            if (live && h * 32 < width) fetch(h);
-            if (!mbar_wait_warp(&bars[B_TFULL + buf], (i >> 1) & 1, abort_f)) break;
-            tc_fence_after();
-            const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
-            for (int c = h; c * 32 < width; c += 2) {
-                const int64_t col0 = t.n0 + c * 32;
-                float z[32], w[DUAL ? 32 : 1];
-                tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
-                if (DUAL) tmem_ld32(acc + width + c * 32, reinterpret_cast<uint32_t*>(w));
-                tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
-                if (DUAL) tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(w));
-                if (!live || col0 >= a.N) continue;
+            if (!MODE && live && h * 32 < width) fetch(h);
+            // MODE 1, 2: the accumulations of the unit, added up
+            float sz[MODE ? CH : 1][32], sw[MODE && DUAL ? 32 : 1];
+            if (MODE) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+#pragma unroll
+                    for (int cc = 0; cc < CH; ++cc) sz[cc][j] = 0.f;
+                    if (DUAL) sw[j] = 0.f;
+                }
+                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush, ++i) {
+                    const int buf = i & 1;
+                    ok = mbar_wait_warp(&bars[B_TFULL + buf], (i >> 1) & 1, abort_f);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
+                    auto add = [&](float* sum, int col) {
+                        float z[32];
+                        tmem_ld32(acc + col, reinterpret_cast<uint32_t*>(z));
+                        if (MODE == 2) {
+                            float y[32];
+                            tmem_ld32(acc + MINOR + col, reinterpret_cast<uint32_t*>(y));
+                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
+                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(y));
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[j] += isfinite(z[j]) ? z[j] + y[j] : z[j];
+                        } else {
+                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[j] += z[j];
+                        }
+                    };
+#pragma unroll
+                    for (int cc = 0; cc < CH; ++cc)
+                        if ((h + 2 * cc) * 32 < width) add(sz[cc], (h + 2 * cc) * 32);
+                    if (DUAL && h * 32 < width) add(sw, width + h * 32);
+                    released(buf);
+                }
+                if (!ok) break;
+                if (live && h * 32 < width) fetch(h);  // (here, or its registers would live through the sums)
+            } else {
+                ok = mbar_wait_warp(&bars[B_TFULL + (i & 1)], (i >> 1) & 1, abort_f);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const uint32_t acc = tmem + (i & 1) * ACC_COLS + ((uint32_t)(q * 32) << 16);
+            auto chunk = [&](int c, float* z, float* w) {
+                const Chunk k = place(c);
+                if (!live || k.cols <= 0) return;
                 float g[32];
-                if (has_side) chunk_to_rows<T>(g, side, e.res.f32, st, lane);
+                if (has_side) pieces_to_rows<T>(g, side, e.res.f32, side_whole(k), e.res, k, st, lane);
                 if (KIND == E_LINEAR || KIND == E_LINEAR_BWD) {
                     __syncwarp();
                     vscale[lane] = ps;
@@ -422,69 +510,85 @@ __global__ void __launch_bounds__(NTHR, 1)
                 }
                 if ((c + 2) * 32 < width) fetch(c + 2);
                 if (KIND == E_STORE) {
-                    const int64_t rows = a.pairs * a.M;
                     if (a.splits > 1)
-                        store_rows<T>(z, a.partial + ((int64_t)t.split * rows + t.pair * a.M) * a.ldp, true, a.ldp, true, row0,
-                                      col0, a.M, a.N, st, lane);
+                        store_rows<T>(z, a.partial + ((int64_t)t.split * a.pairs + t.pair) * a.M * a.ldp, true, a.ldp, true, k,
+                                      st, lane);
                     else
-                        store_rows<T>(z, t.pair ? e.out2 : e.out, false, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
+                        store_rows<T>(z, t.pair ? e.out2 : e.out, false, e.ldo, a.out_vec, k, st, lane);
                 } else if (KIND == E_LINEAR) {
+                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
                     with_act(e.act, [&](auto A) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            z[j] = act16<A.value>(z[j] + vbias[j]) * vscale[j];
-                            if (has_side) z[j] += g[j];
-                        }
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
                     });
-                    store_rows<T>(z, e.out, e.out_f32, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
+                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
+                    if (has_side) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] += g[j];
+                    }
+                    store_rows<T>(z, e.out, e.out_f32, e.ldo, a.out_vec, k, st, lane);
                 } else if (KIND == E_LINEAR_BWD) {
                     float y[32];
-                    const bool in = row0 + lane < a.M;  // rows past the last: no part in the sums
+                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
                     with_act(e.act, [&](auto A) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             float f, d;
-                            act_grad16<A.value>(z[j] + vbias[j], f, d);
-                            z[j] = in ? g[j] * vscale[j] * d : 0.f;
-                            y[j] = in ? g[j] * f : 0.f;
+                            act_grad16<A.value, EXACT>(z[j], f, d);
+                            z[j] = g[j] * d;
+                            y[j] = g[j] * f;
                         }
                     });
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
-                    const int64_t at = (row0 >> 5) * a.N + col0 + lane;
+                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
+                    if (k.rows < 32 && lane >= k.rows) {  // no part in the sums, whatever the bias is
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] = y[j] = 0.f;
+                    }
+                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
+                    const int64_t at = (row0 >> 5) * a.N + k.col0 + lane;
                     if (e.part_bias) {
                         const float s = column_sum(z, lane);
-                        if (col0 + lane < a.N) e.part_bias[at] = s;
+                        if (lane < k.cols) e.part_bias[at] = s;
                     }
                     if (e.part_scale) {
                         const float s = column_sum(y, lane);
-                        if (col0 + lane < a.N) e.part_scale[at] = s;
+                        if (lane < k.cols) e.part_scale[at] = s;
                     }
                 } else if (KIND == E_GLU) {
                     with_act(e.act, [&](auto A) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value>(z[j]) * w[j];
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
                     });
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
+                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
                 } else {
                     with_act(e.act, [&](auto A) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             float f, d;
-                            act_grad16<A.value>(z[j], f, d);
+                            act_grad16<A.value, EXACT>(z[j], f, d);
                             z[j] = g[j] * w[j] * d;
                             w[j] = g[j] * f;
                         }
                     });
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
-                    store_rows<T>(w, e.out2, false, e.ldo, a.out_vec, row0, col0, a.M, a.N, st, lane);
+                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
+                    store_rows<T>(w, e.out2, false, e.ldo, a.out_vec, k, st, lane);
                 }
-            }
-            // this warp has read its part of the accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) mbar_arrive_cluster(cluster_addr(&bars[B_TEMPTY + buf], 0));
-                else mbar_arrive(&bars[B_TEMPTY + buf]);
+            };
+            if (MODE) {
+#pragma unroll
+                for (int cc = 0; cc < CH; ++cc)
+                    if ((h + 2 * cc) * 32 < width) chunk(h + 2 * cc, sz[cc], sw);
+            } else {
+                for (int c = h; c * 32 < width; c += 2) {
+                    float z[32], w[DUAL ? 32 : 1];
+                    tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
+                    if (DUAL) tmem_ld32(acc + width + c * 32, reinterpret_cast<uint32_t*>(w));
+                    tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
+                    if (DUAL) tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(w));
+                    chunk(c, z, w);
+                }
+                released(i & 1);
+                ++i;
             }
         }
     }
@@ -517,43 +621,56 @@ inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
     return (uint32_t)(mn ? (r + 63) / 64 * 64 : r) * 128u;
 }
 
+// How a product's sums are kept: 0 one accumulation, 1 added up in registers every 512
+// indices (float32 results of 16-bit operands), 2 float32 operands, every 256.
+int mode_of(const Product& p, int dt) {
+    if (dt == MABA_F32) return 2;
+    return p.e.kind == E_LINEAR && p.e.out_f32 && p.K > 512 ? 1 : 0;
+}
+
 // The tile and the splits with the least estimated time.  Per k-block and SM: the larger of
 // the products (128 x bn x 64 at 4,096 per cycle) and the loads (60 bytes per cycle from L2);
-// a unit that is not hidden under another adds its fill and epilogue.
-Plan plan_of(const Product& p) {
+// a unit that is not hidden under another adds its fill and epilogue.  The registers that
+// hold a unit's sums bound bn in modes 1 and 2.  Splits also bound what one accumulation
+// truncates: at most 16,384 indices.
+Plan plan_of(const Product& p, int mode) {
     const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE;
     const bool b_mn = store;
     const int64_t kblocks = ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
     const int64_t pairs = p.form == F_PAIR ? 2 : 1;
+    const int planes = mode == 2 ? 3 : 1, terms = mode == 2 ? 6 : 1;
+    int64_t fewest = store && mode == 0 ? ceil_div(kblocks, 256) : 1;
     Plan best;
     double least = 1e300;
     for (int cg = 1; cg <= 2; ++cg) {
-        for (int bn = dual ? 64 : 32; bn <= (cg == 2 ? 256 : 192); bn += dual ? 64 : 32) {
+        const int most = mode ? 128 : (cg == 2 ? 256 : 192);
+        for (int bn = dual ? 64 : 32; bn <= most; bn += dual ? 64 : 32) {
             const int64_t tiles = ceil_div(p.M, 128 * cg) * ceil_div(p.N, dual ? bn / 2 : bn) * pairs;
             const int64_t slots = sm_count() / cg;
-            const double mma = 2.0 * bn, load = (A_BYTES + b_bytes_of(cg, bn, b_mn)) / 60.0;
+            const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, b_mn)) / 60.0;
             const double kcost = mma > load ? mma : load;
-            for (int splits = 1; splits <= (store ? 16 : 1) && splits <= kblocks; ++splits) {
+            for (int64_t splits = fewest; splits <= (store ? fewest + 15 : 1) && splits <= kblocks; ++splits) {
                 const int64_t units = tiles * splits;
                 const double waves = (double)ceil_div(units, slots);
                 const double kb = (double)ceil_div(kblocks, splits);
                 double t = waves * kb * kcost + 2000.0 + 12.0 * bn;
                 // the partial sums, written and read: bytes at ~3,500 per cycle over the GPU, and a launch
                 if (splits > 1) t += 2000.0 + 8.0 * (double)splits * pairs * p.M * p.N / 3500.0;
-                if (t < least) least = t, best = Plan{cg, bn, splits};
+                if (t < least) least = t, best = Plan{cg, bn, (int)splits};
             }
         }
     }
     return best;
 }
 
-// One operand's map: rows x contraction, read K-major (contraction contiguous) or MN-major.
-bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int64_t rows, int64_t k, bool mn, int box_rows) {
-    const int64_t dims[2] = {mn ? rows : k, mn ? k : rows};
-    const int64_t outer = mn ? x.sk : x.sr;
-    const int64_t stride[1] = {dims[1] > 1 ? outer : (dims[0] + 7) / 8 * 8};
-    const uint32_t box[2] = {(uint32_t)BK, (uint32_t)(mn ? BK : box_rows)};
-    return make_map(m, dt, x.p, 2, dims, stride, box);
+// One operand's map: rows x contraction (x planes), read K-major (contraction contiguous) or
+// MN-major.
+bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int planes, int64_t rows, int64_t k, bool mn, int box_rows) {
+    const int64_t dims[3] = {mn ? rows : k, mn ? k : rows, planes};
+    const int64_t ld = dims[1] > 1 ? (mn ? x.sk : x.sr) : (dims[0] + 7) / 8 * 8;
+    const int64_t strides[2] = {ld, planes > 1 ? x.sp : ld};
+    const uint32_t box[3] = {(uint32_t)BK, (uint32_t)(mn ? BK : box_rows), 1};
+    return make_map(m, dt, x.p, 3, dims, strides, box);
 }
 
 bool aligned16(const void* p, int64_t ld, int el) {
@@ -562,13 +679,16 @@ bool aligned16(const void* p, int64_t ld, int el) {
 
 using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap);
 
-template <typename T, int CG> Kernel kernel_of(const Product& p) {
+template <typename T, int CG> Kernel kernel_of(const Product& p, int mode) {
+    constexpr int M = sizeof(T) == 4 ? 2 : 0;
+    if constexpr (M == 0)
+        if (mode == 1) return tc_kernel<T, CG, false, false, E_LINEAR, 1>;
     switch (p.e.kind) {
-        case E_LINEAR: return tc_kernel<T, CG, false, false, E_LINEAR>;
-        case E_LINEAR_BWD: return tc_kernel<T, CG, false, false, E_LINEAR_BWD>;
-        case E_GLU: return tc_kernel<T, CG, false, false, E_GLU>;
-        case E_GLU_BWD: return tc_kernel<T, CG, false, false, E_GLU_BWD>;
-        default: return p.a_mn ? tc_kernel<T, CG, true, true, E_STORE> : tc_kernel<T, CG, false, true, E_STORE>;
+        case E_LINEAR: return tc_kernel<T, CG, false, false, E_LINEAR, M>;
+        case E_LINEAR_BWD: return tc_kernel<T, CG, false, false, E_LINEAR_BWD, M>;
+        case E_GLU: return tc_kernel<T, CG, false, false, E_GLU, M>;
+        case E_GLU_BWD: return tc_kernel<T, CG, false, false, E_GLU_BWD, M>;
+        default: return p.a_mn ? tc_kernel<T, CG, true, true, E_STORE, M> : tc_kernel<T, CG, false, true, E_STORE, M>;
     }
 }
 
@@ -580,12 +700,14 @@ bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t 
     return rows == 1 || (ld % 8 == 0 && ld >= cols);
 }
 
-int tc_splits(const Product& p) { return plan_of(p).splits; }
+int tc_splits(const Product& p, int dt) { return plan_of(p, mode_of(p, dt)).splits; }
 
 template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s) {
     if (encode_fn() == nullptr) return set_error(MABA_ERR_CUDA, "dense: cuTensorMapEncodeTiled not found");
-    constexpr int dt = std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16;
-    const Plan pl = plan_of(p);
+    constexpr int dt = sizeof(T) == 4 ? MABA_F32 : (std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16);
+    constexpr int planes = dt == MABA_F32 ? 3 : 1, odt = dt == MABA_F16 ? MABA_F16 : MABA_BF16;
+    const int mode = mode_of(p, dt);
+    const Plan pl = plan_of(p, mode);
     const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE, a_mn = p.a_mn, b_mn = store;
     TcArgs a{};
     a.M = p.M, a.N = p.N;
@@ -601,22 +723,26 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     if (units > 0x7fffffff) return set_error(MABA_ERR_UNSUPPORTED, "dense: %lld tiles", (long long)units);
     a.units = (int)units;
     const uint32_t bb = b_bytes_of(pl.cg, pl.bn, b_mn);
-    a.stage_bytes = A_BYTES + (bb + 1023) / 1024 * 1024;
-    a.load_bytes = (A_BYTES + bb) * pl.cg;
+    a.flush = mode == 0 ? a.kblocks : (mode == 1 ? 512 / BK : 256 / BK);
+    a.b_at = planes * A_BYTES;
+    a.b_bytes = (bb + 1023) / 1024 * 1024;
+    a.stage_bytes = planes * (A_BYTES + a.b_bytes);
+    a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
     const uint32_t room = SMEM_MAX - 1024 - TAIL;
     a.stages = (int)(room / a.stage_bytes);
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + TAIL;
-    a.idesc = idesc_f16(128 * pl.cg, pl.bn, dt == MABA_BF16, a_mn, b_mn);
+    a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
-    const int sl = p.e.res.f32 ? 4 : 2;
+    const bool out_f32 = planes == 3 || p.e.out_f32;
+    const int sl = p.e.res.f32 ? 4 : 2, ol = out_f32 ? 4 : 2;
     a.side_vec = p.e.res.p && p.e.res.sc == 1 && aligned16(p.e.res.p, p.e.res.sr, sl);
-    a.out_vec = aligned16(p.e.out, p.e.ldo, p.e.out_f32 ? 4 : 2) && (!p.e.out2 || aligned16(p.e.out2, p.e.ldo, 2));
+    a.out_vec = aligned16(p.e.out, p.e.ldo, ol) && (!p.e.out2 || aligned16(p.e.out2, p.e.ldo, ol));
     a.partial = partial;
     a.ldp = ldp;
     // (before the maps: this call binds the device's context to the thread, which encoding a
     // map needs and autograd's threads may not have)
-    const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p) : kernel_of<T, 1>(p);
+    const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p, mode) : kernel_of<T, 1>(p, mode);
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     CUtensorMap m[4];
@@ -624,8 +750,8 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     const int box = dual ? pl.bn / 2 : a.b_rows;
     bool ok = true;
     for (int i = 0; i < 2; ++i) {
-        ok = ok && operand_map(&m[i], dt, p.a[i < na ? i : 0], p.M, p.K, a_mn, 128);
-        ok = ok && operand_map(&m[2 + i], dt, p.b[i < nb ? i : 0], p.N, p.K, b_mn, box);
+        ok = ok && operand_map(&m[i], odt, p.a[i < na ? i : 0], planes, p.M, p.K, a_mn, 128);
+        ok = ok && operand_map(&m[2 + i], odt, p.b[i < nb ? i : 0], planes, p.N, p.K, b_mn, box);
     }
     if (!ok) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     const int slots = sm_count() / pl.cg;
@@ -644,6 +770,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
 }
+template int tc_product<float>(const Product&, float*, int64_t, cudaStream_t);
 template int tc_product<__half>(const Product&, float*, int64_t, cudaStream_t);
 template int tc_product<__nv_bfloat16>(const Product&, float*, int64_t, cudaStream_t);
 
