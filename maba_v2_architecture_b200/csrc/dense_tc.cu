@@ -16,7 +16,7 @@
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
 // A and one half of B, so a k-block costs an SM 32 KB for 128 x 256 x 64 products instead
-// of 48 KB, below what L2 delivers per SM) over one split of the contraction.  Ten warps:
+// of 48 KB, below what L2 delivers per SM) over one split of the contraction.  Twelve warps:
 //  * 0..7   epilogue: warp w reads TMEM lanes 32 (w & 3).. and every second 32-column
 //           chunk, applies the epilogue and stores whole rows' segments, staged through
 //           shared memory so that global accesses run along the rows;
@@ -45,7 +45,12 @@ __device__ int g_dense_error = 0;
 namespace {
 using namespace tc;
 
-constexpr int NTHR = 320, EPI_WARPS = 8, W_TMA = 8, W_MMA = 9;
+// Three warpgroups: 0..7 epilogue, 8 TMA, 9 MMA, 10 and 11 idle (they complete the warpgroup
+// that lends its registers): 256 x REG_EPI + 128 x REG_OTHER is what 384 threads are launched
+// with, and the epilogue's sums and pieces in flight do not spill.
+constexpr int NTHR = 384, EPI_WARPS = 8, W_TMA = 8, W_MMA = 9;
+constexpr int REG_LAUNCH = 168, REG_EPI = 224, REG_OTHER = 56;
+static_assert(256 * REG_EPI + 128 * REG_OTHER <= NTHR * REG_LAUNCH, "register split exceeds the launch");
 constexpr int BK = 64;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
@@ -153,9 +158,10 @@ template <int EL> __device__ __forceinline__ void fetch_pieces(uint4* v, const S
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * step);
 }
+// ... put into the staging area (the others straight from memory)
 template <typename T>
-__device__ __forceinline__ void pieces_to_rows(float* x, const uint4* v, bool f32, bool whole, const Side& s, const Chunk& k,
-                                               unsigned char* st, int lane) {
+__device__ __forceinline__ void stage_side(const uint4* v, bool f32, bool whole, const Side& s, const Chunk& k,
+                                           unsigned char* st, int lane) {
     __syncwarp();
     if (sizeof(T) == 4 || f32) {
         if (whole) {
@@ -164,25 +170,36 @@ __device__ __forceinline__ void pieces_to_rows(float* x, const uint4* v, bool f3
         } else {
             stage_in<float>(st, static_cast<const float*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols, lane);
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(x + 4 * i) = *at32(st, lane, i);
-    } else if constexpr (sizeof(T) == 2) {
+    } else {
         if (whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) *at16(st, i * 8 + (lane >> 2), lane & 3) = v[i];
         } else {
-            stage_in<uint16_t>(st, static_cast<const uint16_t*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols, lane);
+            stage_in<uint16_t>(st, static_cast<const uint16_t*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols,
+                               lane);
         }
-        __syncwarp();
+    }
+    __syncwarp();
+}
+// f(j, value) for the 32 staged values of this lane's row (read piece by piece: 32 registers
+// for all of them would spill)
+template <typename T, typename F>
+__device__ __forceinline__ void with_side(bool f32, unsigned char* st, int lane, F f) {
+    if (sizeof(T) == 4 || f32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 q = *reinterpret_cast<const float4*>(at32(st, lane, i));
+            f(4 * i, q.x), f(4 * i + 1, q.y), f(4 * i + 2, q.z), f(4 * i + 3, q.w);
+        }
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 q = *at16(st, lane, i);
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<T>(w[e]);
-                x[8 * i + 2 * e] = f.x, x[8 * i + 2 * e + 1] = f.y;
+                const float2 x = unpack2<T>(w[e]);
+                f(8 * i + 2 * e, x.x), f(8 * i + 2 * e + 1, x.y);
             }
         }
     }
@@ -296,6 +313,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         return t;
     };
 
+    if (warp >= EPI_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
     if (warp == W_TMA) {
         // ============================ TMA producer ============================
         int it = 0;
@@ -405,7 +424,9 @@ __global__ void __launch_bounds__(NTHR, 1)
             else umma_commit_elect(&bars[B_DRAIN]);
             mbar_wait_warp(&bars[B_DRAIN], 0, nullptr);
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_EPI));
         // ============================== epilogue ==============================
         constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
         constexpr int CH = MODE == 0 ? 1 : (DUAL ? 1 : 2);  // chunks whose sums a warp of MODE 1, 2 holds
@@ -500,8 +521,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             auto chunk = [&](int c, float* z, float* w) {
                 const Chunk k = place(c);
                 if (!live || k.cols <= 0) return;
-                float g[32];
-                if (has_side) pieces_to_rows<T>(g, side, e.res.f32, side_whole(k), e.res, k, st, lane);
+                if (has_side) stage_side<T>(side, e.res.f32, side_whole(k), e.res, k, st, lane);
                 if (KIND == E_LINEAR || KIND == E_LINEAR_BWD) {
                     __syncwarp();
                     vscale[lane] = ps;
@@ -522,22 +542,18 @@ __global__ void __launch_bounds__(NTHR, 1)
                         for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
                     });
                     if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
-                    if (has_side) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] += g[j];
-                    }
+                    if (has_side) with_side<T>(e.res.f32, st, lane, [&](int j, float g) { z[j] += g; });
                     store_rows<T>(z, e.out, e.out_f32, e.ldo, a.out_vec, k, st, lane);
                 } else if (KIND == E_LINEAR_BWD) {
                     float y[32];
                     if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
                     with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
+                        with_side<T>(e.res.f32, st, lane, [&](int j, float g) {
                             float f, d;
                             act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g[j] * d;
-                            y[j] = g[j] * f;
-                        }
+                            z[j] = g * d;
+                            y[j] = g * f;
+                        });
                     });
                     if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
                     if (k.rows < 32 && lane >= k.rows) {  // no part in the sums, whatever the bias is
@@ -562,13 +578,12 @@ __global__ void __launch_bounds__(NTHR, 1)
                     store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
                 } else {
                     with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
+                        with_side<T>(false, st, lane, [&](int j, float g) {
                             float f, d;
                             act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g[j] * w[j] * d;
-                            w[j] = g[j] * f;
-                        }
+                            z[j] = g * w[j] * d;
+                            w[j] = g * f;
+                        });
                     });
                     store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
                     store_rows<T>(w, e.out2, false, e.ldo, a.out_vec, k, st, lane);
@@ -679,16 +694,26 @@ bool aligned16(const void* p, int64_t ld, int el) {
 
 using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap);
 
+// The register split assumes REG_LAUNCH registers per thread at launch; with fewer, the
+// epilogue's increase would never complete, so such a build is not launched (nullptr).
+template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> Kernel checked() {
+    static const bool ok = [] {
+        cudaFuncAttributes fa{};
+        return cudaFuncGetAttributes(&fa, tc_kernel<T, CG, A_MN, B_MN, KIND, MODE>) == cudaSuccess && fa.numRegs == REG_LAUNCH;
+    }();
+    return ok ? tc_kernel<T, CG, A_MN, B_MN, KIND, MODE> : nullptr;
+}
+
 template <typename T, int CG> Kernel kernel_of(const Product& p, int mode) {
     constexpr int M = sizeof(T) == 4 ? 2 : 0;
     if constexpr (M == 0)
-        if (mode == 1) return tc_kernel<T, CG, false, false, E_LINEAR, 1>;
+        if (mode == 1) return checked<T, CG, false, false, E_LINEAR, 1>();
     switch (p.e.kind) {
-        case E_LINEAR: return tc_kernel<T, CG, false, false, E_LINEAR, M>;
-        case E_LINEAR_BWD: return tc_kernel<T, CG, false, false, E_LINEAR_BWD, M>;
-        case E_GLU: return tc_kernel<T, CG, false, false, E_GLU, M>;
-        case E_GLU_BWD: return tc_kernel<T, CG, false, false, E_GLU_BWD, M>;
-        default: return p.a_mn ? tc_kernel<T, CG, true, true, E_STORE, M> : tc_kernel<T, CG, false, true, E_STORE, M>;
+        case E_LINEAR: return checked<T, CG, false, false, E_LINEAR, M>();
+        case E_LINEAR_BWD: return checked<T, CG, false, false, E_LINEAR_BWD, M>();
+        case E_GLU: return checked<T, CG, false, false, E_GLU, M>();
+        case E_GLU_BWD: return checked<T, CG, false, false, E_GLU_BWD, M>();
+        default: return p.a_mn ? checked<T, CG, true, true, E_STORE, M>() : checked<T, CG, false, true, E_STORE, M>();
     }
 }
 
@@ -743,6 +768,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     // (before the maps: this call binds the device's context to the thread, which encoding a
     // map needs and autograd's threads may not have)
     const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p, mode) : kernel_of<T, 1>(p, mode);
+    if (kern == nullptr) return set_error(MABA_ERR_UNSUPPORTED, "dense(tcgen05): built with another register count");
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     CUtensorMap m[4];
