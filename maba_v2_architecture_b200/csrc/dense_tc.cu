@@ -64,7 +64,7 @@ static_assert(N_BARS * 8 + 8 <= 256, "barrier area");
 
 struct TcArgs {
     int64_t M, N;
-    int kblocks, kseg;  // contraction blocks over all segments, and of one
+    int kblocks, kseg, kb_split;  // contraction blocks over all segments, of one segment, of one split
     int tiles_n, splits, pairs, units, dual;
     int bn, b_rows;  // columns of the MMA, rows of B per CTA
     int flush;       // contraction blocks between two readings of the accumulator
@@ -300,16 +300,17 @@ __global__ void __launch_bounds__(NTHR, 1)
         int split, pair, kb0, kb1;
         int64_t m0, n0;
     };
-    auto unit_of = [&](int u) {
+    auto unit_of = [&](int unit) {
         Unit t;
-        t.split = u % a.splits;
-        u /= a.splits;
-        t.pair = u % a.pairs;
-        u /= a.pairs;
-        t.n0 = (int64_t)(u % a.tiles_n) * (a.dual ? a.bn / 2 : a.bn);
-        t.m0 = (int64_t)(u / a.tiles_n) * (128 * CG) + rank * 128;
-        t.kb0 = (int)((int64_t)a.kblocks * t.split / a.splits);
-        t.kb1 = (int)((int64_t)a.kblocks * (t.split + 1) / a.splits);
+        unsigned u = (unsigned)unit;
+        t.split = t.pair = 0;
+        if (a.splits > 1) t.split = (int)(u % (unsigned)a.splits), u /= (unsigned)a.splits;
+        if (a.pairs > 1) t.pair = (int)(u & 1u), u >>= 1;
+        const unsigned row = u / (unsigned)a.tiles_n;
+        t.n0 = (int64_t)(u - row * (unsigned)a.tiles_n) * (a.dual ? a.bn / 2 : a.bn);
+        t.m0 = (int64_t)row * (128 * CG) + rank * 128;
+        t.kb0 = t.split * a.kb_split;
+        t.kb1 = t.kb0 + a.kb_split < a.kblocks ? t.kb0 + a.kb_split : a.kblocks;
         return t;
     };
 
@@ -317,18 +318,21 @@ __global__ void __launch_bounds__(NTHR, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
     if (warp == W_TMA) {
         // ============================ TMA producer ============================
-        int it = 0;
+        // One thread runs the loop: a warp-wide one with an election for each copy took longer
+        // to issue a k-block than the tensor cores to multiply it.
+        if (elect_one()) {
+        int st = 0, it = 0;
+        uint32_t phase = 1;  // (a fresh barrier's previous phase counts as complete)
         bool ok = true;
         for (int u = worker; u < a.units && ok; u += workers) {
             const Unit t = unit_of(u);
             for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                const int st = it % a.stages, round = it / a.stages;
-                if (round > 0) ok = mbar_wait_warp(&bars[B_EMPTY + st], (round - 1) & 1, abort_f);
+                ok = mbar_wait(&bars[B_EMPTY + st], phase, abort_f);
                 if (!ok) break;
                 const int seg = kb >= a.kseg ? 1 : 0, k0 = (kb - seg * a.kseg) * BK;
                 const CUtensorMap* ma = (a.pairs == 2 ? t.pair : seg) ? &ta1 : &ta0;
                 unsigned char* sa = base + st * a.stage_bytes;
-                if (elect_one()) {
+                {
                     uint64_t* full = &bars[B_FULL + st];
                     const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : 0u;
                     auto load = [&](unsigned char* dst, const CUtensorMap* m, int x, int y, int plane) {
@@ -363,36 +367,41 @@ __global__ void __launch_bounds__(NTHR, 1)
                         }
                     }
                 }
-                __syncwarp();
+                if (++st == a.stages) st = 0, phase ^= 1;
             }
         }
         // every copy has landed before a CTA may exit (rank 0's barriers count the pair's)
         if (rank == 0)
             for (int s = 0; s < a.stages && s < it; ++s)
-                mbar_wait_warp(&bars[B_FULL + s], (((it - 1 - s) / a.stages)) & 1, nullptr);
+                mbar_wait(&bars[B_FULL + s], (((it - 1 - s) / a.stages)) & 1, nullptr);
+        }
     } else if (warp == W_MMA) {
         // ============================ MMA issuer ==============================
-        if (rank == 0) {
+        if (rank == 0 && elect_one()) {
             const uint64_t ad0 = sdesc_sw128(smem_addr(base), A_MN ? A_BYTES / 2 : 16, 1024);
             const uint64_t bd0 = sdesc_sw128(smem_addr(base + a.b_at), B_MN ? 8192 : 16, 1024);
             constexpr uint32_t ak = A_MN ? 2048 >> 4 : 32 >> 4, bk = B_MN ? 2048 >> 4 : 32 >> 4;
             auto mma = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t acc) {
-                if (CG == 2) umma_f16_ss_pair_elect(d, ad, bd, a.idesc, acc);
-                else umma_f16_ss_elect(d, ad, bd, a.idesc, acc);
+                if (CG == 2) umma_f16_ss_pair(d, ad, bd, a.idesc, acc);
+                else umma_f16_ss(d, ad, bd, a.idesc, acc);
             };
-            int it = 0, i = 0;  // i: accumulations begun
+            auto commit = [&](uint64_t* bar) {
+                if (CG == 2) umma_commit_pair(bar);
+                else umma_commit(bar);
+            };
+            int st = 0, buf = 0;
+            uint32_t phase = 0, tphase = 1;
             bool ok = true;
             for (int u = worker; u < a.units && ok; u += workers) {
                 const Unit t = unit_of(u);
-                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush, ++i) {
-                    const int buf = i & 1, f1 = f0 + a.flush < t.kb1 ? f0 + a.flush : t.kb1;
+                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush) {
+                    const int f1 = f0 + a.flush < t.kb1 ? f0 + a.flush : t.kb1;
                     const uint32_t d = tmem + buf * ACC_COLS;
-                    if (i >= 2) ok = mbar_wait_warp(&bars[B_TEMPTY + buf], ((i >> 1) - 1) & 1, abort_f);
+                    ok = mbar_wait(&bars[B_TEMPTY + buf], tphase, abort_f);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int kb = f0; kb < f1; ++kb, ++it) {
-                        const int st = it % a.stages;
-                        ok = mbar_wait_warp(&bars[B_FULL + st], (it / a.stages) & 1, abort_f);
+                    for (int kb = f0; kb < f1; ++kb) {
+                        ok = mbar_wait(&bars[B_FULL + st], phase, abort_f);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t so = (uint64_t)(st * (a.stage_bytes >> 4));
@@ -411,18 +420,18 @@ __global__ void __launch_bounds__(NTHR, 1)
                                 mma(d + MINOR, ad + k * ak + ap, bd + k * bk, 1u);
                             }
                         }
-                        if (CG == 2) umma_commit_pair_elect(&bars[B_EMPTY + st]);
-                        else umma_commit_elect(&bars[B_EMPTY + st]);
+                        commit(&bars[B_EMPTY + st]);
+                        if (++st == a.stages) st = 0, phase ^= 1;
                     }
                     if (!ok) break;
-                    if (CG == 2) umma_commit_pair_elect(&bars[B_TFULL + buf]);
-                    else umma_commit_elect(&bars[B_TFULL + buf]);
+                    commit(&bars[B_TFULL + buf]);
+                    buf ^= 1;
+                    if (buf == 0) tphase ^= 1;
                 }
             }
             // every product has completed before TMEM is freed
-            if (CG == 2) umma_commit_pair_elect(&bars[B_DRAIN]);
-            else umma_commit_elect(&bars[B_DRAIN]);
-            mbar_wait_warp(&bars[B_DRAIN], 0, nullptr);
+            commit(&bars[B_DRAIN]);
+            mbar_wait(&bars[B_DRAIN], 0, nullptr);
         }
     }
     } else {
@@ -725,7 +734,10 @@ bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t 
     return rows == 1 || (ld % 8 == 0 && ld >= cols);
 }
 
-int tc_splits(const Product& p, int dt) { return plan_of(p, mode_of(p, dt)).splits; }
+int tc_splits(const Product& p, int dt) {
+    const int64_t kblocks = ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
+    return (int)ceil_div(kblocks, ceil_div(kblocks, plan_of(p, mode_of(p, dt)).splits));  // none is empty
+}
 
 template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s) {
     if (encode_fn() == nullptr) return set_error(MABA_ERR_CUDA, "dense: cuTensorMapEncodeTiled not found");
@@ -740,7 +752,8 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.kblocks = a.kseg * (p.form == F_SUM ? 2 : 1);
     a.pairs = p.form == F_PAIR ? 2 : 1;
     a.dual = dual;
-    a.splits = pl.splits;
+    a.kb_split = (int)ceil_div(a.kblocks, pl.splits);
+    a.splits = (int)ceil_div(a.kblocks, a.kb_split);
     a.bn = pl.bn;
     a.b_rows = b_rows_of(pl.cg, pl.bn);
     a.tiles_n = (int)ceil_div(p.N, dual ? pl.bn / 2 : pl.bn);
