@@ -55,7 +55,8 @@ constexpr int BK = 64;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
 constexpr uint32_t STAGING = 32 * 128;  // one warp's 32 x 32 float32 chunk
-constexpr uint32_t TAIL = EPI_WARPS * STAGING + EPI_WARPS * 2 * 32 * 4 + 256;
+constexpr uint32_t ROW_TAIL = EPI_WARPS * STAGING + EPI_WARPS * 2 * 32 * 4;  // (not in fragment order)
+constexpr uint32_t BAR_BYTES = 256;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
 constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
 
@@ -244,15 +245,115 @@ template <typename F> __device__ __forceinline__ void with_vector(float* x, cons
         f(x[j], q.x), f(x[j + 1], q.y), f(x[j + 2], q.z), f(x[j + 3], q.w);
     }
 }
-// Sums of 32 columns over the warp's 32 rows, in a fixed tree; lane l returns column l's.
-__device__ __forceinline__ float column_sum(float* v, int lane) {
+// --------------------------------------------------------------------------
+// The same chunks in fragment order (tmem_ld_frag32): four lanes hold a 32-byte piece of a
+// float32 row, so they load and store without staging.  Float32 tiles staged both ways took
+// the shared memory bandwidth that the tensor cores read their operands with; and a column's
+// 32 rows lie in 8 lanes, so its sum takes 7 exchanges for 8 columns instead of 31 for 32.
+// Element j = 16 b + 4 g + 2 i + e: row 16 b + 8 i + lane / 4, column 8 g + 2 (lane % 4) + e.
+// --------------------------------------------------------------------------
+__device__ __forceinline__ int frag_row(int j, int lane) { return (j >> 4) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2); }
+__device__ __forceinline__ int frag_col(int j, int lane) { return ((j >> 2) & 3) * 8 + (lane & 3) * 2 + (j & 1); }
+
+template <typename E> struct Pair2;
+template <> struct Pair2<float> { using type = float2; };
+template <> struct Pair2<uint16_t> { using type = uint32_t; };
+
+// v: 16 pairs (pair j / 2 of elements j, j + 1)
+template <typename E>
+__device__ __forceinline__ void frag_fetch(typename Pair2<E>::type* v, const Side& s, bool vec, const Chunk& k, int lane) {
+    using P = typename Pair2<E>::type;
+    const E* p = static_cast<const E*>(s.p) + (k.row0 + (lane >> 2)) * s.sr + (k.col0 + (lane & 3) * 2) * s.sc;
+    if (vec && k.rows == 32 && k.cols == 32) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+        for (int q = 0; q < 16; ++q)
+            v[q] = *reinterpret_cast<const P*>(p + ((q >> 3) * 16 + (q & 1) * 8) * s.sr + ((q >> 1) & 3) * 8);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            E t[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = frag_row(2 * q, lane), c = frag_col(2 * q, lane) + e;
+                t[e] = r < k.rows && c < k.cols ? p[(r - (lane >> 2)) * s.sr + (c - (lane & 3) * 2) * s.sc] : E(0);
+            }
+            v[q] = *reinterpret_cast<P*>(t);
+        }
+    }
+}
+template <typename E>
+__device__ __forceinline__ void frag_put(const typename Pair2<E>::type* v, void* out, int64_t ld, bool vec, const Chunk& k,
+                                         int lane) {
+    using P = typename Pair2<E>::type;
+    E* p = static_cast<E*>(out) + (k.row0 + (lane >> 2)) * ld + k.col0 + (lane & 3) * 2;
+    if (vec && k.rows == 32 && k.cols == 32) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) *reinterpret_cast<P*>(p + ((q >> 3) * 16 + (q & 1) * 8) * ld + ((q >> 1) & 3) * 8) = v[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const E* t = reinterpret_cast<const E*>(&v[q]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = frag_row(2 * q, lane), c = frag_col(2 * q, lane) + e;
+                if (r < k.rows && c < k.cols) p[(r - (lane >> 2)) * ld + c - (lane & 3) * 2] = t[e];
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void frag_store(const float* z, void* out, bool f32, int64_t ld, bool vec, const Chunk& k, int lane) {
+    if (sizeof(T) == 4 || f32) {
+        frag_put<float>(reinterpret_cast<const float2*>(z), out, ld, vec, k, lane);
+    } else if constexpr (sizeof(T) == 2) {
+        uint32_t v[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) v[q] = pack2<T>(z[2 * q], z[2 * q + 1]);
+        frag_put<uint16_t>(v, out, ld, vec, k, lane);
+    }
+}
+// f(j, value) for the 32 fetched values
+template <typename T, typename F> __device__ __forceinline__ void with_frag(bool f32, const uint32_t* v, F f) {
+    if (sizeof(T) == 4 || f32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f(j, __uint_as_float(v[j]));
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const float2 x = unpack2<T>(v[q]);
+            f(2 * q, x.x), f(2 * q + 1, x.y);
+        }
+    }
+}
+// this lane's 8 columns of a vector, and x[j] op= the one of element j
+template <typename T> __device__ __forceinline__ void frag_vector(float* v, const Side& s, const Chunk& k, int lane, float none) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const int c = (q >> 1) * 8 + (lane & 3) * 2 + (q & 1);
+        v[q] = c < k.cols ? side_at<T>(s, 0, k.col0 + c) : none;
+    }
+}
+__device__ __forceinline__ int frag_vec_of(int j) { return ((j >> 2) & 3) * 2 + (j & 1); }
+// Column sums of a chunk over its 32 rows, in a fixed order: a lane's four rows, then the
+// eight lanes of a column.  Lane l returns column frag_sum_col(l).
+__device__ __forceinline__ int frag_sum_col(int lane) {
+    const int q = ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
+    return (q >> 1) * 8 + (lane & 3) * 2 + (q & 1);
+}
+__device__ __forceinline__ float frag_column_sum(const float* z, int lane) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const int j = (q >> 1) * 4 + (q & 1);
+        v[q] = (z[j] + z[j + 2]) + (z[j + 16] + z[j + 18]);
+    }
+#pragma unroll
+    for (int o = 16, n = 4; o > 2; o >>= 1, n >>= 1) {
         const bool hi = (lane & o) != 0;
 #pragma unroll
-        for (int j = 0; j < o; ++j) {
-            const float keep = hi ? v[j + o] : v[j], give = hi ? v[j] : v[j + o];
-            v[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        for (int q = 0; q < n; ++q) {
+            const float keep = hi ? v[q + n] : v[q], give = hi ? v[q] : v[q + n];
+            v[q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
         }
     }
     return v[0];
@@ -265,9 +366,8 @@ __global__ void __launch_bounds__(NTHR, 1)
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-    unsigned char* tail = base + a.stages * a.stage_bytes;
-    float* vecs = reinterpret_cast<float*>(tail + EPI_WARPS * STAGING);  // [8 warps][scale, bias][32]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(tail + EPI_WARPS * STAGING + EPI_WARPS * 2 * 32 * 4);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + a.stages * a.stage_bytes);
+    unsigned char* tail = base + a.stages * a.stage_bytes + BAR_BYTES;  // staging, then [8 warps][scale, bias][32]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* abort_f = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -438,71 +538,210 @@ __global__ void __launch_bounds__(NTHR, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_EPI));
         // ============================== epilogue ==============================
         constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
-        constexpr int CH = MODE == 0 ? 1 : (DUAL ? 1 : 2);  // chunks whose sums a warp of MODE 1, 2 holds
+        // chunks in fragment order: float32 in and out, and where columns are summed
+        constexpr bool FRAG = MODE != 0 || KIND == E_LINEAR_BWD;
+        constexpr bool VECS = KIND == E_LINEAR || KIND == E_LINEAR_BWD;
+        // MODE 1, 2: chunks (of a pair of projections: one) whose sums a warp holds
+        constexpr int CH = MODE == 0 || DUAL ? 1 : (MODE == 1 ? 4 : 2);
         const int q = warp & 3, h = warp >> 2;
         unsigned char* st = tail + warp * STAGING;
-        float* vscale = vecs + warp * 64;
+        float* vscale = reinterpret_cast<float*>(tail + EPI_WARPS * STAGING) + warp * 64;
         float* vbias = vscale + 32;
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
         const bool has_side = KIND != E_STORE && KIND != E_GLU && e.res.p != nullptr;
-        int i = 0;  // accumulations read
-        auto released = [&](int buf) {  // this warp has read its part of the accumulator
+        const bool side_f32 = sizeof(T) == 4 || e.res.f32, out_f32 = sizeof(T) == 4 || e.out_f32;
+        int buf = 0;
+        uint32_t phase = 0;
+        auto wait_full = [&]() {
+            const bool ok = mbar_wait_warp(&bars[B_TFULL + buf], phase, abort_f);
+            tc_fence_after();
+            return ok;
+        };
+        auto release = [&]() {  // this warp has read its part of the accumulator
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 if (CG == 2) mbar_arrive_cluster(cluster_addr(&bars[B_TEMPTY + buf], 0));
                 else mbar_arrive(&bars[B_TEMPTY + buf]);
             }
+            buf ^= 1;
+            if (buf == 0) phase ^= 1;
         };
-        bool ok = true;
         for (int u = worker; u < a.units; u += workers) {
             const Unit t = unit_of(u);
             const int64_t row0 = t.m0 + q * 32;
             const bool live = row0 < a.M;
-            uint4 side[8];
-            float ps = 0.f, pb = 0.f;  // this lane's column of scale and bias
+            const int rows = a.M - row0 < 32 ? (int)(a.M - row0) : 32;
             auto place = [&](int c) {
                 Chunk k;
                 k.row0 = row0, k.col0 = t.n0 + c * 32;
-                k.rows = a.M - row0 < 32 ? (int)(a.M - row0) : 32;
+                k.rows = rows;
                 k.cols = a.N - k.col0 < 32 ? (int)(a.N - k.col0) : 32;
                 return k;
             };
             auto side_whole = [&](const Chunk& k) { return a.side_vec && k.rows == 32 && k.cols == 32; };
+            uint4 side[8];           // the chunk's pieces of residual or gradient, in flight
+            float ps = 0.f, pb = 0.f;  // this lane's column of scale and bias
             auto fetch = [&](int c) {
                 const Chunk k = place(c);
+                if (k.cols <= 0) return;
+                if (FRAG) {
+                    if (has_side) {
+                        if (side_f32) frag_fetch<float>(reinterpret_cast<float2*>(side), e.res, a.side_vec, k, lane);
+                        else frag_fetch<uint16_t>(reinterpret_cast<uint32_t*>(side), e.res, a.side_vec, k, lane);
+                    }
+                    return;
+                }
                 if (has_side && side_whole(k)) {
-                    if (sizeof(T) == 4 || e.res.f32) fetch_pieces<4>(side, e.res, k, lane);
+                    if (side_f32) fetch_pieces<4>(side, e.res, k, lane);
                     else fetch_pieces<2>(side, e.res, k, lane);
                 }
-                if (KIND == E_LINEAR || KIND == E_LINEAR_BWD) {
+                if (VECS) {
                     if (e.scale.p) ps = lane < k.cols ? side_at<T>(e.scale, 0, k.col0 + lane) : 1.f;
                     if (e.bias.p) pb = lane < k.cols ? side_at<T>(e.bias, 0, k.col0 + lane) : 0.f;
                 }
             };
-            if (!MODE && live && h * 32 < width) fetch(h);
-            // MODE 1, 2: the accumulations of the unit, added up
-            float sz[MODE ? CH : 1][32], sw[MODE && DUAL ? 32 : 1];
-            if (MODE) {
+            // one chunk of sums: the epilogue in fragment order
+            auto chunk_frag = [&](int c, float* z, float* w, bool more) {
+                const Chunk k = place(c);
+                if (!live || k.cols <= 0) return;
+                const uint32_t* sv = reinterpret_cast<const uint32_t*>(side);
+                if (KIND == E_STORE) {
+                    if (a.splits > 1)
+                        frag_store<T>(z, a.partial + ((int64_t)t.split * a.pairs + t.pair) * a.M * a.ldp, true, a.ldp, true, k,
+                                      lane);
+                    else
+                        frag_store<T>(z, t.pair ? e.out2 : e.out, out_f32, e.ldo, a.out_vec, k, lane);
+                    return;
+                }
+                float vs[VECS ? 8 : 1], vb[VECS ? 8 : 1];
+                if (VECS && e.scale.p) frag_vector<T>(vs, e.scale, k, lane, 1.f);
+                if (VECS && e.bias.p) {
+                    frag_vector<T>(vb, e.bias, k, lane, 0.f);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) z[j] += vb[frag_vec_of(j)];
+                }
+                if (KIND == E_LINEAR) {
+                    with_act(e.act, [&](auto A) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
+                    });
+                    if (e.scale.p) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] *= vs[frag_vec_of(j)];
+                    }
+                    if (has_side) with_frag<T>(side_f32, sv, [&](int j, float g) { z[j] += g; });
+                    if (more) fetch(c + 2);
+                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
+                } else if (KIND == E_LINEAR_BWD) {
+                    float y[32];
+                    with_act(e.act, [&](auto A) {
+                        with_frag<T>(side_f32, sv, [&](int j, float g) {
+                            float f, d;
+                            act_grad16<A.value, EXACT>(z[j], f, d);
+                            z[j] = g * d;
+                            y[j] = g * f;
+                        });
+                    });
+                    if (more) fetch(c + 2);
+                    if (e.scale.p) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] *= vs[frag_vec_of(j)];
+                    }
+                    if (k.rows < 32) {  // rows past the last: no part in the sums, whatever the bias is
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (frag_row(j, lane) >= k.rows) z[j] = y[j] = 0.f;
+                    }
+                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
+                    const int col = frag_sum_col(lane);
+                    const int64_t at = (row0 >> 5) * a.N + k.col0 + col;
+                    if (e.part_bias) {
+                        const float s = frag_column_sum(z, lane);
+                        if (col < k.cols) e.part_bias[at] = s;
+                    }
+                    if (e.part_scale) {
+                        const float s = frag_column_sum(y, lane);
+                        if (col < k.cols) e.part_scale[at] = s;
+                    }
+                } else if (KIND == E_GLU) {
+                    with_act(e.act, [&](auto A) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
+                    });
+                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
+                } else {
+                    with_act(e.act, [&](auto A) {
+                        with_frag<T>(side_f32, sv, [&](int j, float g) {
+                            float f, d;
+                            act_grad16<A.value, EXACT>(z[j], f, d);
+                            z[j] = g * w[j] * d;
+                            w[j] = g * f;
+                        });
+                    });
+                    if (more) fetch(c + 2);
+                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
+                    frag_store<T>(w, e.out2, out_f32, e.ldo, a.out_vec, k, lane);
+                }
+            };
+            // and with a lane for a row, through the staging area
+            auto chunk_rows = [&](int c, float* z, float* w, bool more) {
+                const Chunk k = place(c);
+                if (!live || k.cols <= 0) return;
+                if (has_side) stage_side<T>(side, side_f32, side_whole(k), e.res, k, st, lane);
+                if (VECS) {
+                    __syncwarp();
+                    vscale[lane] = ps;
+                    vbias[lane] = pb;
+                    __syncwarp();
+                }
+                if (more) fetch(c + 2);
+                if (KIND == E_LINEAR) {
+                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
+                    with_act(e.act, [&](auto A) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
+                    });
+                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
+                    if (has_side) with_side<T>(side_f32, st, lane, [&](int j, float g) { z[j] += g; });
+                } else if (KIND == E_GLU) {
+                    with_act(e.act, [&](auto A) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
+                    });
+                } else if (KIND == E_GLU_BWD) {
+                    with_act(e.act, [&](auto A) {
+                        with_side<T>(false, st, lane, [&](int j, float g) {
+                            float f, d;
+                            act_grad16<A.value, EXACT>(z[j], f, d);
+                            z[j] = g * w[j] * d;
+                            w[j] = g * f;
+                        });
+                    });
+                }
+                store_rows<T>(z, t.pair ? e.out2 : e.out, out_f32, e.ldo, a.out_vec, k, st, lane);
+                if (KIND == E_GLU_BWD) store_rows<T>(w, e.out2, out_f32, e.ldo, a.out_vec, k, st, lane);
+            };
+            if constexpr (MODE != 0) {
+                float sz[CH][32], sw[DUAL ? 32 : 1];  // the unit's accumulations, added up
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
 #pragma unroll
                     for (int cc = 0; cc < CH; ++cc) sz[cc][j] = 0.f;
                     if (DUAL) sw[j] = 0.f;
                 }
-                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush, ++i) {
-                    const int buf = i & 1;
-                    ok = mbar_wait_warp(&bars[B_TFULL + buf], (i >> 1) & 1, abort_f);
+                bool ok = true;
+                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush) {
+                    ok = wait_full();
                     if (!ok) break;
-                    tc_fence_after();
                     const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
                     auto add = [&](float* sum, int col) {
                         float z[32];
-                        tmem_ld32(acc + col, reinterpret_cast<uint32_t*>(z));
+                        tmem_ld_frag32(acc + col, reinterpret_cast<uint32_t*>(z));
                         if (MODE == 2) {
                             float y[32];
-                            tmem_ld32(acc + MINOR + col, reinterpret_cast<uint32_t*>(y));
+                            tmem_ld_frag32(acc + MINOR + col, reinterpret_cast<uint32_t*>(y));
                             tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
                             tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(y));
 #pragma unroll
@@ -517,102 +756,36 @@ __global__ void __launch_bounds__(NTHR, 1)
                     for (int cc = 0; cc < CH; ++cc)
                         if ((h + 2 * cc) * 32 < width) add(sz[cc], (h + 2 * cc) * 32);
                     if (DUAL && h * 32 < width) add(sw, width + h * 32);
-                    released(buf);
+                    release();
                 }
                 if (!ok) break;
                 if (live && h * 32 < width) fetch(h);  // (here, or its registers would live through the sums)
-            } else {
-                ok = mbar_wait_warp(&bars[B_TFULL + (i & 1)], (i >> 1) & 1, abort_f);
-                if (!ok) break;
-                tc_fence_after();
-            }
-            const uint32_t acc = tmem + (i & 1) * ACC_COLS + ((uint32_t)(q * 32) << 16);
-            auto chunk = [&](int c, float* z, float* w) {
-                const Chunk k = place(c);
-                if (!live || k.cols <= 0) return;
-                if (has_side) stage_side<T>(side, e.res.f32, side_whole(k), e.res, k, st, lane);
-                if (KIND == E_LINEAR || KIND == E_LINEAR_BWD) {
-                    __syncwarp();
-                    vscale[lane] = ps;
-                    vbias[lane] = pb;
-                    __syncwarp();
+#pragma unroll
+                for (int cc = 0; cc < CH; ++cc) {
+                    const int c = h + 2 * cc;
+                    if (c * 32 < width) chunk_frag(c, sz[cc], sw, cc + 1 < CH && (c + 2) * 32 < width);
                 }
-                if ((c + 2) * 32 < width) fetch(c + 2);
-                if (KIND == E_STORE) {
-                    if (a.splits > 1)
-                        store_rows<T>(z, a.partial + ((int64_t)t.split * a.pairs + t.pair) * a.M * a.ldp, true, a.ldp, true, k,
-                                      st, lane);
-                    else
-                        store_rows<T>(z, t.pair ? e.out2 : e.out, false, e.ldo, a.out_vec, k, st, lane);
-                } else if (KIND == E_LINEAR) {
-                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
-                    });
-                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
-                    if (has_side) with_side<T>(e.res.f32, st, lane, [&](int j, float g) { z[j] += g; });
-                    store_rows<T>(z, e.out, e.out_f32, e.ldo, a.out_vec, k, st, lane);
-                } else if (KIND == E_LINEAR_BWD) {
-                    float y[32];
-                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
-                    with_act(e.act, [&](auto A) {
-                        with_side<T>(e.res.f32, st, lane, [&](int j, float g) {
-                            float f, d;
-                            act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g * d;
-                            y[j] = g * f;
-                        });
-                    });
-                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
-                    if (k.rows < 32 && lane >= k.rows) {  // no part in the sums, whatever the bias is
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = y[j] = 0.f;
-                    }
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
-                    const int64_t at = (row0 >> 5) * a.N + k.col0 + lane;
-                    if (e.part_bias) {
-                        const float s = column_sum(z, lane);
-                        if (lane < k.cols) e.part_bias[at] = s;
-                    }
-                    if (e.part_scale) {
-                        const float s = column_sum(y, lane);
-                        if (lane < k.cols) e.part_scale[at] = s;
-                    }
-                } else if (KIND == E_GLU) {
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
-                    });
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
-                } else {
-                    with_act(e.act, [&](auto A) {
-                        with_side<T>(false, st, lane, [&](int j, float g) {
-                            float f, d;
-                            act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g * w[j] * d;
-                            w[j] = g * f;
-                        });
-                    });
-                    store_rows<T>(z, e.out, false, e.ldo, a.out_vec, k, st, lane);
-                    store_rows<T>(w, e.out2, false, e.ldo, a.out_vec, k, st, lane);
-                }
-            };
-            if (MODE) {
-#pragma unroll
-                for (int cc = 0; cc < CH; ++cc)
-                    if ((h + 2 * cc) * 32 < width) chunk(h + 2 * cc, sz[cc], sw);
             } else {
+                if (live && h * 32 < width) fetch(h);
+                if (!wait_full()) break;
+                const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
+                if (h * 32 >= width) release();
                 for (int c = h; c * 32 < width; c += 2) {
+                    const bool more = (c + 2) * 32 < width;
                     float z[32], w[DUAL ? 32 : 1];
-                    tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
-                    if (DUAL) tmem_ld32(acc + width + c * 32, reinterpret_cast<uint32_t*>(w));
+                    const bool frag = FRAG || (KIND == E_STORE && a.splits > 1);
+                    if (frag) {
+                        tmem_ld_frag32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
+                    } else {
+                        tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
+                        if (DUAL) tmem_ld32(acc + width + c * 32, reinterpret_cast<uint32_t*>(w));
+                    }
                     tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
                     if (DUAL) tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(w));
-                    chunk(c, z, w);
+                    if (!more) release();
+                    if (frag) chunk_frag(c, z, w, more);
+                    else chunk_rows(c, z, w, more);
                 }
-                released(i & 1);
-                ++i;
             }
         }
     }
@@ -645,11 +818,11 @@ inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
     return (uint32_t)(mn ? (r + 63) / 64 * 64 : r) * 128u;
 }
 
-// How a product's sums are kept: 0 one accumulation, 1 added up in registers every 512
-// indices (float32 results of 16-bit operands), 2 float32 operands, every 256.
+// How a product's sums are kept: 0 one accumulation (16-bit results), 1 added up in registers
+// every 512 indices (float32 results of 16-bit operands), 2 float32 operands, every 256.
 int mode_of(const Product& p, int dt) {
     if (dt == MABA_F32) return 2;
-    return p.e.kind == E_LINEAR && p.e.out_f32 && p.K > 512 ? 1 : 0;
+    return p.e.kind == E_LINEAR && p.e.out_f32 ? 1 : 0;
 }
 
 // The tile and the splits with the least estimated time.  Per k-block and SM: the larger of
@@ -667,7 +840,7 @@ Plan plan_of(const Product& p, int mode) {
     Plan best;
     double least = 1e300;
     for (int cg = 1; cg <= 2; ++cg) {
-        const int most = mode ? 128 : (cg == 2 ? 256 : 192);
+        const int most = mode == 2 ? 128 : (cg == 2 ? 256 : 192);
         for (int bn = dual ? 64 : 32; bn <= most; bn += dual ? 64 : 32) {
             const int64_t tiles = ceil_div(p.M, 128 * cg) * ceil_div(p.N, dual ? bn / 2 : bn) * pairs;
             const int64_t slots = sm_count() / cg;
@@ -697,8 +870,8 @@ bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int planes, int64_t ro
     return make_map(m, dt, x.p, 3, dims, strides, box);
 }
 
-bool aligned16(const void* p, int64_t ld, int el) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * el) % 16 == 0;
+bool aligned(const void* p, int64_t ld, int el, int bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * el) % bytes == 0;
 }
 
 using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap);
@@ -766,16 +939,20 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.b_bytes = (bb + 1023) / 1024 * 1024;
     a.stage_bytes = planes * (A_BYTES + a.b_bytes);
     a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
-    const uint32_t room = SMEM_MAX - 1024 - TAIL;
+    const uint32_t tail = BAR_BYTES + (mode == 0 && p.e.kind != E_LINEAR_BWD ? ROW_TAIL : 0);
+    const uint32_t room = SMEM_MAX - 1024 - tail;
     a.stages = (int)(room / a.stage_bytes);
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
-    const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + TAIL;
+    const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + tail;
     a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
     const bool out_f32 = planes == 3 || p.e.out_f32;
     const int sl = p.e.res.f32 ? 4 : 2, ol = out_f32 ? 4 : 2;
-    a.side_vec = p.e.res.p && p.e.res.sc == 1 && aligned16(p.e.res.p, p.e.res.sr, sl);
-    a.out_vec = aligned16(p.e.out, p.e.ldo, ol) && (!p.e.out2 || aligned16(p.e.out2, p.e.ldo, ol));
+    // pieces of 16 bytes, or pairs of elements in fragment order
+    const bool frag = mode != 0 || p.e.kind == E_LINEAR_BWD;
+    a.side_vec = p.e.res.p && p.e.res.sc == 1 && aligned(p.e.res.p, p.e.res.sr, sl, frag ? 2 * sl : 16);
+    const int ob = frag ? 2 * ol : 16;
+    a.out_vec = aligned(p.e.out, p.e.ldo, ol, ob) && (!p.e.out2 || aligned(p.e.out2, p.e.ldo, ol, ob));
     a.partial = partial;
     a.ldp = ldp;
     // (before the maps: this call binds the device's context to the thread, which encoding a
