@@ -54,14 +54,14 @@ static_assert(256 * REG_EPI + 128 * REG_OTHER <= NTHR * REG_LAUNCH, "register sp
 constexpr int BK = 64;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
-constexpr uint32_t STAGING = 32 * 128;  // one warp's 32 x 32 float32 chunk
-constexpr uint32_t ROW_TAIL = EPI_WARPS * STAGING + EPI_WARPS * 2 * 32 * 4;  // (not in fragment order)
-constexpr uint32_t BAR_BYTES = 256;
+constexpr uint32_t VEC_BYTES = 2 * 4 * 32 * 4;  // a warp's scale and bias of four chunks
+constexpr uint32_t BAR_BYTES = 512;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
 constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
 
-enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2, N_BARS };
-static_assert(N_BARS * 8 + 8 <= 256, "barrier area");
+enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2,
+       B_SIDE = B_DRAIN + 1, N_BARS = B_SIDE + 2 * EPI_WARPS };
+static_assert(N_BARS * 8 + 8 <= BAR_BYTES, "barrier area");
 
 struct TcArgs {
     int64_t M, N;
@@ -72,7 +72,9 @@ struct TcArgs {
     int stages;
     uint32_t stage_bytes, b_at, b_bytes, load_bytes;  // B's place in a stage, one plane of it, bytes per stage
     uint32_t idesc;
-    int side_vec, out_vec;
+    int side_tma, out_tma;               // the epilogue's matrices move by copies
+    int n_in, n_out;                     // staging buffers per warp
+    uint32_t in_bytes, out_bytes, vec_at, bar_at;  // of one buffer; places of the vectors and the barriers
     Epilogue e;
     float* partial;
     int64_t ldp;
@@ -118,11 +120,12 @@ template <typename F> __device__ __forceinline__ void with_act(int act, F f) {
 }
 
 // --------------------------------------------------------------------------
-// 32 x 32 chunks between global memory (a warp's lanes along the rows) and registers (lane
-// = row), through the warp's staging area; 16-byte pieces are swizzled so that both
-// directions are free of bank conflicts.  A chunk that lies inside the matrix and on 16-byte
-// boundaries moves in 16-byte pieces with one address and constant steps (the epilogue is
-// bound by its instruction count); the others go element by element, out of line.
+// The epilogue works on chunks of 32 x 32 elements that tensor-memory copies bring into, and
+// take out of, a warp's staging buffers (moved by loads and stores they were bound by the
+// load/store unit's address stage).  A buffer has the copy's swizzle: rows of 128 bytes
+// (float32) or 64 (16 bits), 16-byte piece p of row r at p ^ (r & 7) or p ^ (r / 2 & 3), so
+// that a lane can read its row, or eight lanes a column of pieces, without bank conflicts.
+// What a copy cannot address (unaligned rows, strides) moves element by element, out of line.
 // --------------------------------------------------------------------------
 __device__ __forceinline__ uint4* at32(unsigned char* st, int row, int piece) {
     return reinterpret_cast<uint4*>(st + row * 128 + ((piece ^ (row & 7)) << 4));
@@ -130,11 +133,6 @@ __device__ __forceinline__ uint4* at32(unsigned char* st, int row, int piece) {
 __device__ __forceinline__ uint4* at16(unsigned char* st, int row, int piece) {
     return reinterpret_cast<uint4*>(st + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
 }
-struct Chunk {
-    int64_t row0, col0;
-    int rows, cols;  // of 32, inside the matrix
-};
-
 template <typename E> __device__ __forceinline__ E* element(unsigned char* st, int r, int c) {
     return sizeof(E) == 4 ? reinterpret_cast<E*>(at32(st, r, c >> 2)) + (c & 3)
                           : reinterpret_cast<E*>(at16(st, r, c >> 3)) + (c & 7);
@@ -150,192 +148,97 @@ __device__ __noinline__ void stage_out(unsigned char* st, E* dst, int64_t ld, in
         if (lane < cols) dst[r * ld + lane] = *element<E>(st, r, lane);
 }
 
-// The pieces of a whole chunk, in flight in registers (8 of float32, 4 of 16 bits).
-template <int EL> __device__ __forceinline__ void fetch_pieces(uint4* v, const Side& s, const Chunk& k, int lane) {
-    constexpr int PER = 32 * EL / 16, N = 32 * PER / 32;  // pieces per row, pieces per lane
-    const unsigned char* p = static_cast<const unsigned char*>(s.p) +
-                             ((k.row0 + lane / PER) * s.sr + k.col0) * EL + (lane % PER) * 16;
-    const int64_t step = s.sr * (EL * (32 / PER));
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * step);
-}
-// ... put into the staging area (the others straight from memory)
-template <typename T>
-__device__ __forceinline__ void stage_side(const uint4* v, bool f32, bool whole, const Side& s, const Chunk& k,
-                                           unsigned char* st, int lane) {
-    __syncwarp();
-    if (sizeof(T) == 4 || f32) {
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *at32(st, i * 4 + (lane >> 3), lane & 7) = v[i];
-        } else {
-            stage_in<float>(st, static_cast<const float*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols, lane);
-        }
-    } else {
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *at16(st, i * 8 + (lane >> 2), lane & 3) = v[i];
-        } else {
-            stage_in<uint16_t>(st, static_cast<const uint16_t*>(s.p) + k.row0 * s.sr + k.col0 * s.sc, s.sr, s.sc, k.rows, k.cols,
-                               lane);
-        }
-    }
-    __syncwarp();
-}
-// f(j, value) for the 32 staged values of this lane's row (read piece by piece: 32 registers
-// for all of them would spill)
-template <typename T, typename F>
-__device__ __forceinline__ void with_side(bool f32, unsigned char* st, int lane, F f) {
-    if (sizeof(T) == 4 || f32) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 q = *reinterpret_cast<const float4*>(at32(st, lane, i));
-            f(4 * i, q.x), f(4 * i + 1, q.y), f(4 * i + 2, q.z), f(4 * i + 3, q.w);
-        }
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 q = *at16(st, lane, i);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 x = unpack2<T>(w[e]);
-                f(8 * i + 2 * e, x.x), f(8 * i + 2 * e + 1, x.y);
-            }
-        }
-    }
-}
-template <int EL>
-__device__ __forceinline__ void store_pieces(unsigned char* st, void* out, int64_t ld, const Chunk& k, int lane) {
-    constexpr int PER = 32 * EL / 16, N = 32 * PER / 32, RS = 32 / PER;
-    unsigned char* p = static_cast<unsigned char*>(out) + ((k.row0 + lane / PER) * ld + k.col0) * EL + (lane % PER) * 16;
-    const int64_t step = ld * (EL * RS);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        *reinterpret_cast<uint4*>(p + i * step) =
-            EL == 4 ? *at32(st, i * RS + lane / PER, lane % PER) : *at16(st, i * RS + lane / PER, lane % PER);
-}
-template <typename T>
-__device__ __forceinline__ void store_rows(const float* x, void* out, bool f32, int64_t ld, bool vec, const Chunk& k,
-                                           unsigned char* st, int lane) {
-    const bool whole = vec && k.rows == 32 && k.cols == 32;
-    __syncwarp();
-    if (sizeof(T) == 4 || f32) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(at32(st, lane, i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        __syncwarp();
-        if (whole) store_pieces<4>(st, out, ld, k, lane);
-        else stage_out<float>(st, static_cast<float*>(out) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *at16(st, lane, i) = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]),
-                                            pack2<T>(x[8 * i + 4], x[8 * i + 5]), pack2<T>(x[8 * i + 6], x[8 * i + 7]));
-        __syncwarp();
-        if (whole) store_pieces<2>(st, out, ld, k, lane);
-        else stage_out<uint16_t>(st, static_cast<uint16_t*>(out) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
-    }
-}
-// x op= the 32 values of a shared vector
-template <typename F> __device__ __forceinline__ void with_vector(float* x, const float* v, F f) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(v + j);
-        f(x[j], q.x), f(x[j + 1], q.y), f(x[j + 2], q.z), f(x[j + 3], q.w);
-    }
-}
-// --------------------------------------------------------------------------
-// The same chunks in fragment order (tmem_ld_frag32): four lanes hold a 32-byte piece of a
-// float32 row, so they load and store without staging.  Float32 tiles staged both ways took
-// the shared memory bandwidth that the tensor cores read their operands with; and a column's
-// 32 rows lie in 8 lanes, so its sum takes 7 exchanges for 8 columns instead of 31 for 32.
-// Element j = 16 b + 4 g + 2 i + e: row 16 b + 8 i + lane / 4, column 8 g + 2 (lane % 4) + e.
-// --------------------------------------------------------------------------
+// A lane's 32 elements of a chunk: its row, or (FRAG, tmem_ld_frag32) the fragment order
+// j = 16 b + 4 g + 2 i + e: row 16 b + 8 i + lane / 4, column 8 g + 2 (lane % 4) + e, in which
+// a column's 32 rows lie in 8 lanes and its sum takes 7 exchanges for 8 columns, not 31 for 32.
 __device__ __forceinline__ int frag_row(int j, int lane) { return (j >> 4) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2); }
 __device__ __forceinline__ int frag_col(int j, int lane) { return ((j >> 2) & 3) * 8 + (lane & 3) * 2 + (j & 1); }
 
-template <typename E> struct Pair2;
-template <> struct Pair2<float> { using type = float2; };
-template <> struct Pair2<uint16_t> { using type = uint32_t; };
-
-// v: 16 pairs (pair j / 2 of elements j, j + 1)
-template <typename E>
-__device__ __forceinline__ void frag_fetch(typename Pair2<E>::type* v, const Side& s, bool vec, const Chunk& k, int lane) {
-    using P = typename Pair2<E>::type;
-    const E* p = static_cast<const E*>(s.p) + (k.row0 + (lane >> 2)) * s.sr + (k.col0 + (lane & 3) * 2) * s.sc;
-    if (vec && k.rows == 32 && k.cols == 32) {
+// f(j, value) for the 32 elements of a staged chunk
+template <typename T, bool FRAG, typename F>
+__device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane, F f) {
+    if (sizeof(T) == 4 || f32) {
+        if (FRAG) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-            v[q] = *reinterpret_cast<const P*>(p + ((q >> 3) * 16 + (q & 1) * 8) * s.sr + ((q >> 1) & 3) * 8);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            E t[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = frag_row(2 * q, lane), c = frag_col(2 * q, lane) + e;
-                t[e] = r < k.rows && c < k.cols ? p[(r - (lane >> 2)) * s.sr + (c - (lane & 3) * 2) * s.sc] : E(0);
+            for (int j = 0; j < 32; j += 2) {
+                const float2 x = *reinterpret_cast<const float2*>(element<float>(st, frag_row(j, lane), frag_col(j, lane)));
+                f(j, x.x), f(j + 1, x.y);
             }
-            v[q] = *reinterpret_cast<P*>(t);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(at32(st, lane, i));
+                f(4 * i, x.x), f(4 * i + 1, x.y), f(4 * i + 2, x.z), f(4 * i + 3, x.w);
+            }
         }
-    }
-}
-template <typename E>
-__device__ __forceinline__ void frag_put(const typename Pair2<E>::type* v, void* out, int64_t ld, bool vec, const Chunk& k,
-                                         int lane) {
-    using P = typename Pair2<E>::type;
-    E* p = static_cast<E*>(out) + (k.row0 + (lane >> 2)) * ld + k.col0 + (lane & 3) * 2;
-    if (vec && k.rows == 32 && k.cols == 32) {
+    } else if constexpr (sizeof(T) == 2) {
+        if (FRAG) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) *reinterpret_cast<P*>(p + ((q >> 3) * 16 + (q & 1) * 8) * ld + ((q >> 1) & 3) * 8) = v[q];
-    } else {
+            for (int j = 0; j < 32; j += 2) {
+                const float2 x =
+                    unpack2<T>(*reinterpret_cast<const uint32_t*>(element<uint16_t>(st, frag_row(j, lane), frag_col(j, lane))));
+                f(j, x.x), f(j + 1, x.y);
+            }
+        } else {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const E* t = reinterpret_cast<const E*>(&v[q]);
+            for (int i = 0; i < 4; ++i) {
+                const uint4 v = *at16(st, lane, i);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = frag_row(2 * q, lane), c = frag_col(2 * q, lane) + e;
-                if (r < k.rows && c < k.cols) p[(r - (lane >> 2)) * ld + c - (lane & 3) * 2] = t[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = unpack2<T>(w[e]);
+                    f(8 * i + 2 * e, x.x), f(8 * i + 2 * e + 1, x.y);
+                }
             }
         }
     }
 }
-template <typename T>
-__device__ __forceinline__ void frag_store(const float* z, void* out, bool f32, int64_t ld, bool vec, const Chunk& k, int lane) {
+template <typename T, bool FRAG> __device__ __forceinline__ void put_chunk(const float* z, bool f32, unsigned char* st, int lane) {
     if (sizeof(T) == 4 || f32) {
-        frag_put<float>(reinterpret_cast<const float2*>(z), out, ld, vec, k, lane);
+        if (FRAG) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+                *reinterpret_cast<float2*>(element<float>(st, frag_row(j, lane), frag_col(j, lane))) = make_float2(z[j], z[j + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(at32(st, lane, i)) = make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
+        }
     } else if constexpr (sizeof(T) == 2) {
-        uint32_t v[16];
+        if (FRAG) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) v[q] = pack2<T>(z[2 * q], z[2 * q + 1]);
-        frag_put<uint16_t>(v, out, ld, vec, k, lane);
-    }
-}
-// f(j, value) for the 32 fetched values
-template <typename T, typename F> __device__ __forceinline__ void with_frag(bool f32, const uint32_t* v, F f) {
-    if (sizeof(T) == 4 || f32) {
+            for (int j = 0; j < 32; j += 2)
+                *reinterpret_cast<uint32_t*>(element<uint16_t>(st, frag_row(j, lane), frag_col(j, lane))) = pack2<T>(z[j], z[j + 1]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f(j, __uint_as_float(v[j]));
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const float2 x = unpack2<T>(v[q]);
-            f(2 * q, x.x), f(2 * q + 1, x.y);
+            for (int i = 0; i < 4; ++i)
+                *at16(st, lane, i) = make_uint4(pack2<T>(z[8 * i], z[8 * i + 1]), pack2<T>(z[8 * i + 2], z[8 * i + 3]),
+                                                pack2<T>(z[8 * i + 4], z[8 * i + 5]), pack2<T>(z[8 * i + 6], z[8 * i + 7]));
         }
     }
 }
-// this lane's 8 columns of a vector, and x[j] op= the one of element j
-template <typename T> __device__ __forceinline__ void frag_vector(float* v, const Side& s, const Chunk& k, int lane, float none) {
+// f(z[j], v of j's column) for a vector of the chunk's 32 columns in shared memory
+template <bool FRAG, typename F> __device__ __forceinline__ void with_vector(float* z, const float* v, int lane, F f) {
+    if (FRAG) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int c = (q >> 1) * 8 + (lane & 3) * 2 + (q & 1);
-        v[q] = c < k.cols ? side_at<T>(s, 0, k.col0 + c) : none;
+        for (int g = 0; g < 4; ++g) {
+            const float2 x = *reinterpret_cast<const float2*>(v + g * 8 + (lane & 3) * 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = (r >> 1) * 16 + g * 4 + (r & 1) * 2;
+                f(z[j], x.x), f(z[j + 1], x.y);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(v + j);
+            f(z[j], x.x), f(z[j + 1], x.y), f(z[j + 2], x.z), f(z[j + 3], x.w);
+        }
     }
 }
-__device__ __forceinline__ int frag_vec_of(int j) { return ((j >> 2) & 3) * 2 + (j & 1); }
-// Column sums of a chunk over its 32 rows, in a fixed order: a lane's four rows, then the
-// eight lanes of a column.  Lane l returns column frag_sum_col(l).
+// Column sums of a chunk (FRAG) over its 32 rows, in a fixed order: a lane's four rows, then
+// the eight lanes of a column.  Lane l returns column frag_sum_col(l).
 __device__ __forceinline__ int frag_sum_col(int lane) {
     const int q = ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
     return (q >> 1) * 8 + (lane & 3) * 2 + (q & 1);
@@ -362,12 +265,14 @@ __device__ __forceinline__ float frag_column_sum(const float* z, int lane) {
 template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE>
 __global__ void __launch_bounds__(NTHR, 1)
     tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap ta0, const __grid_constant__ CUtensorMap ta1,
-              const __grid_constant__ CUtensorMap tb0, const __grid_constant__ CUtensorMap tb1) {
+              const __grid_constant__ CUtensorMap tb0, const __grid_constant__ CUtensorMap tb1,
+              const __grid_constant__ CUtensorMap tside, const __grid_constant__ CUtensorMap tout,
+              const __grid_constant__ CUtensorMap tout2) {
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + a.stages * a.stage_bytes);
-    unsigned char* tail = base + a.stages * a.stage_bytes + BAR_BYTES;  // staging, then [8 warps][scale, bias][32]
+    unsigned char* staging = base + a.stages * a.stage_bytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + a.bar_at);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* abort_f = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -538,27 +443,125 @@ __global__ void __launch_bounds__(NTHR, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_EPI));
         // ============================== epilogue ==============================
         constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
-        // chunks in fragment order: float32 in and out, and where columns are summed
-        constexpr bool FRAG = MODE != 0 || KIND == E_LINEAR_BWD;
-        constexpr bool VECS = KIND == E_LINEAR || KIND == E_LINEAR_BWD;
+        constexpr bool FRAG = KIND == E_LINEAR_BWD, VECS = KIND == E_LINEAR || KIND == E_LINEAR_BWD;
+        constexpr bool SIDE = KIND != E_STORE && KIND != E_GLU;
         // MODE 1, 2: chunks (of a pair of projections: one) whose sums a warp holds
         constexpr int CH = MODE == 0 || DUAL ? 1 : (MODE == 1 ? 4 : 2);
         const int q = warp & 3, h = warp >> 2;
-        unsigned char* st = tail + warp * STAGING;
-        float* vscale = reinterpret_cast<float*>(tail + EPI_WARPS * STAGING) + warp * 64;
-        float* vbias = vscale + 32;
+        unsigned char* in_buf = staging + warp * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
+        unsigned char* out_buf = in_buf + a.n_in * a.in_bytes;
+        float* vscale = reinterpret_cast<float*>(base + a.vec_at + warp * VEC_BYTES);  // [4 chunks][32]
+        float* vbias = vscale + 128;
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
-        const bool has_side = KIND != E_STORE && KIND != E_GLU && e.res.p != nullptr;
-        const bool side_f32 = sizeof(T) == 4 || e.res.f32, out_f32 = sizeof(T) == 4 || e.out_f32;
+        const bool has_side = SIDE && e.res.p != nullptr;
+        const bool side_f32 = sizeof(T) == 4 || e.res.f32;
+        const bool out_f32 = sizeof(T) == 4 || e.out_f32 || (KIND == E_STORE && a.splits > 1);
+        struct Chunk {
+            int row0, col0, rows, cols;  // rows, cols: of 32, inside the matrix
+        };
+        auto place = [&](const Unit& t, int c) {
+            Chunk k;
+            k.row0 = (int)t.m0 + q * 32, k.col0 = (int)t.n0 + c * 32;
+            k.rows = a.M - k.row0 < 32 ? (int)(a.M - k.row0) : 32;
+            k.cols = a.N - k.col0 < 32 ? (int)(a.N - k.col0) : 32;
+            return k;
+        };
+        // ---- residual or gradient: this warp's chunks in order, n_in of them ahead
+        int next_u = worker, next_c = h;  // the next chunk to bring
+        Unit next_t = unit_of(worker);
+        uint32_t brought = 0, used = 0;
+        auto bring = [&]() {
+            if (!has_side || !a.side_tma) return;
+            while (brought - used < (uint32_t)a.n_in && next_u < a.units) {
+                if (next_c * 32 >= width) {
+                    next_u += workers, next_c = h;
+                    if (next_u < a.units) next_t = unit_of(next_u);
+                    continue;
+                }
+                const Chunk k = place(next_t, next_c);
+                next_c += 2;
+                if (k.rows <= 0 || k.cols <= 0) continue;
+                const int slot = a.n_in == 2 ? (int)(brought & 1) : 0;
+                if (lane == 0) {
+                    uint64_t* bar = &bars[B_SIDE + 2 * warp + slot];
+                    mbar_arrive_expect_tx(bar, a.in_bytes);
+                    tma_load_3d(in_buf + slot * a.in_bytes, &tside, bar, k.col0, k.row0, 0);
+                }
+                ++brought;
+            }
+            __syncwarp();
+        };
+        auto side_wait = [&](uint32_t n, volatile int* abort) {
+            const int slot = a.n_in == 2 ? (int)(n & 1) : 0;
+            return mbar_wait_warp(&bars[B_SIDE + 2 * warp + slot], (a.n_in == 2 ? n >> 1 : n) & 1, abort);
+        };
+        bool ok = true;
+        auto side_ready = [&](const Chunk& k) {
+            if (a.side_tma) {
+                ok = side_wait(used, abort_f);
+                return in_buf + (a.n_in == 2 ? (used & 1) * a.in_bytes : 0u);
+            }
+            __syncwarp();
+            if (side_f32)
+                stage_in<float>(in_buf, static_cast<const float*>(e.res.p) + k.row0 * e.res.sr + k.col0 * e.res.sc, e.res.sr,
+                                e.res.sc, k.rows, k.cols, lane);
+            else
+                stage_in<uint16_t>(in_buf, static_cast<const uint16_t*>(e.res.p) + k.row0 * e.res.sr + k.col0 * e.res.sc,
+                                   e.res.sr, e.res.sc, k.rows, k.cols, lane);
+            __syncwarp();
+            return in_buf;
+        };
+        auto side_used = [&]() {
+            __syncwarp();
+            ++used;
+            bring();
+        };
+        // ---- results
+        uint32_t stored = 0;
+        auto store = [&](const Chunk& k, const float* z, const CUtensorMap* map, void* dst, int64_t ld, int plane) {
+            unsigned char* buf = out_buf + (a.n_out == 2 ? (stored & 1) * a.out_bytes : 0u);
+            ++stored;
+            if (lane == 0) {
+                if (a.n_out == 2) bulk_wait_read<1>();
+                else bulk_wait_read<0>();
+            }
+            __syncwarp();
+            put_chunk<T, FRAG>(z, out_f32, buf, lane);
+            if (a.out_tma) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_3d(map, buf, k.col0, k.row0, plane);
+                    bulk_commit();
+                }
+            } else {
+                __syncwarp();
+                if (out_f32) stage_out<float>(buf, static_cast<float*>(dst) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
+                else stage_out<uint16_t>(buf, static_cast<uint16_t*>(dst) + k.row0 * ld + k.col0, ld, k.rows, k.cols, lane);
+                __syncwarp();
+            }
+        };
+        // ---- scale and bias of a unit's columns, one unit ahead in registers
+        float ps[VECS ? 4 : 1], pb[VECS ? 4 : 1];
+        auto fetch_vectors = [&](const Unit& t) {
+#pragma unroll
+            for (int cc = 0; cc < (VECS ? 4 : 0); ++cc) {
+                const int64_t col = t.n0 + (h + 2 * cc) * 32 + lane;
+                const bool in = (h + 2 * cc) * 32 < width && col < a.N;
+                ps[cc] = in && e.scale.p ? side_at<T>(e.scale, 0, col) : 1.f;
+                pb[cc] = in && e.bias.p ? side_at<T>(e.bias, 0, col) : 0.f;
+            }
+        };
+        // ---- accumulators
         int buf = 0;
         uint32_t phase = 0;
         auto wait_full = [&]() {
-            const bool ok = mbar_wait_warp(&bars[B_TFULL + buf], phase, abort_f);
+            ok = mbar_wait_warp(&bars[B_TFULL + buf], phase, abort_f);
             tc_fence_after();
             return ok;
         };
-        auto release = [&]() {  // this warp has read its part of the accumulator
+        auto release = [&]() {  // this warp has read its part
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -568,161 +571,93 @@ __global__ void __launch_bounds__(NTHR, 1)
             buf ^= 1;
             if (buf == 0) phase ^= 1;
         };
+        auto load_sums = [&](float* z, uint32_t at) {
+            if (FRAG) tmem_ld_frag32(at, reinterpret_cast<uint32_t*>(z));
+            else tmem_ld32(at, reinterpret_cast<uint32_t*>(z));
+        };
+        // ---- one chunk
+        auto chunk = [&](const Unit& t, int c, float* z, float* w) {
+            const Chunk k = place(t, c);
+            if (k.rows <= 0 || k.cols <= 0) return;
+            unsigned char* in = nullptr;
+            const float *vs = vscale + (c >> 1) * 32, *vb = vbias + (c >> 1) * 32;
+            if (KIND == E_LINEAR) {
+                if (e.bias.p) with_vector<FRAG>(z, vb, lane, [](float& x, float v) { x += v; });
+                with_act(e.act, [&](auto A) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
+                });
+                if (e.scale.p) with_vector<FRAG>(z, vs, lane, [](float& x, float v) { x *= v; });
+                if (has_side) {
+                    in = side_ready(k);
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) { z[j] += g; });
+                    side_used();
+                }
+            } else if (KIND == E_LINEAR_BWD) {
+                float y[32];
+                if (e.bias.p) with_vector<FRAG>(z, vb, lane, [](float& x, float v) { x += v; });
+                in = side_ready(k);
+                with_act(e.act, [&](auto A) {
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) {
+                        float f, d;
+                        act_grad16<A.value, EXACT>(z[j], f, d);
+                        z[j] = g * d;
+                        y[j] = g * f;
+                    });
+                });
+                side_used();
+                if (e.scale.p) with_vector<FRAG>(z, vs, lane, [](float& x, float v) { x *= v; });
+                if (k.rows < 32) {  // rows past the last: no part in the sums, whatever the bias is
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (frag_row(j, lane) >= k.rows) z[j] = y[j] = 0.f;
+                }
+                const int col = frag_sum_col(lane);
+                const int64_t at = (int64_t)(k.row0 >> 5) * a.N + k.col0 + col;
+                if (e.part_bias) {
+                    const float s = frag_column_sum(z, lane);
+                    if (col < k.cols) e.part_bias[at] = s;
+                }
+                if (e.part_scale) {
+                    const float s = frag_column_sum(y, lane);
+                    if (col < k.cols) e.part_scale[at] = s;
+                }
+            } else if (KIND == E_GLU) {
+                with_act(e.act, [&](auto A) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
+                });
+            } else if (KIND == E_GLU_BWD) {
+                in = side_ready(k);
+                with_act(e.act, [&](auto A) {
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) {
+                        float f, d;
+                        act_grad16<A.value, EXACT>(z[j], f, d);
+                        z[j] = g * w[j] * d;
+                        w[j] = g * f;
+                    });
+                });
+                side_used();
+            }
+            if (KIND == E_STORE && a.splits > 1)
+                store(k, z, &tout, a.partial + (int64_t)(t.split * a.pairs + t.pair) * a.M * a.ldp, a.ldp,
+                      t.split * a.pairs + t.pair);
+            else
+                store(k, z, t.pair ? &tout2 : &tout, t.pair ? e.out2 : e.out, e.ldo, 0);
+            if (KIND == E_GLU_BWD) store(k, w, &tout2, e.out2, e.ldo, 0);
+        };
+
+        if (worker < a.units) fetch_vectors(next_t);
+        bring();
         for (int u = worker; u < a.units; u += workers) {
             const Unit t = unit_of(u);
-            const int64_t row0 = t.m0 + q * 32;
-            const bool live = row0 < a.M;
-            const int rows = a.M - row0 < 32 ? (int)(a.M - row0) : 32;
-            auto place = [&](int c) {
-                Chunk k;
-                k.row0 = row0, k.col0 = t.n0 + c * 32;
-                k.rows = rows;
-                k.cols = a.N - k.col0 < 32 ? (int)(a.N - k.col0) : 32;
-                return k;
-            };
-            auto side_whole = [&](const Chunk& k) { return a.side_vec && k.rows == 32 && k.cols == 32; };
-            uint4 side[8];           // the chunk's pieces of residual or gradient, in flight
-            float ps = 0.f, pb = 0.f;  // this lane's column of scale and bias
-            auto fetch = [&](int c) {
-                const Chunk k = place(c);
-                if (k.cols <= 0) return;
-                if (FRAG) {
-                    if (has_side) {
-                        if (side_f32) frag_fetch<float>(reinterpret_cast<float2*>(side), e.res, a.side_vec, k, lane);
-                        else frag_fetch<uint16_t>(reinterpret_cast<uint32_t*>(side), e.res, a.side_vec, k, lane);
-                    }
-                    return;
-                }
-                if (has_side && side_whole(k)) {
-                    if (side_f32) fetch_pieces<4>(side, e.res, k, lane);
-                    else fetch_pieces<2>(side, e.res, k, lane);
-                }
-                if (VECS) {
-                    if (e.scale.p) ps = lane < k.cols ? side_at<T>(e.scale, 0, k.col0 + lane) : 1.f;
-                    if (e.bias.p) pb = lane < k.cols ? side_at<T>(e.bias, 0, k.col0 + lane) : 0.f;
-                }
-            };
-            // one chunk of sums: the epilogue in fragment order
-            auto chunk_frag = [&](int c, float* z, float* w, bool more) {
-                const Chunk k = place(c);
-                if (!live || k.cols <= 0) return;
-                const uint32_t* sv = reinterpret_cast<const uint32_t*>(side);
-                if (KIND == E_STORE) {
-                    if (a.splits > 1)
-                        frag_store<T>(z, a.partial + ((int64_t)t.split * a.pairs + t.pair) * a.M * a.ldp, true, a.ldp, true, k,
-                                      lane);
-                    else
-                        frag_store<T>(z, t.pair ? e.out2 : e.out, out_f32, e.ldo, a.out_vec, k, lane);
-                    return;
-                }
-                float vs[VECS ? 8 : 1], vb[VECS ? 8 : 1];
-                if (VECS && e.scale.p) frag_vector<T>(vs, e.scale, k, lane, 1.f);
-                if (VECS && e.bias.p) {
-                    frag_vector<T>(vb, e.bias, k, lane, 0.f);
+            if (VECS) {
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) z[j] += vb[frag_vec_of(j)];
-                }
-                if (KIND == E_LINEAR) {
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
-                    });
-                    if (e.scale.p) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] *= vs[frag_vec_of(j)];
-                    }
-                    if (has_side) with_frag<T>(side_f32, sv, [&](int j, float g) { z[j] += g; });
-                    if (more) fetch(c + 2);
-                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
-                } else if (KIND == E_LINEAR_BWD) {
-                    float y[32];
-                    with_act(e.act, [&](auto A) {
-                        with_frag<T>(side_f32, sv, [&](int j, float g) {
-                            float f, d;
-                            act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g * d;
-                            y[j] = g * f;
-                        });
-                    });
-                    if (more) fetch(c + 2);
-                    if (e.scale.p) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] *= vs[frag_vec_of(j)];
-                    }
-                    if (k.rows < 32) {  // rows past the last: no part in the sums, whatever the bias is
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (frag_row(j, lane) >= k.rows) z[j] = y[j] = 0.f;
-                    }
-                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
-                    const int col = frag_sum_col(lane);
-                    const int64_t at = (row0 >> 5) * a.N + k.col0 + col;
-                    if (e.part_bias) {
-                        const float s = frag_column_sum(z, lane);
-                        if (col < k.cols) e.part_bias[at] = s;
-                    }
-                    if (e.part_scale) {
-                        const float s = frag_column_sum(y, lane);
-                        if (col < k.cols) e.part_scale[at] = s;
-                    }
-                } else if (KIND == E_GLU) {
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
-                    });
-                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
-                } else {
-                    with_act(e.act, [&](auto A) {
-                        with_frag<T>(side_f32, sv, [&](int j, float g) {
-                            float f, d;
-                            act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g * w[j] * d;
-                            w[j] = g * f;
-                        });
-                    });
-                    if (more) fetch(c + 2);
-                    frag_store<T>(z, e.out, out_f32, e.ldo, a.out_vec, k, lane);
-                    frag_store<T>(w, e.out2, out_f32, e.ldo, a.out_vec, k, lane);
-                }
-            };
-            // and with a lane for a row, through the staging area
-            auto chunk_rows = [&](int c, float* z, float* w, bool more) {
-                const Chunk k = place(c);
-                if (!live || k.cols <= 0) return;
-                if (has_side) stage_side<T>(side, side_f32, side_whole(k), e.res, k, st, lane);
-                if (VECS) {
-                    __syncwarp();
-                    vscale[lane] = ps;
-                    vbias[lane] = pb;
-                    __syncwarp();
-                }
-                if (more) fetch(c + 2);
-                if (KIND == E_LINEAR) {
-                    if (e.bias.p) with_vector(z, vbias, [](float& x, float v) { x += v; });
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
-                    });
-                    if (e.scale.p) with_vector(z, vscale, [](float& x, float v) { x *= v; });
-                    if (has_side) with_side<T>(side_f32, st, lane, [&](int j, float g) { z[j] += g; });
-                } else if (KIND == E_GLU) {
-                    with_act(e.act, [&](auto A) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
-                    });
-                } else if (KIND == E_GLU_BWD) {
-                    with_act(e.act, [&](auto A) {
-                        with_side<T>(false, st, lane, [&](int j, float g) {
-                            float f, d;
-                            act_grad16<A.value, EXACT>(z[j], f, d);
-                            z[j] = g * w[j] * d;
-                            w[j] = g * f;
-                        });
-                    });
-                }
-                store_rows<T>(z, t.pair ? e.out2 : e.out, out_f32, e.ldo, a.out_vec, k, st, lane);
-                if (KIND == E_GLU_BWD) store_rows<T>(w, e.out2, out_f32, e.ldo, a.out_vec, k, st, lane);
-            };
+                for (int cc = 0; cc < 4; ++cc) vscale[cc * 32 + lane] = ps[cc], vbias[cc * 32 + lane] = pb[cc];
+                __syncwarp();
+                if (u + workers < a.units) fetch_vectors(unit_of(u + workers));
+            }
             if constexpr (MODE != 0) {
                 float sz[CH][32], sw[DUAL ? 32 : 1];  // the unit's accumulations, added up
 #pragma unroll
@@ -731,17 +666,15 @@ __global__ void __launch_bounds__(NTHR, 1)
                     for (int cc = 0; cc < CH; ++cc) sz[cc][j] = 0.f;
                     if (DUAL) sw[j] = 0.f;
                 }
-                bool ok = true;
                 for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush) {
-                    ok = wait_full();
-                    if (!ok) break;
+                    if (!wait_full()) break;
                     const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
                     auto add = [&](float* sum, int col) {
                         float z[32];
-                        tmem_ld_frag32(acc + col, reinterpret_cast<uint32_t*>(z));
+                        load_sums(z, acc + col);
                         if (MODE == 2) {
                             float y[32];
-                            tmem_ld_frag32(acc + MINOR + col, reinterpret_cast<uint32_t*>(y));
+                            load_sums(y, acc + MINOR + col);
                             tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
                             tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(y));
 #pragma unroll
@@ -759,35 +692,30 @@ __global__ void __launch_bounds__(NTHR, 1)
                     release();
                 }
                 if (!ok) break;
-                if (live && h * 32 < width) fetch(h);  // (here, or its registers would live through the sums)
 #pragma unroll
                 for (int cc = 0; cc < CH; ++cc) {
                     const int c = h + 2 * cc;
-                    if (c * 32 < width) chunk_frag(c, sz[cc], sw, cc + 1 < CH && (c + 2) * 32 < width);
+                    if (c * 32 < width) chunk(t, c, sz[cc], sw);
                 }
             } else {
-                if (live && h * 32 < width) fetch(h);
                 if (!wait_full()) break;
                 const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
                 if (h * 32 >= width) release();
                 for (int c = h; c * 32 < width; c += 2) {
-                    const bool more = (c + 2) * 32 < width;
                     float z[32], w[DUAL ? 32 : 1];
-                    const bool frag = FRAG || (KIND == E_STORE && a.splits > 1);
-                    if (frag) {
-                        tmem_ld_frag32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
-                    } else {
-                        tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z));
-                        if (DUAL) tmem_ld32(acc + width + c * 32, reinterpret_cast<uint32_t*>(w));
-                    }
+                    load_sums(z, acc + c * 32);
+                    if (DUAL) load_sums(w, acc + width + c * 32);
                     tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
                     if (DUAL) tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(w));
-                    if (!more) release();
-                    if (frag) chunk_frag(c, z, w, more);
-                    else chunk_rows(c, z, w, more);
+                    if ((c + 2) * 32 >= width) release();
+                    chunk(t, c, z, w);
                 }
             }
+            if (!ok) break;
         }
+        // copies in flight end before the CTA may
+        for (; used < brought; ++used) side_wait(used, nullptr);
+        if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
     tc_fence_before();
@@ -870,11 +798,18 @@ bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int planes, int64_t ro
     return make_map(m, dt, x.p, 3, dims, strides, box);
 }
 
-bool aligned(const void* p, int64_t ld, int el, int bytes) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * el) % bytes == 0;
+// The map of a matrix that the epilogue reads or writes in chunks, rows x cols (x planes).
+bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t planes) {
+    const int el = dt == MABA_F32 ? 4 : 2;
+    if (rows == 1) ld = (cols + 7) / 8 * 8;
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (ld * el) % 16 != 0 || ld < cols) return false;
+    const int64_t dims[3] = {cols, rows, planes}, strides[2] = {ld, planes > 1 ? rows * ld : ld};
+    const uint32_t box[3] = {32, 32, 1};
+    return make_map(m, dt, p, 3, dims, strides, box);
 }
 
-using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap);
+using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
+                        const CUtensorMap, const CUtensorMap, const CUtensorMap);
 
 // The register split assumes REG_LAUNCH registers per thread at launch; with fewer, the
 // epilogue's increase would never complete, so such a build is not launched (nullptr).
@@ -939,20 +874,26 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.b_bytes = (bb + 1023) / 1024 * 1024;
     a.stage_bytes = planes * (A_BYTES + a.b_bytes);
     a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
-    const uint32_t tail = BAR_BYTES + (mode == 0 && p.e.kind != E_LINEAR_BWD ? ROW_TAIL : 0);
-    const uint32_t room = SMEM_MAX - 1024 - tail;
-    a.stages = (int)(room / a.stage_bytes);
+    // staging: two buffers each way where that leaves three stages (two of the large ones of
+    // float32 operands) for the products, else fewer
+    const bool out_f32 = planes == 3 || p.e.out_f32 || a.splits > 1, side_f32 = planes == 3 || p.e.res.f32;
+    const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
+    a.in_bytes = p.e.res.p ? (side_f32 ? 4096 : 2048) : 0;
+    a.out_bytes = out_f32 ? 4096 : 2048;
+    const uint32_t fixed = 1024 + BAR_BYTES + (vecs ? EPI_WARPS * VEC_BYTES : 0);
+    uint32_t staging = 0;
+    for (int t = 0; t < 3; ++t) {
+        a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
+        staging = EPI_WARPS * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
+        a.stages = (int)((SMEM_MAX - fixed - staging) / a.stage_bytes);
+        if (a.stages >= (mode == 2 ? 2 : 3)) break;
+    }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
-    const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + tail;
+    a.vec_at = a.stages * a.stage_bytes + staging;
+    a.bar_at = a.vec_at + (vecs ? EPI_WARPS * VEC_BYTES : 0);
+    const size_t smem = 1024 + a.bar_at + BAR_BYTES;
     a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
-    const bool out_f32 = planes == 3 || p.e.out_f32;
-    const int sl = p.e.res.f32 ? 4 : 2, ol = out_f32 ? 4 : 2;
-    // pieces of 16 bytes, or pairs of elements in fragment order
-    const bool frag = mode != 0 || p.e.kind == E_LINEAR_BWD;
-    a.side_vec = p.e.res.p && p.e.res.sc == 1 && aligned(p.e.res.p, p.e.res.sr, sl, frag ? 2 * sl : 16);
-    const int ob = frag ? 2 * ol : 16;
-    a.out_vec = aligned(p.e.out, p.e.ldo, ol, ob) && (!p.e.out2 || aligned(p.e.out2, p.e.ldo, ol, ob));
     a.partial = partial;
     a.ldp = ldp;
     // (before the maps: this call binds the device's context to the thread, which encoding a
@@ -961,7 +902,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     if (kern == nullptr) return set_error(MABA_ERR_UNSUPPORTED, "dense(tcgen05): built with another register count");
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
-    CUtensorMap m[4];
+    CUtensorMap m[7];
     const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = p.form == F_SUM || dual ? 2 : 1;
     const int box = dual ? pl.bn / 2 : a.b_rows;
     bool ok = true;
@@ -970,6 +911,15 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
         ok = ok && operand_map(&m[2 + i], odt, p.b[i < nb ? i : 0], planes, p.N, p.K, b_mn, box);
     }
     if (!ok) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
+    m[4] = m[5] = m[6] = m[0];
+    a.side_tma = p.e.res.p && p.e.res.sc == 1 &&
+                 chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1);
+    if (a.splits > 1) {
+        a.out_tma = chunk_map(&m[5], MABA_F32, partial, p.M, p.N, ldp, a.splits * a.pairs);
+    } else {
+        a.out_tma = chunk_map(&m[5], out_f32 ? MABA_F32 : odt, p.e.out, p.M, p.N, p.e.ldo, 1) &&
+                    (!p.e.out2 || chunk_map(&m[6], out_f32 ? MABA_F32 : odt, p.e.out2, p.M, p.N, p.e.ldo, 1));
+    }
     const int slots = sm_count() / pl.cg;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((a.units < slots ? a.units : slots) * pl.cg));
@@ -982,7 +932,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pl.cg == 2 ? 1 : 0;
-    err = cudaLaunchKernelEx(&cfg, kern, a, m[0], m[1], m[2], m[3]);
+    err = cudaLaunchKernelEx(&cfg, kern, a, m[0], m[1], m[2], m[3], m[4], m[5], m[6]);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
 }

@@ -25,23 +25,28 @@ inline EncodeTiled encode_fn() {
     return fn;
 }
 
-// rank-R tiled map of 16-bit elements, 128-byte swizzle; strides in elements (R-1 of them)
+// rank-R tiled map of 16-bit (or float32) elements; strides in elements (R-1 of them).  The
+// swizzle is the inner box's width, 128 or 64 bytes.
 inline bool make_map(CUtensorMap* m, int dtype, const void* ptr, int rank, const int64_t* dims, const int64_t* strides,
-              const uint32_t* box) {
+                     const uint32_t* box) {
     EncodeTiled fn = encode_fn();
     if (fn == nullptr) return false;
+    const int el = dtype == MABA_F32 ? 4 : 2;
     cuuint64_t gd[5], gs[4];
     cuuint32_t bx[5], es[5];
     for (int i = 0; i < rank; ++i) {
         gd[i] = (cuuint64_t)dims[i];
         bx[i] = box[i];
         es[i] = 1;
-        if (i + 1 < rank) gs[i] = (cuuint64_t)strides[i] * 2;
+        if (i + 1 < rank) gs[i] = (cuuint64_t)strides[i] * el;
     }
     const CUresult r =
-        fn(m, dtype == MABA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
-           const_cast<void*>(ptr), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        fn(m,
+           dtype == MABA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+           : dtype == MABA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+           (cuuint32_t)rank, const_cast<void*>(ptr), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           box[0] * el == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
 
