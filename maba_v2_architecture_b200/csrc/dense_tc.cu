@@ -17,7 +17,7 @@
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
 // A and one half of B, so a k-block costs an SM 32 KB for 128 x 256 x 64 products instead
 // of 48 KB, below what L2 delivers per SM) over one split of the contraction.  Twelve warps:
-//  * 0..7   epilogue: warp w reads TMEM lanes 32 (w & 3).. and every second 32-column
+//  * 0..7   epilogue: warp w reads TMEM lanes 32 (w & 3).. and every fourth 32-column
 //           chunk, applies the epilogue and stores whole rows' segments, staged through
 //           shared memory so that global accesses run along the rows;
 //  * 8      TMA producer: 64 contraction indices per stage, 128-byte swizzle, operands
@@ -45,22 +45,26 @@ __device__ int g_dense_error = 0;
 namespace {
 using namespace tc;
 
-// Three warpgroups: 0..7 epilogue, 8 TMA, 9 MMA, 10 and 11 idle (they complete the warpgroup
-// that lends its registers): 256 x REG_EPI + 128 x REG_OTHER is what 384 threads are launched
-// with, and the epilogue's sums and pieces in flight do not spill.
-constexpr int NTHR = 384, EPI_WARPS = 8, W_TMA = 8, W_MMA = 9;
-constexpr int REG_LAUNCH = 168, REG_EPI = 224, REG_OTHER = 56;
-static_assert(256 * REG_EPI + 128 * REG_OTHER <= NTHR * REG_LAUNCH, "register split exceeds the launch");
+// Epilogue warps: 16 where a chunk's registers allow four warps per scheduler (their chains of
+// shared-memory, copy and SFU latencies hide each other), 8 where a warp holds a unit's sums.
+// Then one warpgroup: TMA, MMA and two idle warps that complete it; it lends registers to the
+// epilogue's.  What the split hands out is what the block is launched with.
+template <int MODE> struct Warps {
+    static constexpr int EPI = MODE == 0 ? 16 : 8, TMA = EPI, MMA = EPI + 1, THREADS = (EPI + 4) * 32;
+    static constexpr int REG_LAUNCH = MODE == 0 ? 96 : 168, REG_EPI = MODE == 0 ? 104 : 224, REG_OTHER = MODE == 0 ? 64 : 56;
+    static_assert(EPI * 32 * REG_EPI + 128 * REG_OTHER <= THREADS * REG_LAUNCH, "register split exceeds the launch");
+};
+constexpr int MAX_EPI = 16;
 constexpr int BK = 64;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
-constexpr uint32_t VEC_BYTES = 2 * 4 * 32 * 4;  // a warp's scale and bias of four chunks
+constexpr uint32_t VEC_BYTES = 2 * 4 * 32 * 4;  // a warp's scale and bias of up to four chunks
 constexpr uint32_t BAR_BYTES = 512;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
 constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
 
 enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2,
-       B_SIDE = B_DRAIN + 1, N_BARS = B_SIDE + 2 * EPI_WARPS };
+       B_SIDE = B_DRAIN + 1, N_BARS = B_SIDE + 2 * MAX_EPI };
 static_assert(N_BARS * 8 + 8 <= BAR_BYTES, "barrier area");
 
 struct TcArgs {
@@ -263,7 +267,7 @@ __device__ __forceinline__ float frag_column_sum(const float* z, int lane) {
 }
 
 template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE>
-__global__ void __launch_bounds__(NTHR, 1)
+__global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     tc_kernel(const TcArgs a, const __grid_constant__ CUtensorMap ta0, const __grid_constant__ CUtensorMap ta1,
               const __grid_constant__ CUtensorMap tb0, const __grid_constant__ CUtensorMap tb1,
               const __grid_constant__ CUtensorMap tside, const __grid_constant__ CUtensorMap tout,
@@ -277,6 +281,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     volatile int* abort_f = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     constexpr int PLANES = MODE == 2 ? 3 : 1;
+    constexpr int EPI_WARPS = Warps<MODE>::EPI, W_TMA = Warps<MODE>::TMA, W_MMA = Warps<MODE>::MMA;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     };
 
     if (warp >= EPI_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Warps<MODE>::REG_OTHER));
     if (warp == W_TMA) {
         // ============================ TMA producer ============================
         // One thread runs the loop: a warp-wide one with an election for each copy took longer
@@ -440,18 +445,20 @@ __global__ void __launch_bounds__(NTHR, 1)
         }
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_EPI));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Warps<MODE>::REG_EPI));
         // ============================== epilogue ==============================
         constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
         constexpr bool FRAG = KIND == E_LINEAR_BWD, VECS = KIND == E_LINEAR || KIND == E_LINEAR_BWD;
         constexpr bool SIDE = KIND != E_STORE && KIND != E_GLU;
         // MODE 1, 2: chunks (of a pair of projections: one) whose sums a warp holds
         constexpr int CH = MODE == 0 || DUAL ? 1 : (MODE == 1 ? 4 : 2);
+        constexpr int CS = EPI_WARPS / 4;  // a warp's chunks are CS apart
+        constexpr int NV = 8 / CS;         // and at most so many
         const int q = warp & 3, h = warp >> 2;
         unsigned char* in_buf = staging + warp * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
         unsigned char* out_buf = in_buf + a.n_in * a.in_bytes;
-        float* vscale = reinterpret_cast<float*>(base + a.vec_at + warp * VEC_BYTES);  // [4 chunks][32]
-        float* vbias = vscale + 128;
+        float* vscale = reinterpret_cast<float*>(base + a.vec_at + warp * VEC_BYTES);  // [NV chunks][32]
+        float* vbias = vscale + NV * 32;
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
         const bool has_side = SIDE && e.res.p != nullptr;
@@ -480,7 +487,7 @@ __global__ void __launch_bounds__(NTHR, 1)
                     continue;
                 }
                 const Chunk k = place(next_t, next_c);
-                next_c += 2;
+                next_c += CS;
                 if (k.rows <= 0 || k.cols <= 0) continue;
                 const int slot = a.n_in == 2 ? (int)(brought & 1) : 0;
                 if (lane == 0) {
@@ -543,12 +550,12 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
         };
         // ---- scale and bias of a unit's columns, one unit ahead in registers
-        float ps[VECS ? 4 : 1], pb[VECS ? 4 : 1];
+        float ps[NV], pb[NV];
         auto fetch_vectors = [&](const Unit& t) {
 #pragma unroll
-            for (int cc = 0; cc < (VECS ? 4 : 0); ++cc) {
-                const int64_t col = t.n0 + (h + 2 * cc) * 32 + lane;
-                const bool in = (h + 2 * cc) * 32 < width && col < a.N;
+            for (int cc = 0; cc < (VECS ? NV : 0); ++cc) {
+                const int64_t col = t.n0 + (h + CS * cc) * 32 + lane;
+                const bool in = (h + CS * cc) * 32 < width && col < a.N;
                 ps[cc] = in && e.scale.p ? side_at<T>(e.scale, 0, col) : 1.f;
                 pb[cc] = in && e.bias.p ? side_at<T>(e.bias, 0, col) : 0.f;
             }
@@ -580,7 +587,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             const Chunk k = place(t, c);
             if (k.rows <= 0 || k.cols <= 0) return;
             unsigned char* in = nullptr;
-            const float *vs = vscale + (c >> 1) * 32, *vb = vbias + (c >> 1) * 32;
+            const float *vs = vscale + c / CS * 32, *vb = vbias + c / CS * 32;
             if (KIND == E_LINEAR) {
                 if (e.bias.p) with_vector<FRAG>(z, vb, lane, [](float& x, float v) { x += v; });
                 with_act(e.act, [&](auto A) {
@@ -654,7 +661,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             if (VECS) {
                 __syncwarp();
 #pragma unroll
-                for (int cc = 0; cc < 4; ++cc) vscale[cc * 32 + lane] = ps[cc], vbias[cc * 32 + lane] = pb[cc];
+                for (int cc = 0; cc < NV; ++cc) vscale[cc * 32 + lane] = ps[cc], vbias[cc * 32 + lane] = pb[cc];
                 __syncwarp();
                 if (u + workers < a.units) fetch_vectors(unit_of(u + workers));
             }
@@ -687,27 +694,27 @@ __global__ void __launch_bounds__(NTHR, 1)
                     };
 #pragma unroll
                     for (int cc = 0; cc < CH; ++cc)
-                        if ((h + 2 * cc) * 32 < width) add(sz[cc], (h + 2 * cc) * 32);
+                        if ((h + CS * cc) * 32 < width) add(sz[cc], (h + CS * cc) * 32);
                     if (DUAL && h * 32 < width) add(sw, width + h * 32);
                     release();
                 }
                 if (!ok) break;
 #pragma unroll
                 for (int cc = 0; cc < CH; ++cc) {
-                    const int c = h + 2 * cc;
+                    const int c = h + CS * cc;
                     if (c * 32 < width) chunk(t, c, sz[cc], sw);
                 }
             } else {
                 if (!wait_full()) break;
                 const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
                 if (h * 32 >= width) release();
-                for (int c = h; c * 32 < width; c += 2) {
+                for (int c = h; c * 32 < width; c += CS) {
                     float z[32], w[DUAL ? 32 : 1];
                     load_sums(z, acc + c * 32);
                     if (DUAL) load_sums(w, acc + width + c * 32);
                     tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
                     if (DUAL) tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(w));
-                    if ((c + 2) * 32 >= width) release();
+                    if ((c + CS) * 32 >= width) release();
                     chunk(t, c, z, w);
                 }
             }
@@ -816,7 +823,7 @@ using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, cons
 template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> Kernel checked() {
     static const bool ok = [] {
         cudaFuncAttributes fa{};
-        return cudaFuncGetAttributes(&fa, tc_kernel<T, CG, A_MN, B_MN, KIND, MODE>) == cudaSuccess && fa.numRegs == REG_LAUNCH;
+        return cudaFuncGetAttributes(&fa, tc_kernel<T, CG, A_MN, B_MN, KIND, MODE>) == cudaSuccess && fa.numRegs == Warps<MODE>::REG_LAUNCH;
     }();
     return ok ? tc_kernel<T, CG, A_MN, B_MN, KIND, MODE> : nullptr;
 }
@@ -874,23 +881,23 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.b_bytes = (bb + 1023) / 1024 * 1024;
     a.stage_bytes = planes * (A_BYTES + a.b_bytes);
     a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
-    // staging: two buffers each way where that leaves three stages (two of the large ones of
-    // float32 operands) for the products, else fewer
+    // staging: two buffers each way where that leaves enough stages for the products, else fewer
+    const int epi = mode == 0 ? Warps<0>::EPI : Warps<1>::EPI, threads = mode == 0 ? Warps<0>::THREADS : Warps<1>::THREADS;
     const bool out_f32 = planes == 3 || p.e.out_f32 || a.splits > 1, side_f32 = planes == 3 || p.e.res.f32;
     const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
     a.in_bytes = p.e.res.p ? (side_f32 ? 4096 : 2048) : 0;
     a.out_bytes = out_f32 ? 4096 : 2048;
-    const uint32_t fixed = 1024 + BAR_BYTES + (vecs ? EPI_WARPS * VEC_BYTES : 0);
+    const uint32_t fixed = 1024 + BAR_BYTES + (vecs ? epi * VEC_BYTES : 0);
     uint32_t staging = 0;
     for (int t = 0; t < 3; ++t) {
         a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
-        staging = EPI_WARPS * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
+        staging = epi * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
         a.stages = (int)((SMEM_MAX - fixed - staging) / a.stage_bytes);
-        if (a.stages >= (mode == 2 ? 2 : 3)) break;
+        if (a.stages >= (mode == 2 ? 2 : (mode == 1 ? 3 : 4))) break;
     }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     a.vec_at = a.stages * a.stage_bytes + staging;
-    a.bar_at = a.vec_at + (vecs ? EPI_WARPS * VEC_BYTES : 0);
+    a.bar_at = a.vec_at + (vecs ? epi * VEC_BYTES : 0);
     const size_t smem = 1024 + a.bar_at + BAR_BYTES;
     a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
@@ -923,7 +930,7 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     const int slots = sm_count() / pl.cg;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((a.units < slots ? a.units : slots) * pl.cg));
-    cfg.blockDim = dim3(NTHR);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
