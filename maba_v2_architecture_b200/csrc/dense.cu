@@ -22,14 +22,6 @@ struct Scratch {
     }
 };
 
-struct Ctx {
-    int dt;            // operand type
-    bool dry;          // workspace query: no launches
-    Scratch ws;
-    cudaStream_t s;
-};
-
-inline size_t esize(int dt) { return dt == MABA_F32 ? 4 : 2; }
 
 #define DENSE_DISPATCH(DT, ...)                                                  \
     [&]() -> int {                                                               \
@@ -42,50 +34,98 @@ inline size_t esize(int dt) { return dt == MABA_F32 ? 4 : 2; }
 // ---------------------------------------------------------------------------
 // small kernels
 // ---------------------------------------------------------------------------
-// dst [rows][ld] (T) = src (T or float32, any strides)
-template <typename T>
-__global__ void __launch_bounds__(256) copy_kernel(Side src, int64_t rows, int64_t cols, T* dst, int64_t ld) {
-    const int64_t n = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        dst[r * ld + c] = Cvt<T>::from_f(side_at<T>(src, r, c));
+// x = x1 + x2 + x3: each the nearest bf16 of what the ones before left, so the three hold all
+// 24 bits of x (a finite x that would round to infinity is truncated).  An infinity or NaN is
+// x1 alone.
+__device__ __forceinline__ void split_planes(float x, __nv_bfloat16 (&v)[3]) {
+    v[0] = __float2bfloat16_rn(x), v[1] = v[2] = __float2bfloat16_rn(0.f);
+    if (isfinite(x)) {
+        if (!isfinite(__bfloat162float(v[0]))) v[0] = __float2bfloat16_rz(x);
+        const float r = x - __bfloat162float(v[0]);
+        v[1] = __float2bfloat16_rn(r);
+        v[2] = __float2bfloat16_rn(r - __bfloat162float(v[1]));
     }
 }
 
-// dst [3][rows][ld] (bf16) = x1, x2, x3 with x = x1 + x2 + x3: each the nearest bf16 of what
-// the ones before left, so the three hold all 24 bits of x (the largest finite float32 would
-// round to infinity: it is truncated).  An infinity or NaN is x1 alone.
-__global__ void __launch_bounds__(256)
-    planes_kernel(const float* __restrict__ src, int64_t sr, int64_t sc, int64_t rows, int64_t cols, __nv_bfloat16* dst,
-                  int64_t ld, int64_t plane) {
-    const int64_t n = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        const float x = src[r * sr + c * sc];
-        __nv_bfloat16 x1 = __float2bfloat16_rn(x), x2 = __float2bfloat16_rn(0.f), x3 = x2;
-        if (isfinite(x)) {
-            if (!isfinite(__bfloat162float(x1))) x1 = __float2bfloat16_rz(x);
-            const float r1 = x - __bfloat162float(x1);
-            x2 = __float2bfloat16_rn(r1);
-            x3 = __float2bfloat16_rn(r1 - __bfloat162float(x2));
+// Operands made readable, up to three in one launch: dst [rows][ld] of a 16-bit type = src (that
+// type or float32, any strides), or the three planes of a float32 src.  Tiles of 32 x 64 pass
+// through shared memory, so that both sides run along their contiguous axis.
+struct Job {
+    Side src;
+    int64_t rows = 0, cols = 0;
+    void* dst = nullptr;
+    int64_t ld = 0, plane = 0;
+};
+struct Jobs {
+    Job j[3];
+    int n = 0;
+};
+template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Jobs jobs) {
+    __shared__ float tile[32][65];
+    const Job& b = jobs.j[blockIdx.y];
+    const int tiles_c = (int)((b.cols + 63) / 64);
+    const int64_t tiles = (b.rows + 31) / 32 * tiles_c;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t r0 = t / tiles_c * 32, c0 = t % tiles_c * 64;
+        if (b.src.sc <= b.src.sr) {  // lanes along the columns
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = w * 4 + (i >> 1), c = (i & 1) * 32 + lane;
+                if (r0 + r < b.rows && c0 + c < b.cols) tile[r][c] = side_at<T>(b.src, r0 + r, c0 + c);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = lane, c = w * 8 + i;
+                if (r0 + r < b.rows && c0 + c < b.cols) tile[r][c] = side_at<T>(b.src, r0 + r, c0 + c);
+            }
         }
-        __nv_bfloat16* d = dst + r * ld + c;
-        d[0] = x1, d[plane] = x2, d[2 * plane] = x3;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = w * 4 + i, c = lane * 2;
+            if (r0 + r >= b.rows || c0 + c >= b.cols) continue;  // (ld is a multiple of 8: the pair fits)
+            const float x = tile[r][c], y = c0 + c + 1 < b.cols ? tile[r][c + 1] : 0.f;
+            const int64_t at = (r0 + r) * b.ld + c0 + c;
+            if constexpr (sizeof(T) == 4) {
+                __nv_bfloat16 p[3], q[3];
+                split_planes(x, p), split_planes(y, q);
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(b.dst) + e * b.plane + at) =
+                        __halves2bfloat162(p[e], q[e]);
+            } else {
+                T* d = static_cast<T*>(b.dst) + at;
+                const T v[2] = {Cvt<T>::from_f(x), Cvt<T>::from_f(y)};
+                *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(v);
+            }
+        }
+        __syncthreads();
     }
 }
 
-// out = sum over splits of partial [splits][rows][ldp]; rows from `half` on go to out2
+// out = sum over splits of partial [splits][rows][ldp]; rows from `half` on go to out2.  A
+// thread adds four columns; ldp is a multiple of 4.
 template <typename T>
 __global__ void __launch_bounds__(256)
     sum_splits_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t rows, int64_t cols, T* out,
                       T* out2, int64_t half, int64_t ld) {
-    const int64_t n = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        float z = 0.f;
-        for (int q = 0; q < splits; ++q) z += partial[(q * rows + r) * ldp + c];
-        T* o = r < half ? out + r * ld : out2 + (r - half) * ld;
-        o[c] = Cvt<T>::from_f(z);
+    const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 4;
+    if (c >= cols) return;
+    for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
+        const float* p = partial + r * ldp + c;
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int q = 0; q < splits; ++q) {
+            const float4 v = *reinterpret_cast<const float4*>(p + q * rows * ldp);
+            z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+        }
+        T* o = (r < half ? out + r * ld : out2 + (r - half) * ld) + c;
+        const float zz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) o[e] = Cvt<T>::from_f(zz[e]);
     }
 }
 
@@ -109,30 +149,42 @@ __global__ void __launch_bounds__(256) colsum_kernel(Side g, int64_t rows, int64
     }
 }
 
-// out[n] = sum over blocks of part [blocks][cols]
+// out[n] = sum over blocks of part [blocks][cols], for one or two vectors (blockIdx.y): 32
+// threads add a column's blocks in turn, then their sums in order
+struct Columns {
+    const float* part[2];
+    void* out[2];
+    int64_t so[2];
+    int f32[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(256)
-    colsum_finish_kernel(const float* __restrict__ part, int64_t blocks, int64_t cols, void* out, int64_t so, int out_f32) {
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int w = threadIdx.x >> 5;
-    __shared__ float red[8][32];
+__global__ void __launch_bounds__(1024) colsum_finish_kernel(const Columns v, int64_t blocks, int64_t cols) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.y;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    __shared__ float red[32][33];
     float s = 0.f;
-    if (c < cols)
-        for (int64_t b = w; b < blocks; b += 8) s += part[b * cols + c];
-    red[w][threadIdx.x & 31] = s;
+    if (c < cols) {
+        const float* p = v.part[i] + c;
+#pragma unroll 8
+        for (int64_t b = w; b < blocks; b += 32) s += p[b * cols];
+    }
+    red[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < cols) {
         float t = 0.f;
-        for (int q = 0; q < 8; ++q) t += red[q][threadIdx.x];
-        if (out_f32) static_cast<float*>(out)[c * so] = t;
-        else static_cast<T*>(out)[c * so] = Cvt<T>::from_f(t);
+        for (int q = 0; q < 32; ++q) t += red[q][lane];
+        if (v.f32[i]) static_cast<float*>(v.out[i])[c * v.so[i]] = t;
+        else static_cast<T*>(v.out[i])[c * v.so[i]] = Cvt<T>::from_f(t);
     }
 }
 
-inline unsigned grid1d(int64_t n) {
-    const int64_t g = ceil_div(n, 256), cap = 8 * (int64_t)sm_count();
-    return (unsigned)(g < cap ? (g > 0 ? g : 1) : cap);
-}
+struct Ctx {
+    int dt;    // operand type
+    bool dry;  // workspace query: no launches
+    Scratch ws;
+    cudaStream_t s;
+    Jobs jobs;  // operand copies not launched yet
+};
 
 // ---------------------------------------------------------------------------
 // products
@@ -144,24 +196,37 @@ int run(Ctx& c, const Product& p) {
     }
     // a plain product whose tiles do not fill the GPU splits its contraction; the partial
     // sums are float32 and added in split order
-    const int splits = tc_splits(p, c.dt);
+    const Plan plan = tc_plan(p, c.dt);
     const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
-    float* partial = splits > 1 ? static_cast<float*>(c.ws.take((size_t)splits * rows * ldp * 4)) : nullptr;
+    float* partial = plan.splits > 1 ? static_cast<float*>(c.ws.take((size_t)plan.splits * rows * ldp * 4)) : nullptr;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        MABA_TRY(tc_product<T>(p, partial, ldp, c.s));
-        if (splits == 1) return (int)MABA_OK;
-        sum_splits_kernel<T><<<grid1d(rows * p.N), 256, 0, c.s>>>(partial, ldp, splits, rows, p.N, static_cast<T*>(p.e.out),
-                                                                  static_cast<T*>(p.e.out2), p.M, p.e.ldo);
+        MABA_TRY(tc_product<T>(p, plan, partial, ldp, c.s));
+        if (plan.splits == 1) return (int)MABA_OK;
+        const int64_t gy = ceil_div(rows, 8), cap = 32768;
+        sum_splits_kernel<T><<<dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), 256, 0, c.s>>>(
+            partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2), p.M, p.e.ldo);
         return check_launch("dense(split sums)");
     });
 }
 
-int copy_matrix(Ctx& c, const Side& src, int64_t rows, int64_t cols, void* dst, int64_t ld) {
+// Launches the copies that operand() has noted.
+int prepare(Ctx& c) {
+    const int n = c.jobs.n;
+    if (n == 0) return MABA_OK;
+    int64_t most = 1;
+    for (int i = 0; i < n; ++i) {
+        const int64_t t = ceil_div(c.jobs.j[i].rows, 32) * ceil_div(c.jobs.j[i].cols, 64);
+        most = t > most ? t : most;
+    }
+    const int64_t cap = 16 * (int64_t)sm_count();
+    const dim3 grid((unsigned)(most < cap ? most : cap), (unsigned)n);
+    const Jobs jobs = c.jobs;
+    c.jobs.n = 0;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        copy_kernel<T><<<grid1d(rows * cols), 256, 0, c.s>>>(src, rows, cols, static_cast<T*>(dst), ld);
-        return check_launch("dense(copy)");
+        prepare_kernel<T><<<grid, 256, 0, c.s>>>(jobs);
+        return check_launch("dense(operands)");
     });
 }
 
@@ -174,11 +239,19 @@ int column_sums(Ctx& c, const Side& g, int64_t rows, int64_t cols, float* part) 
     });
 }
 
-int finish_columns(Ctx& c, const float* part, int64_t blocks, int64_t cols, const maba_tensor* out) {
-    if (c.dry) return MABA_OK;
+int finish_columns(Ctx& c, const float* pb, const maba_tensor* db, const float* ps, const maba_tensor* ds, int64_t blocks,
+                   int64_t cols) {
+    Columns v{};
+    int n = 0;
+    for (int i = 0; i < 2; ++i) {
+        const maba_tensor* t = i ? ds : db;
+        if (!(i ? ps : pb)) continue;
+        v.part[n] = i ? ps : pb, v.out[n] = t->data, v.so[n] = t->stride[0], v.f32[n] = t->dtype == MABA_F32;
+        ++n;
+    }
+    if (n == 0) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        colsum_finish_kernel<T><<<(unsigned)ceil_div(cols, 32), 256, 0, c.s>>>(part, blocks, cols, out->data,
-                                                                               out->stride[0], out->dtype == MABA_F32);
+        colsum_finish_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), n), 1024, 0, c.s>>>(v, blocks, cols);
         return check_launch("dense(column sums)");
     });
 }
@@ -241,28 +314,23 @@ Side side1(const maba_tensor* t) { return given(t) ? Side{t->data, 0, t->stride[
 // the operators
 // ---------------------------------------------------------------------------
 // A matrix as an operand.  The tensor-memory loads of the 16-bit products want rows on
-// 16-byte boundaries; what is not laid out so is copied once per call, and a float32 matrix
-// is split into its planes.  One copy serves both directions of a matrix: K-major along its
-// rows, MN-major across them.
-int operand(Ctx& c, const Side& t, int64_t rows, int64_t cols, Matrix& m) {
-    m = Matrix{t.p, t.sr, t.sc, 0};
-    if (!t.f32 && tc_readable(t.p, rows, cols, t.sr, t.sc)) return MABA_OK;
+// 16-byte boundaries; what is not laid out so is copied once per call (noted here, launched by
+// prepare()), and a float32 matrix is split into its planes.  One copy serves both directions
+// of a matrix: K-major along its rows, MN-major across them.
+void operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
+    const Side src = side2(t);
+    const int64_t rows = t->shape[0], cols = t->shape[1];
+    m = Matrix{src.p, src.sr, src.sc, 0};
+    if (as_is || (!src.f32 && tc_readable(src.p, rows, cols, src.sr, src.sc))) return;
     const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
     void* to = c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2);
     m = Matrix{to, ld, 1, plane};
-    if (c.dt != MABA_F32) return copy_matrix(c, t, rows, cols, to, ld);
-    if (c.dry) return MABA_OK;
-    planes_kernel<<<grid1d(rows * cols), 256, 0, c.s>>>(static_cast<const float*>(t.p), t.sr, t.sc, rows, cols,
-                                                        static_cast<__nv_bfloat16*>(to), ld, plane);
-    return check_launch("dense(planes)");
+    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, plane};
 }
-int operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
-    m = Matrix{t->data, t->stride[0], t->stride[1], 0};
-    return as_is ? (int)MABA_OK : operand(c, side2(t), t->shape[0], t->shape[1], m);
-}
-// What an epilogue of this call wrote, [rows][ld] in the operands' type.
-int own_operand(Ctx& c, void* p, int64_t ld, int64_t rows, int64_t cols, Matrix& m) {
-    return operand(c, Side{p, ld, 1, c.dt == MABA_F32}, rows, cols, m);
+// A gradient that an epilogue writes as an operand of the next products.
+Matrix written_operand(Ctx& c, int64_t rows, int64_t cols) {
+    const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
+    return Matrix{c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2), ld, 1, plane};
 }
 Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr, m.sp}; }
 
@@ -278,8 +346,9 @@ int linear_forward(Ctx& c, const LinearArgs& a) {
     if (p.M == 0) return MABA_OK;
     p.e.kind = E_LINEAR;
     const bool as_is = skinny_takes(p, c.dt);
-    MABA_TRY(operand(c, a.x, p.a[0], as_is));
-    MABA_TRY(operand(c, a.w, p.b[0], as_is));
+    operand(c, a.x, p.a[0], as_is);
+    operand(c, a.w, p.b[0], as_is);
+    MABA_TRY(prepare(c));
     p.e.act = a.act;
     p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.res);
     if (a.out) p.e.out = a.out->data, p.e.ldo = a.out->stride[0], p.e.out_f32 = a.out->dtype == MABA_F32;
@@ -331,29 +400,28 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
     float* pb = need_db ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     float* ps = need_ds ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     Matrix x, w, d;
-    if (!through || need_dw) MABA_TRY(operand(c, a.x, x));
-    if (!through || need_dx) MABA_TRY(operand(c, a.w, w));
+    if (!through || need_dw) operand(c, a.x, x);
+    if (!through || need_dx) operand(c, a.w, w);
+    // (the products take one type: where dz = g, a float32 gradient is rounded to x's here)
+    if (through && (need_dx || need_dw)) operand(c, a.g, d);
+    MABA_TRY(prepare(c));
     if (!through) {
         // z again, rather than a copy kept by the forward pass: a 16-bit z would add its own
         // rounding to phi'(z), and a float32 one costs more traffic than the product
-        const int64_t ld = (N + 7) / 8 * 8;
+        d = written_operand(c, M, N);
         Product p;
         p.M = M, p.N = N, p.K = K;
         p.a[0] = x, p.b[0] = w;
         p.e.kind = E_LINEAR_BWD;
         p.e.act = a.act;
         p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.g);
-        p.e.out = c.ws.take((size_t)M * ld * esize(c.dt)), p.e.ldo = ld;
+        p.e.out = const_cast<void*>(d.p), p.e.ldo = d.sr, p.e.planes = d.sp;
         p.e.part_bias = pb, p.e.part_scale = ps;
         MABA_TRY(run(c, p));
-        if (need_dx || need_dw) MABA_TRY(own_operand(c, p.e.out, ld, M, N, d));
-    } else {
-        if (need_db) MABA_TRY(column_sums(c, side2(a.g), M, N, pb));
-        // the products take one type: a float32 gradient is rounded to x's here
-        if (need_dx || need_dw) MABA_TRY(operand(c, a.g, d));
+    } else if (need_db) {
+        MABA_TRY(column_sums(c, side2(a.g), M, N, pb));
     }
-    if (need_db) MABA_TRY(finish_columns(c, pb, blocks, N, a.dbias));
-    if (need_ds) MABA_TRY(finish_columns(c, ps, blocks, N, a.dscale));
+    if (!c.dry) MABA_TRY(finish_columns(c, pb, a.dbias, ps, a.dscale, blocks, N));
     if (need_dx) MABA_TRY(dx_product(c, M, N, 1, &d, &w, a.dx));
     if (need_dw) MABA_TRY(dw_product(c, M, 1, &d, x, &a.dw));
     return MABA_OK;
@@ -372,9 +440,10 @@ int ffn_product(Ctx& c, const FfnArgs& a, Product& p) {
     p.e.kind = given(a.g) ? E_GLU_BWD : E_GLU;
     if (p.M == 0) return MABA_OK;
     const bool as_is = skinny_takes(p, c.dt);
-    MABA_TRY(operand(c, a.x, p.a[0], as_is));
-    MABA_TRY(operand(c, a.wg, p.b[0], as_is));
-    return operand(c, a.wu, p.b[1], as_is);
+    operand(c, a.x, p.a[0], as_is);
+    operand(c, a.wg, p.b[0], as_is);
+    operand(c, a.wu, p.b[1], as_is);
+    return prepare(c);
 }
 
 int ffn_forward(Ctx& c, const FfnArgs& a) {
@@ -394,16 +463,12 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     if (!given(a.dx) && !given(a.dwg) && !given(a.dwu)) return MABA_OK;
     Product p;
     MABA_TRY(ffn_product(c, a, p));
-    const int64_t ld = (p.N + 7) / 8 * 8;
     // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
     // the one rounding between the two passes
+    const Matrix d[2] = {written_operand(c, M, p.N), written_operand(c, M, p.N)};
     p.e.res = side2(a.g);
-    p.e.out = c.ws.take((size_t)M * ld * esize(c.dt)), p.e.ldo = ld;
-    p.e.out2 = c.ws.take((size_t)M * ld * esize(c.dt));
+    p.e.out = const_cast<void*>(d[0].p), p.e.out2 = const_cast<void*>(d[1].p), p.e.ldo = d[0].sr, p.e.planes = d[0].sp;
     MABA_TRY(run(c, p));
-    Matrix d[2];
-    MABA_TRY(own_operand(c, p.e.out, ld, M, p.N, d[0]));
-    MABA_TRY(own_operand(c, p.e.out2, ld, M, p.N, d[1]));
     if (given(a.dx)) MABA_TRY(dx_product(c, M, p.N, 2, d, p.b, a.dx));
     const maba_tensor* dw[2] = {a.dwg, a.dwu};
     if (given(a.dwg) && given(a.dwu) && a.dwg->stride[0] == a.dwu->stride[0])
@@ -451,7 +516,7 @@ int check_ffn(const FfnArgs& a, bool backward) {
 }
 
 template <typename Args, typename F> size_t query(const Args& a, F op) {
-    Ctx c{a.x->dtype, true, {}, nullptr};
+    Ctx c{a.x->dtype, true, {}, nullptr, {}};
     return op(c, a) == MABA_OK ? c.ws.used : 0;
 }
 
@@ -460,7 +525,7 @@ int execute(const Args& a, F op, const char* name, void* workspace, size_t bytes
     const size_t need = query(a, op);
     if (need > 0 && (workspace == nullptr || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
         return set_error(MABA_ERR_WORKSPACE, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", name, need, bytes);
-    Ctx c{a.x->dtype, false, {static_cast<unsigned char*>(workspace), 0}, as_stream(stream)};
+    Ctx c{a.x->dtype, false, {static_cast<unsigned char*>(workspace), 0}, as_stream(stream), {}};
     return op(c, a);
 }
 

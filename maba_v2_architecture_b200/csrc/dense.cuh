@@ -53,6 +53,7 @@ struct Epilogue {
     void* out = nullptr;   // row-major, unit column stride
     void* out2 = nullptr;  // laid out like out: du of E_GLU_BWD, C1 of F_PAIR
     int64_t ldo = 0;
+    int64_t planes = 0;    // float32, E_LINEAR_BWD and E_GLU_BWD: out (out2) receives bf16 planes, this far apart
     Side bias, scale, res;
     float* part_bias = nullptr;   // E_LINEAR_BWD: [row blocks][N] column sums of dz
     float* part_scale = nullptr;  // and of g * act(z + bias)
@@ -107,9 +108,14 @@ template <typename T> int skinny_product(const Product& p, cudaStream_t s);
 // dense_tc.cu: tensor cores.  Operands as tc_readable() accepts them (float32: as planes);
 // column sums per TC_ROWS rows; T is the type of what the epilogue reads and writes.
 constexpr int TC_ROWS = 32;
+struct Plan {
+    int cg = 1, bn = 32;  // CTAs per tile, columns of the MMA
+    int splits = 1;       // of the contraction
+};
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
-int tc_splits(const Product& p, int dt);
-template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s);
+Plan tc_plan(const Product& p, int dt);
+template <typename T>
+int tc_product(const Product& p, const Plan& plan, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);
 
 }  // namespace dense

@@ -35,6 +35,7 @@
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 
+#include <cmath>
 #include <type_traits>
 
 namespace maba {
@@ -196,6 +197,20 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
             }
         }
     }
+}
+// The next of a float32 value's three bf16 planes (dense.cu's split_planes); what it leaves
+// stays in z.
+__device__ __forceinline__ float next_plane(float& z) {
+    float v = __bfloat162float(__float2bfloat16_rn(z));
+    if (!isfinite(v)) {
+        if (!isfinite(z)) {  // the first plane alone
+            v = z, z = 0.f;
+            return v;
+        }
+        v = __bfloat162float(__float2bfloat16_rz(z));
+    }
+    z -= v;
+    return v;
 }
 template <typename T, bool FRAG> __device__ __forceinline__ void put_chunk(const float* z, bool f32, unsigned char* st, int lane) {
     if (sizeof(T) == 4 || f32) {
@@ -463,7 +478,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         const int width = DUAL ? a.bn / 2 : a.bn;
         const bool has_side = SIDE && e.res.p != nullptr;
         const bool side_f32 = sizeof(T) == 4 || e.res.f32;
-        const bool out_f32 = sizeof(T) == 4 || e.out_f32 || (KIND == E_STORE && a.splits > 1);
+        // (the gradients of float32 operands leave as planes)
+        constexpr bool TO_PLANES = MODE == 2 && (KIND == E_LINEAR_BWD || KIND == E_GLU_BWD);
+        const bool out_f32 = !TO_PLANES && (sizeof(T) == 4 || e.out_f32 || (KIND == E_STORE && a.splits > 1));
+        using OT = typename std::conditional<TO_PLANES, __nv_bfloat16, T>::type;
         struct Chunk {
             int row0, col0, rows, cols;  // rows, cols: of 32, inside the matrix
         };
@@ -534,7 +552,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 else bulk_wait_read<0>();
             }
             __syncwarp();
-            put_chunk<T, FRAG>(z, out_f32, buf, lane);
+            put_chunk<OT, FRAG>(z, out_f32, buf, lane);
             if (a.out_tma) {
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -646,6 +664,16 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 });
                 side_used();
             }
+            if (TO_PLANES) {
+#pragma unroll
+                for (int pl = 0; pl < (KIND == E_GLU_BWD ? 6 : 3); ++pl) {
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = next_plane(pl < 3 ? z[j] : w[j]);
+                    store(k, v, pl < 3 ? &tout : &tout2, nullptr, e.ldo, pl % 3);
+                }
+                return;
+            }
             if (KIND == E_STORE && a.splits > 1)
                 store(k, z, &tout, a.partial + (int64_t)(t.split * a.pairs + t.pair) * a.M * a.ldp, a.ldp,
                       t.split * a.pairs + t.pair);
@@ -743,10 +771,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
 // --------------------------------------------------------------------------
 // host side
 // --------------------------------------------------------------------------
-struct Plan {
-    int cg = 1, bn = 32, splits = 1;
-};
-
 inline int b_rows_of(int cg, int bn) { return bn / cg; }
 inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
     const int r = b_rows_of(cg, bn);
@@ -766,29 +790,29 @@ int mode_of(const Product& p, int dt) {
 // hold a unit's sums bound bn in modes 1 and 2.  Splits also bound what one accumulation
 // truncates: at most 16,384 indices.
 Plan plan_of(const Product& p, int mode) {
-    const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE;
-    const bool b_mn = store;
-    const int64_t kblocks = ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
-    const int64_t pairs = p.form == F_PAIR ? 2 : 1;
+    const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE, b_mn = store;
+    const int kblocks = (int)ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
+    const int pairs = p.form == F_PAIR ? 2 : 1;
     const int planes = mode == 2 ? 3 : 1, terms = mode == 2 ? 6 : 1;
-    int64_t fewest = store && mode == 0 ? ceil_div(kblocks, 256) : 1;
+    const int fewest = store && mode == 0 ? (kblocks + 255) / 256 : 1;
+    const double out = 8.0 * pairs * (double)p.M * (double)p.N / 3500.0;  // one split's sums, written and read
     Plan best;
     double least = 1e300;
     for (int cg = 1; cg <= 2; ++cg) {
-        const int most = mode == 2 ? 128 : (cg == 2 ? 256 : 192);
+        const int most = mode == 2 ? 128 : (cg == 2 ? 256 : 192), slots = sm_count() / cg;
+        const double rows = (double)ceil_div(p.M, 128 * cg) * pairs;
         for (int bn = dual ? 64 : 32; bn <= most; bn += dual ? 64 : 32) {
-            const int64_t tiles = ceil_div(p.M, 128 * cg) * ceil_div(p.N, dual ? bn / 2 : bn) * pairs;
-            const int64_t slots = sm_count() / cg;
+            const double tiles = rows * (double)ceil_div(p.N, dual ? bn / 2 : bn);
             const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, b_mn)) / 60.0;
             const double kcost = mma > load ? mma : load;
-            for (int64_t splits = fewest; splits <= (store ? fewest + 15 : 1) && splits <= kblocks; ++splits) {
-                const int64_t units = tiles * splits;
-                const double waves = (double)ceil_div(units, slots);
-                const double kb = (double)ceil_div(kblocks, splits);
-                double t = waves * kb * kcost + 2000.0 + 12.0 * bn;
-                // the partial sums, written and read: bytes at ~3,500 per cycle over the GPU, and a launch
-                if (splits > 1) t += 2000.0 + 8.0 * (double)splits * pairs * p.M * p.N / 3500.0;
-                if (t < least) least = t, best = Plan{cg, bn, (int)splits};
+            for (int i = 0; i < (store ? 16 : 1); ++i) {
+                const int kb = (kblocks + fewest + i - 1) / (fewest + i);  // blocks of a split
+                const int splits = (kblocks + kb - 1) / kb;                // none of them empty
+                const double waves = std::ceil(tiles * splits / slots);
+                // (a bit more for the partial sums: a second kernel)
+                const double t = waves * kb * kcost + 2000.0 + 12.0 * bn + (splits > 1 ? 2000.0 + splits * out : 0.0);
+                if (t < least) least = t, best = Plan{cg, bn, splits};
+                if (waves * kb * kcost < 2000.0 || kb == 1) break;  // (more splits cannot pay)
             }
         }
     }
@@ -849,17 +873,14 @@ bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t 
     return rows == 1 || (ld % 8 == 0 && ld >= cols);
 }
 
-int tc_splits(const Product& p, int dt) {
-    const int64_t kblocks = ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
-    return (int)ceil_div(kblocks, ceil_div(kblocks, plan_of(p, mode_of(p, dt)).splits));  // none is empty
-}
+Plan tc_plan(const Product& p, int dt) { return plan_of(p, mode_of(p, dt)); }
 
-template <typename T> int tc_product(const Product& p, float* partial, int64_t ldp, cudaStream_t s) {
+template <typename T>
+int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cudaStream_t s) {
     if (encode_fn() == nullptr) return set_error(MABA_ERR_CUDA, "dense: cuTensorMapEncodeTiled not found");
     constexpr int dt = sizeof(T) == 4 ? MABA_F32 : (std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16);
     constexpr int planes = dt == MABA_F32 ? 3 : 1, odt = dt == MABA_F16 ? MABA_F16 : MABA_BF16;
     const int mode = mode_of(p, dt);
-    const Plan pl = plan_of(p, mode);
     const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE, a_mn = p.a_mn, b_mn = store;
     TcArgs a{};
     a.M = p.M, a.N = p.N;
@@ -883,7 +904,8 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
     // staging: two buffers each way where that leaves enough stages for the products, else fewer
     const int epi = mode == 0 ? Warps<0>::EPI : Warps<1>::EPI, threads = mode == 0 ? Warps<0>::THREADS : Warps<1>::THREADS;
-    const bool out_f32 = planes == 3 || p.e.out_f32 || a.splits > 1, side_f32 = planes == 3 || p.e.res.f32;
+    const bool to_planes = planes == 3 && (p.e.kind == E_LINEAR_BWD || p.e.kind == E_GLU_BWD);
+    const bool out_f32 = !to_planes && (planes == 3 || p.e.out_f32 || a.splits > 1), side_f32 = planes == 3 || p.e.res.f32;
     const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
     a.in_bytes = p.e.res.p ? (side_f32 ? 4096 : 2048) : 0;
     a.out_bytes = out_f32 ? 4096 : 2048;
@@ -903,26 +925,30 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     a.e = p.e;
     a.partial = partial;
     a.ldp = ldp;
-    // (before the maps: this call binds the device's context to the thread, which encoding a
-    // map needs and autograd's threads may not have)
     const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p, mode) : kernel_of<T, 1>(p, mode);
     if (kern == nullptr) return set_error(MABA_ERR_UNSUPPORTED, "dense(tcgen05): built with another register count");
+    // (before the maps: this call binds the device's context to the thread, which encoding a
+    // map needs and autograd's threads may not have)
     cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     CUtensorMap m[7];
     const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = p.form == F_SUM || dual ? 2 : 1;
     const int box = dual ? pl.bn / 2 : a.b_rows;
     bool ok = true;
-    for (int i = 0; i < 2; ++i) {
-        ok = ok && operand_map(&m[i], odt, p.a[i < na ? i : 0], planes, p.M, p.K, a_mn, 128);
-        ok = ok && operand_map(&m[2 + i], odt, p.b[i < nb ? i : 0], planes, p.N, p.K, b_mn, box);
-    }
+    for (int i = 0; i < na; ++i) ok = ok && operand_map(&m[i], odt, p.a[i], planes, p.M, p.K, a_mn, 128);
+    for (int i = 0; i < nb; ++i) ok = ok && operand_map(&m[2 + i], odt, p.b[i], planes, p.N, p.K, b_mn, box);
     if (!ok) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
+    if (na == 1) m[1] = m[0];
+    if (nb == 1) m[3] = m[2];
     m[4] = m[5] = m[6] = m[0];
     a.side_tma = p.e.res.p && p.e.res.sc == 1 &&
                  chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1);
     if (a.splits > 1) {
         a.out_tma = chunk_map(&m[5], MABA_F32, partial, p.M, p.N, ldp, a.splits * a.pairs);
+    } else if (to_planes) {
+        a.out_tma = chunk_map(&m[5], MABA_BF16, p.e.out, p.M, p.N, p.e.ldo, 3) &&
+                    (!p.e.out2 || chunk_map(&m[6], MABA_BF16, p.e.out2, p.M, p.N, p.e.ldo, 3));
+        if (!a.out_tma) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     } else {
         a.out_tma = chunk_map(&m[5], out_f32 ? MABA_F32 : odt, p.e.out, p.M, p.N, p.e.ldo, 1) &&
                     (!p.e.out2 || chunk_map(&m[6], out_f32 ? MABA_F32 : odt, p.e.out2, p.M, p.N, p.e.ldo, 1));
@@ -943,9 +969,9 @@ template <typename T> int tc_product(const Product& p, float* partial, int64_t l
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
 }
-template int tc_product<float>(const Product&, float*, int64_t, cudaStream_t);
-template int tc_product<__half>(const Product&, float*, int64_t, cudaStream_t);
-template int tc_product<__nv_bfloat16>(const Product&, float*, int64_t, cudaStream_t);
+template int tc_product<float>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
+template int tc_product<__half>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
+template int tc_product<__nv_bfloat16>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
 
 int device_error_take(cudaStream_t s, int* out) {
     int v = 0;

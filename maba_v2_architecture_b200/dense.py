@@ -42,11 +42,12 @@ def _check_device(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
 
 
 def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, n: int, k: int) -> None:
+    if w.device == x.device and w.dtype is x.dtype and w.shape == (n, k):
+        return
     _check_device(w, name, x)
     if w.dtype is not x.dtype:
         raise TypeError(f"Tensor dtypes must match, but got {x.dtype} for x and {w.dtype} for {name}")
-    if w.shape != (n, k):
-        raise ValueError(f"{name} shape {list(w.shape)} must be [{n}, {k}]")
+    raise ValueError(f"{name} shape {list(w.shape)} must be [{n}, {k}]")
 
 
 def _check_x(x: torch.Tensor, w: torch.Tensor, name: str) -> Tuple[int, int]:
@@ -64,6 +65,8 @@ def _check_x(x: torch.Tensor, w: torch.Tensor, name: str) -> Tuple[int, int]:
 
 
 def _check_side(t: torch.Tensor, name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
+    if t.device == x.device and t.dtype is x.dtype and t.shape == shape:
+        return
     _check_device(t, name, x)
     if t.dtype is not x.dtype and not (f32 and t.dtype is torch.float32):
         raise TypeError(f"{name} must be {x.dtype}{' or torch.float32' if f32 else ''}, got {t.dtype}")
@@ -103,23 +106,20 @@ def _check_out(out: torch.Tensor, x: torch.Tensor, shape, inputs, residual) -> N
             raise ValueError("out overlaps residual without being the same tensor")
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream without its Stream object
+_current_device = torch._C._cuda_getDevice
+
+
 def _call(fn, size, x: torch.Tensor, head, size_args) -> None:
     """Runs one entry on x's device (made current where it is not: the C entries launch on the current
-    device).  ``size_args`` None: most calls of the entry need no scratch memory, so it is tried
-    without; it refuses before it launches anything."""
-    index = x.device.index
-    if index != torch._C._cuda_getDevice():
+    device) with scratch memory of the size it asks for."""
+    index = x.get_device()
+    if index != _current_device():
         with torch.cuda.device(index):
             return _call(fn, size, x, head, size_args)
-    stream = N.stream_of(x)
-    if size_args is None:
-        rc = fn(*head, None, 0, stream)
-        if rc != N.ERR_WORKSPACE:
-            return None if rc == N.OK else N.check(rc, fn.__name__)
-        size_args = (*head[:len(size.argtypes) - 1], head[-1])
     nbytes = size(*size_args)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, stream)
+    rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
     if rc != N.OK:
         N.check(rc, fn.__name__)
 
@@ -139,12 +139,19 @@ def _vec(t: Optional[torch.Tensor]) -> Optional[bytes]:
 # ---------------------------------------------------------------------------
 def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
     if out is None:
-        out = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype or x.dtype, device=x.device)
+        dt = out_dtype or x.dtype
+        out = x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dt)
     if out.numel() == 0:
         return out
     lib = N.lib()
-    _call(lib.maba_linear, lib.maba_linear_workspace_size, x,
-          (_mat(x), _mat(weight), _vec(bias), act, _vec(scale), _mat(residual), _mat(out)), None)
+    head = (_mat(x), N.pack_matrix(weight), _vec(bias), act, _vec(scale), _mat(residual), _mat(out))
+    index = x.get_device()
+    # most calls need no scratch memory: tried without (the entry refuses before it launches anything)
+    rc = lib.maba_linear(*head, None, 0, _raw_stream(index)) if index == _current_device() else N.ERR_WORKSPACE
+    if rc == N.ERR_WORKSPACE:
+        _call(lib.maba_linear, lib.maba_linear_workspace_size, x, head, (head[0], head[1], head[6]))
+    elif rc != N.OK:
+        N.check(rc, "maba_linear")
     return out
 
 
@@ -256,12 +263,17 @@ def b200_linear_backward(
 # ---------------------------------------------------------------------------
 def _gated_ffn(x, w_gate, w_up, act, out):
     if out is None:
-        out = torch.empty((*x.shape[:-1], w_gate.shape[0]), dtype=x.dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], w_gate.shape[0]))
     if out.numel() == 0:
         return out
     lib = N.lib()
-    _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, x, (_mat(x), _mat(w_gate), _mat(w_up), act, _mat(out)),
-          None)
+    head = (_mat(x), N.pack_matrix(w_gate), N.pack_matrix(w_up), act, _mat(out))
+    index = x.get_device()
+    rc = lib.maba_gated_ffn(*head, None, 0, _raw_stream(index)) if index == _current_device() else N.ERR_WORKSPACE
+    if rc == N.ERR_WORKSPACE:  # (as in _linear)
+        _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, x, head, (*head[:3], head[4]))
+    elif rc != N.OK:
+        N.check(rc, "maba_gated_ffn")
     return out
 
 
