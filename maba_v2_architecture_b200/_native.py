@@ -145,11 +145,13 @@ _pack = struct.Struct("@Pii12q").pack  # a MabaTensor
 
 def pack_matrix(t: torch.Tensor) -> bytes:
     """Descriptor of a 2-D device tensor as bytes (a third of a MabaTensor's cost to make)."""
-    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 2, *t.shape, 0, 0, 0, 0, *t.stride(), 0, 0, 0, 0)
+    rows, cols = t.shape
+    sr, sc = t.stride()
+    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 2, rows, cols, 0, 0, 0, 0, sr, sc, 0, 0, 0, 0)
 
 
 def pack_vector(t: torch.Tensor) -> bytes:
-    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 1, *t.shape, 0, 0, 0, 0, 0, *t.stride(), 0, 0, 0, 0, 0)
+    return _pack(t.data_ptr(), DTYPE_CODES[t.dtype], 1, t.shape[0], 0, 0, 0, 0, 0, t.stride(0), 0, 0, 0, 0, 0)
 
 
 def ref(d: Optional[MabaTensor]):

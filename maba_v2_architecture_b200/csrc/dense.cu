@@ -63,11 +63,11 @@ struct Jobs {
 template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Jobs jobs) {
     __shared__ float tile[32][65];
     const Job& b = jobs.j[blockIdx.y];
-    const int tiles_c = (int)((b.cols + 63) / 64);
+    const unsigned tiles_c = (unsigned)((b.cols + 63) / 64);
     const int64_t tiles = (b.rows + 31) / 32 * tiles_c;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const int64_t r0 = t / tiles_c * 32, c0 = t % tiles_c * 64;
+        const int64_t tr = tiles >> 32 ? t / tiles_c : (unsigned)t / tiles_c, r0 = tr * 32, c0 = (t - tr * tiles_c) * 64;
         if (b.src.sc <= b.src.sr) {  // lanes along the columns
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

@@ -30,11 +30,11 @@
 // Every mbarrier wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
 // freed and the error word behind maba_device_error() is set.
-#include "activations.cuh"
 #include "dense.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -102,19 +102,68 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// phi and phi' of 16-bit operands on the SFU's exponential and reciprocal (a few float32
-// ulp); of float32 ones (EXACT) as dense.cuh has them.
-template <int ACT, bool EXACT> __device__ __forceinline__ float act16(float z) {
-    if (ACT == ACT_SILU && !EXACT) return silu_f(z);
-    return act_f(z, ACT);
+// Pairs of float32 in one instruction each: the epilogue's issue slots are what the products
+// leave it.
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
 }
-template <int ACT, bool EXACT> __device__ __forceinline__ void act_grad16(float z, float& y, float& d) {
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
+// a = a * b + c
+__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ float exp2_sfu(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_sfu(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / (1 + e^-z): the SFU's exponential and reciprocal, a few float32 ulp (e^-z past float32
+// gives 1 / inf = 0)
+__device__ __forceinline__ void sigmoid2(float z0, float z1, float& s0, float& s1) {
+    s0 = z0, s1 = z1;
+    mul2(s0, s1, -1.4426950408889634f, -1.4426950408889634f);
+    s0 = exp2_sfu(s0), s1 = exp2_sfu(s1);
+    add2(s0, s1, 1.f, 1.f);
+    s0 = rcp_sfu(s0), s1 = rcp_sfu(s1);
+}
+// phi and phi' of a pair; of float32 operands (EXACT) as dense.cuh has them.
+template <int ACT, bool EXACT> __device__ __forceinline__ void act2(float& z0, float& z1) {
     if (ACT == ACT_SILU && !EXACT) {
-        const float s = sigmoid_f(z);
-        y = z * s;
-        d = s * (1.f + z * (1.f - s));
+        float s0, s1;
+        sigmoid2(z0, z1, s0, s1);
+        mul2(z0, z1, s0, s1);
     } else {
-        act_grad_f(z, ACT, y, d);
+        z0 = act_f(z0, ACT), z1 = act_f(z1, ACT);
+    }
+}
+template <int ACT, bool EXACT>
+__device__ __forceinline__ void act_grad2(float z0, float z1, float& y0, float& y1, float& d0, float& d1) {
+    if (ACT == ACT_SILU && !EXACT) {
+        float s0, s1;
+        sigmoid2(z0, z1, s0, s1);
+        y0 = z0, y1 = z1;
+        mul2(y0, y1, s0, s1);
+        d0 = s0, d1 = s1;  // phi' = s + y (1 - s)
+        fma2(d0, d1, -1.f, -1.f, 1.f, 1.f);
+        fma2(d0, d1, y0, y1, s0, s1);
+    } else {
+        act_grad_f(z0, ACT, y0, d0), act_grad_f(z1, ACT, y1, d1);
     }
 }
 template <typename F> __device__ __forceinline__ void with_act(int act, F f) {
@@ -145,10 +194,18 @@ template <typename E> __device__ __forceinline__ E* element(unsigned char* st, i
 // (src, dst: the chunk's first element)
 template <typename E>
 __device__ __noinline__ void stage_in(unsigned char* st, const E* src, int64_t sr, int64_t sc, int rows, int cols, int lane) {
-    for (int r = 0; r < 32; ++r) *element<E>(st, r, lane) = r < rows && lane < cols ? src[r * sr + lane * sc] : E(0);
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 16) {
+        E v[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = r0 + r < rows && lane < cols ? src[(r0 + r) * sr + lane * sc] : E(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) *element<E>(st, r0 + r, lane) = v[r];
+    }
 }
 template <typename E>
 __device__ __noinline__ void stage_out(unsigned char* st, E* dst, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll 8
     for (int r = 0; r < rows; ++r)
         if (lane < cols) dst[r * ld + lane] = *element<E>(st, r, lane);
 }
@@ -159,7 +216,7 @@ __device__ __noinline__ void stage_out(unsigned char* st, E* dst, int64_t ld, in
 __device__ __forceinline__ int frag_row(int j, int lane) { return (j >> 4) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2); }
 __device__ __forceinline__ int frag_col(int j, int lane) { return ((j >> 2) & 3) * 8 + (lane & 3) * 2 + (j & 1); }
 
-// f(j, value) for the 32 elements of a staged chunk
+// f(j, value, next value) for the 32 elements of a staged chunk, in pairs
 template <typename T, bool FRAG, typename F>
 __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane, F f) {
     if (sizeof(T) == 4 || f32) {
@@ -167,13 +224,13 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
                 const float2 x = *reinterpret_cast<const float2*>(element<float>(st, frag_row(j, lane), frag_col(j, lane)));
-                f(j, x.x), f(j + 1, x.y);
+                f(j, x.x, x.y);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float4 x = *reinterpret_cast<const float4*>(at32(st, lane, i));
-                f(4 * i, x.x), f(4 * i + 1, x.y), f(4 * i + 2, x.z), f(4 * i + 3, x.w);
+                f(4 * i, x.x, x.y), f(4 * i + 2, x.z, x.w);
             }
         }
     } else if constexpr (sizeof(T) == 2) {
@@ -182,7 +239,7 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
             for (int j = 0; j < 32; j += 2) {
                 const float2 x =
                     unpack2<T>(*reinterpret_cast<const uint32_t*>(element<uint16_t>(st, frag_row(j, lane), frag_col(j, lane))));
-                f(j, x.x), f(j + 1, x.y);
+                f(j, x.x, x.y);
             }
         } else {
 #pragma unroll
@@ -192,7 +249,7 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 x = unpack2<T>(w[e]);
-                    f(8 * i + 2 * e, x.x), f(8 * i + 2 * e + 1, x.y);
+                    f(8 * i + 2 * e, x.x, x.y);
                 }
             }
         }
@@ -236,7 +293,7 @@ template <typename T, bool FRAG> __device__ __forceinline__ void put_chunk(const
         }
     }
 }
-// f(z[j], v of j's column) for a vector of the chunk's 32 columns in shared memory
+// f(z[j], z[j + 1], v of their columns) for a vector of the chunk's 32 columns in shared memory
 template <bool FRAG, typename F> __device__ __forceinline__ void with_vector(float* z, const float* v, int lane, F f) {
     if (FRAG) {
 #pragma unroll
@@ -245,30 +302,25 @@ template <bool FRAG, typename F> __device__ __forceinline__ void with_vector(flo
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = (r >> 1) * 16 + g * 4 + (r & 1) * 2;
-                f(z[j], x.x), f(z[j + 1], x.y);
+                f(z[j], z[j + 1], x.x, x.y);
             }
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
             const float4 x = *reinterpret_cast<const float4*>(v + j);
-            f(z[j], x.x), f(z[j + 1], x.y), f(z[j + 2], x.z), f(z[j + 3], x.w);
+            f(z[j], z[j + 1], x.x, x.y), f(z[j + 2], z[j + 3], x.z, x.w);
         }
     }
 }
-// Column sums of a chunk (FRAG) over its 32 rows, in a fixed order: a lane's four rows, then
-// the eight lanes of a column.  Lane l returns column frag_sum_col(l).
+// Column sums of a chunk (FRAG) over its 32 rows, in a fixed order: v holds a lane's own of its
+// eight columns (8 g + 2 (lane % 4) + e at 2 g + e); those of the eight lanes of a column are
+// added.  Lane l returns column frag_sum_col(l).
 __device__ __forceinline__ int frag_sum_col(int lane) {
     const int q = ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
     return (q >> 1) * 8 + (lane & 3) * 2 + (q & 1);
 }
-__device__ __forceinline__ float frag_column_sum(const float* z, int lane) {
-    float v[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int j = (q >> 1) * 4 + (q & 1);
-        v[q] = (z[j] + z[j + 2]) + (z[j + 16] + z[j + 18]);
-    }
+__device__ __forceinline__ float frag_column_sum(float* v, int lane) {
 #pragma unroll
     for (int o = 16, n = 4; o > 2; o >>= 1, n >>= 1) {
         const bool hi = (lane & o) != 0;
@@ -607,59 +659,66 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             unsigned char* in = nullptr;
             const float *vs = vscale + c / CS * 32, *vb = vbias + c / CS * 32;
             if (KIND == E_LINEAR) {
-                if (e.bias.p) with_vector<FRAG>(z, vb, lane, [](float& x, float v) { x += v; });
+                if (e.bias.p) with_vector<FRAG>(z, vb, lane, add2);
                 with_act(e.act, [&](auto A) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]);
+                    for (int j = 0; j < 32; j += 2) act2<A.value, EXACT>(z[j], z[j + 1]);
                 });
-                if (e.scale.p) with_vector<FRAG>(z, vs, lane, [](float& x, float v) { x *= v; });
+                if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
                 if (has_side) {
                     in = side_ready(k);
-                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) { z[j] += g; });
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) { add2(z[j], z[j + 1], g0, g1); });
                     side_used();
                 }
             } else if (KIND == E_LINEAR_BWD) {
-                float y[32];
-                if (e.bias.p) with_vector<FRAG>(z, vb, lane, [](float& x, float v) { x += v; });
+                float sb[8] = {}, ss[8] = {};  // this lane's part of its eight columns' sums
+                if (e.bias.p) with_vector<FRAG>(z, vb, lane, add2);
                 in = side_ready(k);
                 with_act(e.act, [&](auto A) {
-                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) {
-                        float f, d;
-                        act_grad16<A.value, EXACT>(z[j], f, d);
-                        z[j] = g * d;
-                        y[j] = g * f;
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
+                        float y0, y1, d0, d1;
+                        act_grad2<A.value, EXACT>(z[j], z[j + 1], y0, y1, d0, d1);
+                        if (k.rows < 32 && frag_row(j, lane) >= k.rows) y0 = y1 = d0 = d1 = 0.f;  // whatever the bias is
+                        const int c = ((j >> 2) & 3) * 2;
+                        z[j] = g0, z[j + 1] = g1;
+                        mul2(z[j], z[j + 1], d0, d1);
+                        fma2(y0, y1, g0, g1, ss[c], ss[c + 1]);
+                        ss[c] = y0, ss[c + 1] = y1;
                     });
                 });
                 side_used();
-                if (e.scale.p) with_vector<FRAG>(z, vs, lane, [](float& x, float v) { x *= v; });
-                if (k.rows < 32) {  // rows past the last: no part in the sums, whatever the bias is
+                if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (frag_row(j, lane) >= k.rows) z[j] = y[j] = 0.f;
-                }
+                for (int j = 0; j < 32; j += 2) add2(sb[((j >> 2) & 3) * 2], sb[((j >> 2) & 3) * 2 + 1], z[j], z[j + 1]);
                 const int col = frag_sum_col(lane);
                 const int64_t at = (int64_t)(k.row0 >> 5) * a.N + k.col0 + col;
                 if (e.part_bias) {
-                    const float s = frag_column_sum(z, lane);
+                    const float s = frag_column_sum(sb, lane);
                     if (col < k.cols) e.part_bias[at] = s;
                 }
                 if (e.part_scale) {
-                    const float s = frag_column_sum(y, lane);
+                    const float s = frag_column_sum(ss, lane);
                     if (col < k.cols) e.part_scale[at] = s;
                 }
             } else if (KIND == E_GLU) {
                 with_act(e.act, [&](auto A) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) z[j] = act16<A.value, EXACT>(z[j]) * w[j];
+                    for (int j = 0; j < 32; j += 2) {
+                        act2<A.value, EXACT>(z[j], z[j + 1]);
+                        mul2(z[j], z[j + 1], w[j], w[j + 1]);
+                    }
                 });
             } else if (KIND == E_GLU_BWD) {
                 in = side_ready(k);
                 with_act(e.act, [&](auto A) {
-                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g) {
-                        float f, d;
-                        act_grad16<A.value, EXACT>(z[j], f, d);
-                        z[j] = g * w[j] * d;
-                        w[j] = g * f;
+                    with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
+                        float y0, y1, d0, d1;
+                        act_grad2<A.value, EXACT>(z[j], z[j + 1], y0, y1, d0, d1);
+                        mul2(d0, d1, w[j], w[j + 1]);
+                        w[j] = g0, w[j + 1] = g1;
+                        z[j] = g0, z[j + 1] = g1;
+                        mul2(w[j], w[j + 1], y0, y1);
+                        mul2(z[j], z[j + 1], d0, d1);
                     });
                 });
                 side_used();
@@ -842,26 +901,38 @@ bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols
 using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
                         const CUtensorMap, const CUtensorMap, const CUtensorMap);
 
-// The register split assumes REG_LAUNCH registers per thread at launch; with fewer, the
-// epilogue's increase would never complete, so such a build is not launched (nullptr).
-template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> Kernel checked() {
-    static const bool ok = [] {
-        cudaFuncAttributes fa{};
-        return cudaFuncGetAttributes(&fa, tc_kernel<T, CG, A_MN, B_MN, KIND, MODE>) == cudaSuccess && fa.numRegs == Warps<MODE>::REG_LAUNCH;
-    }();
-    return ok ? tc_kernel<T, CG, A_MN, B_MN, KIND, MODE> : nullptr;
+// A kernel ready to launch on the current device: its shared memory limit raised, and the
+// device's context bound to this thread, which encoding a tensor map needs (autograd's threads
+// come without one).  The register split assumes REG_LAUNCH registers per thread at launch; with
+// fewer, the epilogue's increase would never complete, so such a build is refused.
+template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> int ready(Kernel* out, int device) {
+    static std::atomic<uint64_t> done{0};
+    static thread_local uint64_t bound = 0;
+    const auto kern = tc_kernel<T, CG, A_MN, B_MN, KIND, MODE>;
+    *out = kern;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if ((done.load(std::memory_order_relaxed) & bound & bit) != 0) return MABA_OK;
+    cudaFuncAttributes fa{};
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e == cudaSuccess && fa.numRegs != Warps<MODE>::REG_LAUNCH)
+        return set_error(MABA_ERR_UNSUPPORTED, "dense(tcgen05): built with %d registers", fa.numRegs);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX);
+    if (e != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(e));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    bound |= bit;
+    return MABA_OK;
 }
 
-template <typename T, int CG> Kernel kernel_of(const Product& p, int mode) {
+template <typename T, int CG> int kernel_of(Kernel* k, const Product& p, int mode, int device) {
     constexpr int M = sizeof(T) == 4 ? 2 : 0;
     if constexpr (M == 0)
-        if (mode == 1) return checked<T, CG, false, false, E_LINEAR, 1>();
+        if (mode == 1) return ready<T, CG, false, false, E_LINEAR, 1>(k, device);
     switch (p.e.kind) {
-        case E_LINEAR: return checked<T, CG, false, false, E_LINEAR, M>();
-        case E_LINEAR_BWD: return checked<T, CG, false, false, E_LINEAR_BWD, M>();
-        case E_GLU: return checked<T, CG, false, false, E_GLU, M>();
-        case E_GLU_BWD: return checked<T, CG, false, false, E_GLU_BWD, M>();
-        default: return p.a_mn ? checked<T, CG, true, true, E_STORE, M>() : checked<T, CG, false, true, E_STORE, M>();
+        case E_LINEAR: return ready<T, CG, false, false, E_LINEAR, M>(k, device);
+        case E_LINEAR_BWD: return ready<T, CG, false, false, E_LINEAR_BWD, M>(k, device);
+        case E_GLU: return ready<T, CG, false, false, E_GLU, M>(k, device);
+        case E_GLU_BWD: return ready<T, CG, false, false, E_GLU_BWD, M>(k, device);
+        default: return p.a_mn ? ready<T, CG, true, true, E_STORE, M>(k, device) : ready<T, CG, false, true, E_STORE, M>(k, device);
     }
 }
 
@@ -925,12 +996,11 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.e = p.e;
     a.partial = partial;
     a.ldp = ldp;
-    const Kernel kern = pl.cg == 2 ? kernel_of<T, 2>(p, mode) : kernel_of<T, 1>(p, mode);
-    if (kern == nullptr) return set_error(MABA_ERR_UNSUPPORTED, "dense(tcgen05): built with another register count");
-    // (before the maps: this call binds the device's context to the thread, which encoding a
-    // map needs and autograd's threads may not have)
-    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
+    Kernel kern = nullptr;
+    MABA_TRY((pl.cg == 2 ? kernel_of<T, 2>(&kern, p, mode, device) : kernel_of<T, 1>(&kern, p, mode, device)));
     CUtensorMap m[7];
     const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = p.form == F_SUM || dual ? 2 : 1;
     const int box = dual ? pl.bn / 2 : a.b_rows;

@@ -65,7 +65,7 @@ def _check_x(x: torch.Tensor, w: torch.Tensor, name: str) -> Tuple[int, int]:
 
 
 def _check_side(t: torch.Tensor, name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
-    if t.device == x.device and t.dtype is x.dtype and t.shape == shape:
+    if t.device == x.device and t.shape == shape and (t.dtype is x.dtype or (f32 and t.dtype is torch.float32)):
         return
     _check_device(t, name, x)
     if t.dtype is not x.dtype and not (f32 and t.dtype is torch.float32):
@@ -138,20 +138,26 @@ def _vec(t: Optional[torch.Tensor]) -> Optional[bytes]:
 # the linear map
 # ---------------------------------------------------------------------------
 def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
+    # (one token's call is bound by this function: no helper calls, descriptors packed in place)
     if out is None:
-        dt = out_dtype or x.dtype
-        out = x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dt)
-    if out.numel() == 0:
+        out = x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype or x.dtype)
+    if x.numel() == 0:
         return out
+    pack = N.pack_matrix
+    plain = x.dim() == 2
+    dx, dw, do = pack(x) if plain else _mat(x), pack(weight), pack(out) if plain else _mat(out)
+    db = None if bias is None else N.pack_vector(bias)
+    ds = None if scale is None else N.pack_vector(scale)
+    dr = None if residual is None else (pack(residual) if plain else _mat(residual))
     lib = N.lib()
-    head = (_mat(x), N.pack_matrix(weight), _vec(bias), act, _vec(scale), _mat(residual), _mat(out))
     index = x.get_device()
-    # most calls need no scratch memory: tried without (the entry refuses before it launches anything)
-    rc = lib.maba_linear(*head, None, 0, _raw_stream(index)) if index == _current_device() else N.ERR_WORKSPACE
-    if rc == N.ERR_WORKSPACE:
-        _call(lib.maba_linear, lib.maba_linear_workspace_size, x, head, (head[0], head[1], head[6]))
-    elif rc != N.OK:
-        N.check(rc, "maba_linear")
+    rc = N.ERR_WORKSPACE
+    if index == _current_device():  # most calls need no scratch memory: tried without (refused before any launch)
+        rc = lib.maba_linear(dx, dw, db, act, ds, dr, do, None, 0, _raw_stream(index))
+    if rc:
+        if rc != N.ERR_WORKSPACE:
+            N.check(rc, "maba_linear")
+        _call(lib.maba_linear, lib.maba_linear_workspace_size, x, (dx, dw, db, act, ds, dr, do), (dx, dw, do))
     return out
 
 
@@ -202,7 +208,9 @@ def b200_linear(
     place and may be ``residual`` (a residual stream updated where it is), not another input.
     With the residual gates of MabaBlock as ``scale``: maba_sparse/model.py:107-108, 126-127.
     """
-    act = _activation(activation, True)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        _activation(activation, True)
     n, _ = _check_x(x, weight, "weight")
     shape = (*x.shape[:-1], n)
     if bias is not None:
@@ -211,7 +219,7 @@ def b200_linear(
         _check_side(scale, "scale", x, (n,))
     if residual is not None:
         _check_side(residual, "residual", x, shape)
-    if out_dtype is not None and out_dtype not in (x.dtype, torch.float32):
+    if out_dtype is not None and out_dtype is not torch.float32 and out_dtype is not x.dtype:
         raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
     if not x.is_cuda:
         N.require_cuda(x, op="linear")
@@ -264,16 +272,20 @@ def b200_linear_backward(
 def _gated_ffn(x, w_gate, w_up, act, out):
     if out is None:
         out = x.new_empty((*x.shape[:-1], w_gate.shape[0]))
-    if out.numel() == 0:
+    if x.numel() == 0:
         return out
+    pack = N.pack_matrix
+    plain = x.dim() == 2
+    dx, dg, du, do = pack(x) if plain else _mat(x), pack(w_gate), pack(w_up), pack(out) if plain else _mat(out)
     lib = N.lib()
-    head = (_mat(x), N.pack_matrix(w_gate), N.pack_matrix(w_up), act, _mat(out))
     index = x.get_device()
-    rc = lib.maba_gated_ffn(*head, None, 0, _raw_stream(index)) if index == _current_device() else N.ERR_WORKSPACE
-    if rc == N.ERR_WORKSPACE:  # (as in _linear)
-        _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, x, head, (*head[:3], head[4]))
-    elif rc != N.OK:
-        N.check(rc, "maba_gated_ffn")
+    rc = N.ERR_WORKSPACE
+    if index == _current_device():  # (as in _linear)
+        rc = lib.maba_gated_ffn(dx, dg, du, act, do, None, 0, _raw_stream(index))
+    if rc:
+        if rc != N.ERR_WORKSPACE:
+            N.check(rc, "maba_gated_ffn")
+        _call(lib.maba_gated_ffn, lib.maba_gated_ffn_workspace_size, x, (dx, dg, du, act, do), (dx, dg, du, do))
     return out
 
 
