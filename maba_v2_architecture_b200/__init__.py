@@ -3,7 +3,9 @@
 DGDA chunked prefill and decode step, DG-Indexer pooling + scoring + top-k,
 and MABA-SA three-stream attention with gate superposition, as hand-written
 CUDA kernels behind a C ABI (include/maba_b200.h, libmaba_b200.so), exposed
-with the reference project's op, registry and layer interfaces.
+with the reference project's op, registry and layer interfaces; and the dense
+operators of the model's blocks (linear map with its epilogue, gated feed-forward
+block), which have gradients.
 """
 from .config import MabaSparseConfig, MabaConfig, get_101m_config
 from .dense import b200_gated_ffn, b200_gated_ffn_backward, b200_linear, b200_linear_backward
@@ -25,7 +27,7 @@ from .dispatcher import (
     stream_superposition,
 )
 from .layers import ConvState, DGDALayer, DGIndexer, DecoupledGatedDeltaAttention, DeltaGuidedCentroidIndexer
-from .layers import MABASALayer, MabaSparseAttention
+from .layers import MABASALayer, MabaSparseAttention, SwiGLUFFN
 from .ops import (
     b200_compute_centroids,
     b200_decode_cache_append,

@@ -37,6 +37,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native as N
+from .dense import b200_gated_ffn, b200_linear
 from .ops import (b200_compute_centroids, b200_dgda_frontend, b200_dgda_prefill, b200_hca_pool, b200_index_topk,
                   b200_sa_attention)
 
@@ -222,15 +223,21 @@ class MabaEngine:
     ``MabaEngine(config, state_dict)`` or ``MabaEngine.from_module(model)`` (any module with
     the reference's parameter names, e.g. an unmodified reference model).  ``dtype`` is the
     compute dtype of weights and activations (bfloat16 for the benchmarks, float32 for exact
-    parity checks); the residual stream, recurrent states and logits stay float32."""
+    parity checks); the residual stream, recurrent states and logits stay float32.
+
+    ``fused_dense`` runs the blocks' projections of a prefill on this library's dense operators:
+    the gated feed-forward block as one kernel, and every output projection adding its gated result
+    to the residual stream in its epilogue (``b200_gated_ffn``, ``b200_linear``), in place of matrix
+    products with separate SwiGLU and residual kernels.  Same function; sums are ordered differently."""
 
     def __init__(self, config, state_dict: Dict[str, torch.Tensor], device="cuda", dtype=torch.bfloat16,
-                 ablation_mode: Optional[str] = None):
+                 ablation_mode: Optional[str] = None, fused_dense: bool = False):
         self.shape = s = ModelShape.from_config(config, ablation_mode)
         if s.ablation not in ("full", "pure_dgda"):
             raise NotImplementedError(f"MabaEngine: ablation_mode={s.ablation!r}")
         self.device = torch.device(device)
         self.dtype = dtype
+        self.fused_dense = fused_dense
         dev, dt = self.device, dtype
         N.require_cuda(torch.empty(0, device=dev), op="MabaEngine")
         sd = state_dict
@@ -253,6 +260,27 @@ class MabaEngine:
                                            N.stream_of(x))
         N.check(rc, "maba_rmsnorm_residual")
 
+    def _input(self, h, W):
+        """Input projection of a mixer."""
+        sa = isinstance(W, _SAWeights)
+        if self.fused_dense:
+            return b200_linear(h, W.w_in, W.bias if sa else None)
+        return torch.addmm(W.bias_dt, h, W.w_in.t()) if sa else _lin(h, W.w_in)
+
+    def _output(self, x, a, w, gate, norm_w, h):
+        """x += gate * (a w^T), then h = the next RMSNorm of x."""
+        if self.fused_dense:
+            b200_linear(a, w, scale=gate, residual=x, out=x)
+            self._norm(x, None, None, norm_w, h)
+        else:
+            self._norm(x, _lin_f32(a, w), gate, norm_w, h)
+
+    def _ffn_inner(self, h, w_gu):
+        if self.fused_dense:
+            inner = w_gu.shape[0] // 2
+            return b200_gated_ffn(h, w_gu[:inner], w_gu[inner:])
+        return self._swiglu(_lin(h, w_gu))
+
     def _swiglu(self, u):
         out = torch.empty(u.shape[0], u.shape[1] // 2, dtype=u.dtype, device=u.device)
         N.check(N.lib().maba_swiglu(N.ref(N.desc(u)), N.ref(N.desc(out)), N.stream_of(u)), "maba_swiglu")
@@ -273,11 +301,11 @@ class MabaEngine:
         h = torch.empty(Ntok, s.dim, dtype=dt, device=self.device)
         self._norm(x, None, None, self.layers[0].n1 if self.layers else self.final_norm, h)
         for li, L in enumerate(self.layers):
-            y = self._sa_prefill(L, h, B, T, li, session) if L.attn else self._dgda_prefill(L, h, B, T, li, session)
-            self._norm(x, y, L.g1, L.n2, h)
-            f = _lin_f32(self._swiglu(_lin(h, L.w_gu)), L.w_down)
+            mix = self._sa_prefill if L.attn else self._dgda_prefill
+            a, w_out = mix(L, h, B, T, li, session)
+            self._output(x, a, w_out, L.g1, L.n2, h)
             nxt = self.layers[li + 1].n1 if li + 1 < len(self.layers) else self.final_norm
-            self._norm(x, f, L.g2, nxt, h)
+            self._output(x, self._ffn_inner(h, L.w_gu), L.w_down, L.g2, nxt, h)
         hv = h.view(B, T, s.dim)
         if last_only:
             hv = hv[:, -1:]
@@ -287,7 +315,7 @@ class MabaEngine:
 
     def _dgda_prefill(self, L: _Layer, h, B, T, li, session):
         s, W = self.shape, L.mix
-        P = _lin(h, W.w_in).view(B, T, -1)
+        P = self._input(h, W).view(B, T, -1)
         cols, c0 = [], 0
         for wd in W.widths:
             cols.append(P[:, :, c0:c0 + wd])
@@ -302,12 +330,12 @@ class MabaEngine:
         if session is not None:
             session.states[li].copy_(S)
             session.hists[li].copy_(torch.cat(nh, dim=1))
-        return _lin_f32(o.transpose(1, 2).reshape(B * T, H * dv), W.w_o)
+        return o.transpose(1, 2).reshape(B * T, H * dv), W.w_o
 
     def _sa_prefill(self, L: _Layer, h, B, T, li, session):
         s, W = self.shape, L.mix
         H, dc = s.n_heads, s.d_c
-        P = torch.addmm(W.bias_dt, h, W.w_in.t()).view(B, T, -1)
+        P = self._input(h, W).view(B, T, -1)
         c = P[:, :, W.off_c:W.off_c + dc]
         qhat = P[:, :, W.off_q:W.off_q + H * dc].view(B, T, H, dc)
         qi = P[:, :, W.off_qi:W.off_qi + s.d_idx]
@@ -325,7 +353,7 @@ class MabaEngine:
             cache.cent[:, :cent.shape[1]] = cent
             if hca is not None:
                 cache.hca[:, :hca.shape[1]] = hca
-        return _lin_f32(o_lat.reshape(B * T, H * dc), W.w_ov)
+        return o_lat.reshape(B * T, H * dc), W.w_ov
 
     # ------------------------------------------------------------------ decode
     def new_session(self, batch: int, max_len: int) -> "DecodeSession":

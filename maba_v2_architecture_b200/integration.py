@@ -14,6 +14,8 @@ its layers) run the hot path on the sm_100a kernels:
   fused-kernel version, and ``DGDALayer.forward`` / ``step`` (dgda.py:166-287,
   whose conv, gates and k norm are separate torch ops) by the version with one
   input GEMM and the fused front-end kernel;
+* with ``patch_ffn=True``, ``SwiGLUFFN.forward`` (model.py:28-37) runs on the
+  dense operators, forward and backward;
 * ``MABA_STRICT_BACKEND=1`` is set so the reference dispatcher raises instead of
   silently falling back to its CPU reference.
 
@@ -43,7 +45,8 @@ _OURS = {
 }
 
 
-def install(maba_sparse: Optional[Any] = None, patch_layers: bool = True, strict: bool = True) -> Dict[str, Any]:
+def install(maba_sparse: Optional[Any] = None, patch_layers: bool = True, strict: bool = True,
+            patch_ffn: bool = False) -> Dict[str, Any]:
     if maba_sparse is None:
         import maba_sparse  # noqa: F811
     import importlib
@@ -59,6 +62,7 @@ def install(maba_sparse: Optional[Any] = None, patch_layers: bool = True, strict
         os.environ["MABA_STRICT_BACKEND"] = "1"
     os.environ["MABA_BACKEND"] = "triton"
     disp.clear_dispatcher_cache()
+    patches = []
     if patch_layers:
         sa_mod = importlib.import_module("maba_sparse.layers.sparse_attention")
         ix_mod = importlib.import_module("maba_sparse.layers.indexer")
@@ -69,9 +73,11 @@ def install(maba_sparse: Optional[Any] = None, patch_layers: bool = True, strict
                    (ref_ix, "forward", _layers.DGIndexer), (ref_dg, "forward", _layers.DGDALayer),
                    (ref_dg, "step", _layers.DGDALayer), (ref_dg, "_features", _layers.DGDALayer),
                    (ref_dg, "_in_proj_weight", _layers.DGDALayer)]
-        handle["methods"] = {(cls, name): cls.__dict__.get(name) for cls, name, _ in patches}
-        for cls, name, ours in patches:
-            setattr(cls, name, ours.__dict__[name])
+    if patch_ffn:
+        patches.append((importlib.import_module("maba_sparse.model").SwiGLUFFN, "forward", _layers.SwiGLUFFN))
+    handle["methods"] = {(cls, name): cls.__dict__.get(name) for cls, name, _ in patches}
+    for cls, name, ours in patches:
+        setattr(cls, name, ours.__dict__[name])
     handle["dispatcher"] = disp
     return handle
 

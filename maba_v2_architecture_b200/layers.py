@@ -25,6 +25,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .dense import b200_gated_ffn, b200_linear
 from .dispatcher import dispatch_compute_centroids, dispatch_dgda_prefill, dispatch_dgda_step, dispatch_index_topk
 from .ops import (absorb_queries, b200_dgda_frontend, b200_hca_pool, b200_index_topk, b200_sa_attention,
                   expand_values)
@@ -366,3 +367,27 @@ class MabaSparseAttention(nn.Module):
 
 
 MABASALayer = MabaSparseAttention
+
+
+class SwiGLUFFN(nn.Module):
+    """SwiGLU feed-forward block w_down(silu(w_gate x) * w_up x) (maba_sparse/model.py:28-37).
+
+    Two kernels forward: the gated block, whose projections are never stored, and the down
+    projection; differentiable.  With ``residual`` and ``gate`` ([dim], sigmoid(res_gate)) the down
+    projection returns residual + gate * ffn(x), the block's gated residual add
+    (maba_sparse/model.py:107-108); a float32 residual makes the result float32."""
+
+    def __init__(self, config: Optional[Any] = None, dim: int = 640, intermediate_size: int = 1728) -> None:
+        super().__init__()
+        if config is not None:
+            dim = getattr(config, "dim", getattr(config, "d_model", dim))
+            intermediate_size = getattr(config, "intermediate_size", intermediate_size)
+        self.w_gate = nn.Linear(dim, intermediate_size, bias=False)
+        self.w_up = nn.Linear(dim, intermediate_size, bias=False)
+        self.w_down = nn.Linear(intermediate_size, dim, bias=False)
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+        a = b200_gated_ffn(x, self.w_gate.weight, self.w_up.weight)
+        out_dtype = residual.dtype if residual is not None else None
+        return b200_linear(a, self.w_down.weight, scale=gate, residual=residual, out_dtype=out_dtype)

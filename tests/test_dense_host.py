@@ -115,3 +115,50 @@ def test_c_entry_refusals():
     need = lib.maba_gated_ffn_backward_workspace_size(o, x, w, w, d((4, 16)), None, None)
     assert need >= 2 * 4 * 8 * 4
     assert lib.maba_linear_backward(o, x, w, None, 0, None, None, None, d((8,)), None, None, 0, None) == N.ERR_INVALID
+
+
+# ---------------------------------------------------------------------------
+# the module and its installation
+# ---------------------------------------------------------------------------
+def test_swiglu_module_parameters():
+    from maba_v2_architecture_b200.config import get_101m_config
+    from maba_v2_architecture_b200.engine import ModelShape, parameter_shapes
+
+    m = mb.SwiGLUFFN(get_101m_config())
+    want = {k[len("layers.0.ffn."):]: v for k, v in parameter_shapes(ModelShape.from_config(get_101m_config())).items()
+            if k.startswith("layers.0.ffn.")}
+    assert {k: tuple(v.shape) for k, v in m.state_dict().items()} == want
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        m(torch.zeros(2, 640))
+
+
+def test_install_patches_the_ffn_only_when_asked(monkeypatch):
+    import sys
+    import types
+
+    names = ["maba_sparse", "maba_sparse.kernels", "maba_sparse.kernels.dispatcher", "maba_sparse.model"]
+    mods = {n: types.ModuleType(n) for n in names}
+    disp = mods["maba_sparse.kernels.dispatcher"]
+    disp._KERNEL_REGISTRY = {}
+    disp.register_kernel = lambda b, op: (lambda f: disp._KERNEL_REGISTRY.setdefault(b, {}).__setitem__(op, f))
+    disp.clear_dispatcher_cache = lambda: None
+
+    class SwiGLUFFN(torch.nn.Module):
+        def forward(self, x):
+            return x
+
+    mods["maba_sparse.model"].SwiGLUFFN = SwiGLUFFN
+    for n, m in mods.items():
+        monkeypatch.setitem(sys.modules, n, m)
+    monkeypatch.delenv("MABA_BACKEND", raising=False)
+    monkeypatch.delenv("MABA_STRICT_BACKEND", raising=False)
+    from maba_v2_architecture_b200.integration import install, uninstall
+
+    before = SwiGLUFFN.forward
+    h = install(mods["maba_sparse"], patch_layers=False)
+    assert SwiGLUFFN.forward is before
+    uninstall(h)
+    h = install(mods["maba_sparse"], patch_layers=False, patch_ffn=True)
+    assert SwiGLUFFN.forward is mb.SwiGLUFFN.forward
+    uninstall(h)
+    assert SwiGLUFFN.forward is before

@@ -357,3 +357,29 @@ def test_block_of_ffn_and_gated_residual(dt, m):
     err = gate.double() * (ey + ea @ wd.double().abs().t()) + 3 * O.E23 * (y.abs() + stream.double().abs())
     mb.b200_linear(mb.b200_gated_ffn(h, wg, wu), wd, scale=gate, residual=stream, out=stream)
     O.assert_within(stream, (y, O.stored(y, err, F32)), "block")
+
+
+def test_swiglu_module_trains():
+    """The module under autograd: its gradients are those of the operators' backward calls, chained;
+    and one optimizer step runs."""
+    torch.manual_seed(3)
+    ffn = mb.SwiGLUFFN(dim=96, intermediate_size=200).to(DEV, BF)
+    gate = torch.full((96,), 2.0, device=DEV, requires_grad=True)
+    x = randn(gen(1), 2, 35, 96, dt=BF).requires_grad_(True)
+    r = randn(gen(2), 2, 35, 96).requires_grad_(True)
+    y = ffn(x, residual=r, gate=torch.sigmoid(gate))
+    assert y.dtype == F32 and y.shape == r.shape
+    d = randn(gen(3), 2, 35, 96)
+    y.backward(d)
+    wg, wu, wd = (w.weight.detach() for w in (ffn.w_gate, ffn.w_up, ffn.w_down))
+    a = mb.b200_gated_ffn(x.detach(), wg, wu)
+    s = torch.sigmoid(gate.detach())
+    da, dwd, _, ds = mb.b200_linear_backward(d, a, wd, scale=s)
+    dx, dwg, dwu = mb.b200_gated_ffn_backward(da, x.detach(), wg, wu)
+    for got, want in ((ffn.w_down.weight.grad, dwd), (ffn.w_gate.weight.grad, dwg), (ffn.w_up.weight.grad, dwu),
+                      (x.grad, dx), (r.grad, d)):
+        assert torch.equal(got, want)
+    assert torch.allclose(gate.grad, ds * s * (1 - s), rtol=1e-6, atol=0)
+    before = wg.clone()
+    torch.optim.SGD(ffn.parameters(), lr=0.1).step()
+    assert not torch.equal(ffn.w_gate.weight.detach(), before)
