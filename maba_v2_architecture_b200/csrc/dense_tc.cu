@@ -48,30 +48,32 @@ using namespace tc;
 
 // Epilogue warps: 16 where a chunk's registers allow four warps per scheduler (their chains of
 // shared-memory, copy and SFU latencies hide each other), 8 where a warp holds a unit's sums.
-// Then one warpgroup: TMA, MMA and two idle warps that complete it; it lends registers to the
-// epilogue's.  What the split hands out is what the block is launched with.
+// Then one warpgroup: TMA of the operands, MMA, TMA of the epilogue's matrix, one idle warp; it
+// lends registers to the epilogue's.  What the split hands out is what the block is launched with.
 template <int MODE> struct Warps {
-    static constexpr int EPI = MODE == 0 ? 16 : 8, TMA = EPI, MMA = EPI + 1, THREADS = (EPI + 4) * 32;
+    static constexpr int EPI = MODE == 0 ? 16 : 8, TMA = EPI, MMA = EPI + 1, SIDE = EPI + 2, THREADS = (EPI + 4) * 32;
     static constexpr int REG_LAUNCH = MODE == 0 ? 96 : 168, REG_EPI = MODE == 0 ? 104 : 224, REG_OTHER = MODE == 0 ? 64 : 56;
+    static constexpr int GROUPS = EPI / 4;     // of four warps that share a chunk's columns
+    static constexpr int CHUNKS = 8 / GROUPS;  // a warp's chunks, GROUPS apart, at most
+    static constexpr uint32_t VEC_BYTES = 2 * CHUNKS * 32 * 4;  // a warp's scale and bias
     static_assert(EPI * 32 * REG_EPI + 128 * REG_OTHER <= THREADS * REG_LAUNCH, "register split exceeds the launch");
 };
-constexpr int MAX_EPI = 16;
 constexpr int BK = 64;
 constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
-constexpr uint32_t VEC_BYTES = 2 * 4 * 32 * 4;  // a warp's scale and bias of up to four chunks
 constexpr uint32_t BAR_BYTES = 512;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
 constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
 
 enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2,
-       B_SIDE = B_DRAIN + 1, N_BARS = B_SIDE + 2 * MAX_EPI };
+       B_SFULL = B_DRAIN + 1, B_SEMPTY = B_SFULL + 8, N_BARS = B_SEMPTY + 8 };  // [group][slot]
 static_assert(N_BARS * 8 + 8 <= BAR_BYTES, "barrier area");
 
 struct TcArgs {
     int64_t M, N;
     int kblocks, kseg, kb_split;  // contraction blocks over all segments, of one segment, of one split
     int tiles_n, splits, pairs, units, dual;
+    int d_inner, d_col, d_row;  // from a worker's unit to its next
     int bn, b_rows;  // columns of the MMA, rows of B per CTA
     int flush;       // contraction blocks between two readings of the accumulator
     int stages;
@@ -349,12 +351,14 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
 
     constexpr int PLANES = MODE == 2 ? 3 : 1;
     constexpr int EPI_WARPS = Warps<MODE>::EPI, W_TMA = Warps<MODE>::TMA, W_MMA = Warps<MODE>::MMA;
+    constexpr int W_SIDE = Warps<MODE>::SIDE, GROUPS = Warps<MODE>::GROUPS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
 
     if (tid == 0) {
-        for (int i = 0; i < N_BARS; ++i) mbar_init(&bars[i], i == B_TEMPTY || i == B_TEMPTY + 1 ? EPI_WARPS * CG : 1);
+        for (int i = 0; i < N_BARS; ++i)
+            mbar_init(&bars[i], i == B_TEMPTY || i == B_TEMPTY + 1 ? EPI_WARPS * CG : (i >= B_SEMPTY ? 4 : 1));
         *abort_f = 0;
         fence_barrier_init();
     }
@@ -372,23 +376,36 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // a unit: splits innermost, then the pair index, then columns, then rows of tiles
+    // A unit: splits innermost, then the pair index, then columns, then rows of tiles.  A worker
+    // walks its units by adding (a division for each took the epilogue longer than a chunk).
+    constexpr bool INNER = KIND == E_STORE;  // the others have neither splits nor pairs
     struct Unit {
-        int split, pair, kb0, kb1;
-        int64_t m0, n0;
+        int u, inner, col, row;  // index and its digits
+        __device__ int pair(const TcArgs& a) const { return INNER && inner >= a.splits ? 1 : 0; }
+        __device__ int split(const TcArgs& a) const { return INNER ? inner - pair(a) * a.splits : 0; }
+        __device__ int kb0(const TcArgs& a) const { return INNER ? split(a) * a.kb_split : 0; }
+        __device__ int kb1(const TcArgs& a) const {
+            const int k = INNER ? kb0(a) + a.kb_split : a.kblocks;
+            return k < a.kblocks ? k : a.kblocks;
+        }
+        __device__ int n0(const TcArgs& a) const { return col * (KIND == E_GLU || KIND == E_GLU_BWD ? a.bn / 2 : a.bn); }
     };
-    auto unit_of = [&](int unit) {
+    auto row_of = [&](const Unit& t) { return t.row * (128 * CG) + (int)rank * 128; };
+    auto first_unit = [&]() {
         Unit t;
-        unsigned u = (unsigned)unit;
-        t.split = t.pair = 0;
-        if (a.splits > 1) t.split = (int)(u % (unsigned)a.splits), u /= (unsigned)a.splits;
-        if (a.pairs > 1) t.pair = (int)(u & 1u), u >>= 1;
-        const unsigned row = u / (unsigned)a.tiles_n;
-        t.n0 = (int64_t)(u - row * (unsigned)a.tiles_n) * (a.dual ? a.bn / 2 : a.bn);
-        t.m0 = (int64_t)row * (128 * CG) + rank * 128;
-        t.kb0 = t.split * a.kb_split;
-        t.kb1 = t.kb0 + a.kb_split < a.kblocks ? t.kb0 + a.kb_split : a.kblocks;
+        t.u = worker;
+        const int inner = INNER ? a.splits * a.pairs : 1, tile = worker / inner;
+        t.inner = worker - tile * inner;
+        t.row = tile / a.tiles_n, t.col = tile - t.row * a.tiles_n;
         return t;
+    };
+    auto next_unit = [&](Unit& t) {
+        t.u += workers, t.col += a.d_col, t.row += a.d_row;
+        if (INNER) {
+            t.inner += a.d_inner;
+            if (t.inner >= a.splits * a.pairs) t.inner -= a.splits * a.pairs, ++t.col;
+        }
+        if (t.col >= a.tiles_n) t.col -= a.tiles_n, ++t.row;
     };
 
     if (warp >= EPI_WARPS) {
@@ -401,13 +418,13 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         int st = 0, it = 0;
         uint32_t phase = 1;  // (a fresh barrier's previous phase counts as complete)
         bool ok = true;
-        for (int u = worker; u < a.units && ok; u += workers) {
-            const Unit t = unit_of(u);
-            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+        for (Unit t = first_unit(); t.u < a.units && ok; next_unit(t)) {
+            const int m0 = row_of(t), n0 = t.n0(a), kb1 = t.kb1(a), pair = t.pair(a);
+            for (int kb = t.kb0(a); kb < kb1; ++kb, ++it) {
                 ok = mbar_wait(&bars[B_EMPTY + st], phase, abort_f);
                 if (!ok) break;
                 const int seg = kb >= a.kseg ? 1 : 0, k0 = (kb - seg * a.kseg) * BK;
-                const CUtensorMap* ma = (a.pairs == 2 ? t.pair : seg) ? &ta1 : &ta0;
+                const CUtensorMap* ma = (a.pairs == 2 ? pair : seg) ? &ta1 : &ta0;
                 unsigned char* sa = base + st * a.stage_bytes;
                 {
                     uint64_t* full = &bars[B_FULL + st];
@@ -421,21 +438,21 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                     for (int pl = 0; pl < PLANES; ++pl, sa += A_BYTES) {
                         unsigned char* sb = base + st * a.stage_bytes + a.b_at + pl * a.b_bytes;
                         if (A_MN) {
-                            load(sa, ma, (int)t.m0, k0, pl);
-                            load(sa + A_BYTES / 2, ma, (int)t.m0 + 64, k0, pl);
+                            load(sa, ma, m0, k0, pl);
+                            load(sa + A_BYTES / 2, ma, m0 + 64, k0, pl);
                         } else {
-                            load(sa, ma, k0, (int)t.m0, pl);
+                            load(sa, ma, k0, m0, pl);
                         }
                         if (KIND == E_GLU || KIND == E_GLU_BWD) {
                             if (CG == 2) {
-                                load(sb, rank ? &tb1 : &tb0, k0, (int)t.n0, pl);
+                                load(sb, rank ? &tb1 : &tb0, k0, n0, pl);
                             } else {
-                                load(sb, &tb0, k0, (int)t.n0, pl);
-                                load(sb + a.bn / 2 * 128, &tb1, k0, (int)t.n0, pl);
+                                load(sb, &tb0, k0, n0, pl);
+                                load(sb + a.bn / 2 * 128, &tb1, k0, n0, pl);
                             }
                         } else {
                             const CUtensorMap* mb = seg ? &tb1 : &tb0;
-                            const int y = (int)t.n0 + (int)rank * a.b_rows;
+                            const int y = n0 + (int)rank * a.b_rows;
                             if (B_MN) {
                                 for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0, pl);
                             } else {
@@ -469,10 +486,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             int st = 0, buf = 0;
             uint32_t phase = 0, tphase = 1;
             bool ok = true;
-            for (int u = worker; u < a.units && ok; u += workers) {
-                const Unit t = unit_of(u);
-                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush) {
-                    const int f1 = f0 + a.flush < t.kb1 ? f0 + a.flush : t.kb1;
+            for (Unit t = first_unit(); t.u < a.units && ok; next_unit(t)) {
+                const int kb1 = t.kb1(a);
+                for (int f0 = t.kb0(a); f0 < kb1; f0 += a.flush) {
+                    const int f1 = f0 + a.flush < kb1 ? f0 + a.flush : kb1;
                     const uint32_t d = tmem + buf * ACC_COLS;
                     ok = mbar_wait(&bars[B_TEMPTY + buf], tphase, abort_f);
                     if (!ok) break;
@@ -510,6 +527,36 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             commit(&bars[B_DRAIN]);
             mbar_wait(&bars[B_DRAIN], 0, nullptr);
         }
+    } else if (warp == W_SIDE && KIND != E_STORE && KIND != E_GLU) {
+        // ================= residual or gradient, chunk by chunk ================
+        // One copy brings 32 columns of the CTA's 128 rows, a chunk of each of a group's warps.
+        if (a.side_tma && elect_one()) {
+            const int width = KIND == E_GLU_BWD ? a.bn / 2 : a.bn;
+            uint32_t count[GROUPS] = {};
+            bool ok = true;
+            for (Unit t = first_unit(); t.u < a.units && ok; next_unit(t)) {
+                for (int c0 = 0; c0 * 32 < width && ok; c0 += GROUPS) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) {
+                        const int col = t.n0(a) + (c0 + g) * 32;
+                        if (!ok || (c0 + g) * 32 >= width || col >= a.N) continue;
+                        const uint32_t n = count[g]++, slot = a.n_in == 2 ? n & 1 : 0, use = a.n_in == 2 ? n >> 1 : n;
+                        ok = mbar_wait(&bars[B_SEMPTY + 2 * g + slot], (use & 1) ^ 1, abort_f);
+                        if (!ok) continue;
+                        uint64_t* full = &bars[B_SFULL + 2 * g + slot];
+                        mbar_arrive_expect_tx(full, 4 * a.in_bytes);
+                        tma_load_3d(staging + (g * a.n_in + slot) * 4 * a.in_bytes, &tside, full, col, row_of(t), 0);
+                    }
+                }
+            }
+            // every copy has landed before the CTA may exit
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+                for (uint32_t back = 1; back <= (uint32_t)a.n_in && back <= count[g]; ++back) {
+                    const uint32_t n = count[g] - back, slot = a.n_in == 2 ? n & 1 : 0, use = a.n_in == 2 ? n >> 1 : n;
+                    mbar_wait(&bars[B_SFULL + 2 * g + slot], use & 1, nullptr, 200000000ll);
+                }
+        }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Warps<MODE>::REG_EPI));
@@ -519,12 +566,11 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         constexpr bool SIDE = KIND != E_STORE && KIND != E_GLU;
         // MODE 1, 2: chunks (of a pair of projections: one) whose sums a warp holds
         constexpr int CH = MODE == 0 || DUAL ? 1 : (MODE == 1 ? 4 : 2);
-        constexpr int CS = EPI_WARPS / 4;  // a warp's chunks are CS apart
-        constexpr int NV = 8 / CS;         // and at most so many
+        constexpr int CS = GROUPS, NV = Warps<MODE>::CHUNKS;
         const int q = warp & 3, h = warp >> 2;
-        unsigned char* in_buf = staging + warp * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
-        unsigned char* out_buf = in_buf + a.n_in * a.in_bytes;
-        float* vscale = reinterpret_cast<float*>(base + a.vec_at + warp * VEC_BYTES);  // [NV chunks][32]
+        unsigned char* in_buf = staging + (h * a.n_in * 4 + q) * a.in_bytes;  // slots 4 in_bytes apart
+        unsigned char* out_buf = staging + EPI_WARPS * a.n_in * a.in_bytes + warp * a.n_out * a.out_bytes;
+        float* vscale = reinterpret_cast<float*>(base + a.vec_at + warp * Warps<MODE>::VEC_BYTES);  // [NV chunks][32]
         float* vbias = vscale + NV * 32;
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
@@ -539,45 +585,19 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         };
         auto place = [&](const Unit& t, int c) {
             Chunk k;
-            k.row0 = (int)t.m0 + q * 32, k.col0 = (int)t.n0 + c * 32;
+            k.row0 = row_of(t) + q * 32, k.col0 = t.n0(a) + c * 32;
             k.rows = a.M - k.row0 < 32 ? (int)(a.M - k.row0) : 32;
             k.cols = a.N - k.col0 < 32 ? (int)(a.N - k.col0) : 32;
             return k;
         };
-        // ---- residual or gradient: this warp's chunks in order, n_in of them ahead
-        int next_u = worker, next_c = h;  // the next chunk to bring
-        Unit next_t = unit_of(worker);
-        uint32_t brought = 0, used = 0;
-        auto bring = [&]() {
-            if (!has_side || !a.side_tma) return;
-            while (brought - used < (uint32_t)a.n_in && next_u < a.units) {
-                if (next_c * 32 >= width) {
-                    next_u += workers, next_c = h;
-                    if (next_u < a.units) next_t = unit_of(next_u);
-                    continue;
-                }
-                const Chunk k = place(next_t, next_c);
-                next_c += CS;
-                if (k.rows <= 0 || k.cols <= 0) continue;
-                const int slot = a.n_in == 2 ? (int)(brought & 1) : 0;
-                if (lane == 0) {
-                    uint64_t* bar = &bars[B_SIDE + 2 * warp + slot];
-                    mbar_arrive_expect_tx(bar, a.in_bytes);
-                    tma_load_3d(in_buf + slot * a.in_bytes, &tside, bar, k.col0, k.row0, 0);
-                }
-                ++brought;
-            }
-            __syncwarp();
-        };
-        auto side_wait = [&](uint32_t n, volatile int* abort) {
-            const int slot = a.n_in == 2 ? (int)(n & 1) : 0;
-            return mbar_wait_warp(&bars[B_SIDE + 2 * warp + slot], (a.n_in == 2 ? n >> 1 : n) & 1, abort);
-        };
+        // ---- residual or gradient
+        uint32_t used = 0;
         bool ok = true;
         auto side_ready = [&](const Chunk& k) {
             if (a.side_tma) {
-                ok = side_wait(used, abort_f);
-                return in_buf + (a.n_in == 2 ? (used & 1) * a.in_bytes : 0u);
+                const uint32_t slot = a.n_in == 2 ? used & 1 : 0, use = a.n_in == 2 ? used >> 1 : used;
+                ok = mbar_wait_warp(&bars[B_SFULL + 2 * h + slot], use & 1, abort_f);
+                return in_buf + slot * 4 * a.in_bytes;
             }
             __syncwarp();
             if (side_f32)
@@ -591,8 +611,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         };
         auto side_used = [&]() {
             __syncwarp();
+            if (a.side_tma && lane == 0) mbar_arrive(&bars[B_SEMPTY + 2 * h + (a.n_in == 2 ? used & 1 : 0)]);
             ++used;
-            bring();
         };
         // ---- results
         uint32_t stored = 0;
@@ -624,7 +644,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         auto fetch_vectors = [&](const Unit& t) {
 #pragma unroll
             for (int cc = 0; cc < (VECS ? NV : 0); ++cc) {
-                const int64_t col = t.n0 + (h + CS * cc) * 32 + lane;
+                const int col = t.n0(a) + (h + CS * cc) * 32 + lane;
                 const bool in = (h + CS * cc) * 32 < width && col < a.N;
                 ps[cc] = in && e.scale.p ? side_at<T>(e.scale, 0, col) : 1.f;
                 pb[cc] = in && e.bias.p ? side_at<T>(e.bias, 0, col) : 0.f;
@@ -655,7 +675,11 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         // ---- one chunk
         auto chunk = [&](const Unit& t, int c, float* z, float* w) {
             const Chunk k = place(t, c);
-            if (k.rows <= 0 || k.cols <= 0) return;
+            if (k.cols <= 0) return;
+            if (k.rows <= 0) {  // (the group's copy still counts this warp)
+                if (has_side && a.side_tma) side_ready(k), side_used();
+                return;
+            }
             unsigned char* in = nullptr;
             const float *vs = vscale + c / CS * 32, *vb = vbias + c / CS * 32;
             if (KIND == E_LINEAR) {
@@ -733,24 +757,27 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 }
                 return;
             }
-            if (KIND == E_STORE && a.splits > 1)
-                store(k, z, &tout, a.partial + (int64_t)(t.split * a.pairs + t.pair) * a.M * a.ldp, a.ldp,
-                      t.split * a.pairs + t.pair);
-            else
-                store(k, z, t.pair ? &tout2 : &tout, t.pair ? e.out2 : e.out, e.ldo, 0);
+            if (KIND == E_STORE && a.splits > 1) {
+                const int part = t.split(a) * a.pairs + t.pair(a);
+                store(k, z, &tout, a.partial + (int64_t)part * a.M * a.ldp, a.ldp, part);
+            } else {
+                const bool second = t.pair(a) != 0;
+                store(k, z, second ? &tout2 : &tout, second ? e.out2 : e.out, e.ldo, 0);
+            }
             if (KIND == E_GLU_BWD) store(k, w, &tout2, e.out2, e.ldo, 0);
         };
 
-        if (worker < a.units) fetch_vectors(next_t);
-        bring();
-        for (int u = worker; u < a.units; u += workers) {
-            const Unit t = unit_of(u);
+        Unit t = first_unit();
+        if (t.u < a.units) fetch_vectors(t);
+        while (t.u < a.units) {
+            Unit after = t;
+            next_unit(after);
             if (VECS) {
                 __syncwarp();
 #pragma unroll
                 for (int cc = 0; cc < NV; ++cc) vscale[cc * 32 + lane] = ps[cc], vbias[cc * 32 + lane] = pb[cc];
                 __syncwarp();
-                if (u + workers < a.units) fetch_vectors(unit_of(u + workers));
+                if (after.u < a.units) fetch_vectors(after);
             }
             if constexpr (MODE != 0) {
                 float sz[CH][32], sw[DUAL ? 32 : 1];  // the unit's accumulations, added up
@@ -760,7 +787,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                     for (int cc = 0; cc < CH; ++cc) sz[cc][j] = 0.f;
                     if (DUAL) sw[j] = 0.f;
                 }
-                for (int f0 = t.kb0; f0 < t.kb1; f0 += a.flush) {
+                const int kb1 = t.kb1(a);
+                for (int f0 = t.kb0(a); f0 < kb1; f0 += a.flush) {
                     if (!wait_full()) break;
                     const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
                     auto add = [&](float* sum, int col) {
@@ -806,10 +834,9 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 }
             }
             if (!ok) break;
+            t = after;
         }
-        // copies in flight end before the CTA may
-        for (; used < brought; ++used) side_wait(used, nullptr);
-        if (lane == 0) bulk_wait_all();
+        if (lane == 0) bulk_wait_all();  // the copies out end before the CTA may
     }
     __syncwarp();
     tc_fence_before();
@@ -889,12 +916,13 @@ bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int planes, int64_t ro
 }
 
 // The map of a matrix that the epilogue reads or writes in chunks, rows x cols (x planes).
-bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t planes) {
+bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t planes,
+               uint32_t box_rows = 32) {
     const int el = dt == MABA_F32 ? 4 : 2;
     if (rows == 1) ld = (cols + 7) / 8 * 8;
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (ld * el) % 16 != 0 || ld < cols) return false;
     const int64_t dims[3] = {cols, rows, planes}, strides[2] = {ld, planes > 1 ? rows * ld : ld};
-    const uint32_t box[3] = {32, 32, 1};
+    const uint32_t box[3] = {32, box_rows, 1};
     return make_map(m, dt, p, 3, dims, strides, box);
 }
 
@@ -967,6 +995,10 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     const int64_t units = ceil_div(p.M, 128 * pl.cg) * a.tiles_n * a.pairs * a.splits;
     if (units > 0x7fffffff) return set_error(MABA_ERR_UNSUPPORTED, "dense: %lld tiles", (long long)units);
     a.units = (int)units;
+    const int slots = sm_count() / pl.cg, workers = a.units < slots ? a.units : slots;
+    a.d_inner = workers % (a.splits * a.pairs);
+    a.d_col = workers / (a.splits * a.pairs) % a.tiles_n;
+    a.d_row = workers / (a.splits * a.pairs) / a.tiles_n;
     const uint32_t bb = b_bytes_of(pl.cg, pl.bn, b_mn);
     a.flush = mode == 0 ? a.kblocks : (mode == 1 ? 512 / BK : 256 / BK);
     a.b_at = planes * A_BYTES;
@@ -975,12 +1007,13 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
     // staging: two buffers each way where that leaves enough stages for the products, else fewer
     const int epi = mode == 0 ? Warps<0>::EPI : Warps<1>::EPI, threads = mode == 0 ? Warps<0>::THREADS : Warps<1>::THREADS;
+    const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
+    const uint32_t vec_bytes = !vecs ? 0 : epi * (mode == 0 ? Warps<0>::VEC_BYTES : Warps<1>::VEC_BYTES);
     const bool to_planes = planes == 3 && (p.e.kind == E_LINEAR_BWD || p.e.kind == E_GLU_BWD);
     const bool out_f32 = !to_planes && (planes == 3 || p.e.out_f32 || a.splits > 1), side_f32 = planes == 3 || p.e.res.f32;
-    const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
     a.in_bytes = p.e.res.p ? (side_f32 ? 4096 : 2048) : 0;
     a.out_bytes = out_f32 ? 4096 : 2048;
-    const uint32_t fixed = 1024 + BAR_BYTES + (vecs ? epi * VEC_BYTES : 0);
+    const uint32_t fixed = 1024 + BAR_BYTES + vec_bytes;
     uint32_t staging = 0;
     for (int t = 0; t < 3; ++t) {
         a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
@@ -990,7 +1023,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     a.vec_at = a.stages * a.stage_bytes + staging;
-    a.bar_at = a.vec_at + (vecs ? epi * VEC_BYTES : 0);
+    a.bar_at = a.vec_at + vec_bytes;
     const size_t smem = 1024 + a.bar_at + BAR_BYTES;
     a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
@@ -1012,7 +1045,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     if (nb == 1) m[3] = m[2];
     m[4] = m[5] = m[6] = m[0];
     a.side_tma = p.e.res.p && p.e.res.sc == 1 &&
-                 chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1);
+                 chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1, 128);
     if (a.splits > 1) {
         a.out_tma = chunk_map(&m[5], MABA_F32, partial, p.M, p.N, ldp, a.splits * a.pairs);
     } else if (to_planes) {
@@ -1023,9 +1056,8 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
         a.out_tma = chunk_map(&m[5], out_f32 ? MABA_F32 : odt, p.e.out, p.M, p.N, p.e.ldo, 1) &&
                     (!p.e.out2 || chunk_map(&m[6], out_f32 ? MABA_F32 : odt, p.e.out2, p.M, p.N, p.e.ldo, 1));
     }
-    const int slots = sm_count() / pl.cg;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((a.units < slots ? a.units : slots) * pl.cg));
+    cfg.gridDim = dim3((unsigned)(workers * pl.cg));
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
