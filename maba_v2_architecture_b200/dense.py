@@ -26,6 +26,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
+from ._native import pack_matrix, pack_vector
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DENSE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -52,16 +53,18 @@ def _check_weight(w: torch.Tensor, name: str, x: torch.Tensor, n: int, k: int) -
 
 def _check_x(x: torch.Tensor, w: torch.Tensor, name: str) -> Tuple[int, int]:
     """Output and input features."""
+    dt, shape = w.dtype, w.shape
+    if x.dtype is dt and dt in DENSE_DTYPES and len(shape) == 2 and x.device == w.device:
+        n, k = shape
+        if n and k and x.dim() and x.shape[-1] == k:
+            return n, k
     if x.dtype not in DENSE_DTYPES:
         raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {DENSE_DTYPES}")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
     k = x.shape[-1]
-    n = w.shape[0] if w.dim() else 0
-    _check_weight(w, name, x, n, k)
-    if n == 0 or k == 0:
-        raise ValueError(f"no features: x {list(x.shape)}, {name} {list(w.shape)}")
-    return n, k
+    _check_weight(w, name, x, shape[0] if w.dim() else 0, k)
+    raise ValueError(f"no features: x {list(x.shape)}, {name} {list(shape)}")
 
 
 def _check_side(t: torch.Tensor, name: str, x: torch.Tensor, shape: Sequence[int], f32: bool = True) -> None:
@@ -127,11 +130,11 @@ def _call(fn, size, x: torch.Tensor, head, size_args) -> None:
 def _mat(t: Optional[torch.Tensor]) -> Optional[bytes]:
     if t is None:
         return None
-    return N.pack_matrix(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+    return pack_matrix(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
 def _vec(t: Optional[torch.Tensor]) -> Optional[bytes]:
-    return None if t is None else N.pack_vector(t)
+    return None if t is None else pack_vector(t)
 
 
 # ---------------------------------------------------------------------------
@@ -141,18 +144,21 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
     # (one token's call is bound by this function: no helper calls, descriptors packed in place)
     if out is None:
         out = x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype or x.dtype)
-    if x.numel() == 0:
-        return out
-    pack = N.pack_matrix
-    plain = x.dim() == 2
-    dx, dw, do = pack(x) if plain else _mat(x), pack(weight), pack(out) if plain else _mat(out)
-    db = None if bias is None else N.pack_vector(bias)
-    ds = None if scale is None else N.pack_vector(scale)
-    dr = None if residual is None else (pack(residual) if plain else _mat(residual))
+    if x.dim() == 2:
+        dx, do = pack_matrix(x), pack_matrix(out)
+        dr = None if residual is None else pack_matrix(residual)
+    else:
+        if x.numel() == 0:
+            return out
+        dx, do, dr = _mat(x), _mat(out), _mat(residual)
+    dw = pack_matrix(weight)
+    db = None if bias is None else pack_vector(bias)
+    ds = None if scale is None else pack_vector(scale)
     lib = N.lib()
     index = x.get_device()
     rc = N.ERR_WORKSPACE
-    if index == _current_device():  # most calls need no scratch memory: tried without (refused before any launch)
+    # most calls need no scratch memory: tried without (refused before any launch)
+    if index == _current_device() and (x.dtype is not torch.float32 or x.numel() <= 8 * x.shape[-1]):
         rc = lib.maba_linear(dx, dw, db, act, ds, dr, do, None, 0, _raw_stream(index))
     if rc:
         if rc != N.ERR_WORKSPACE:
@@ -224,7 +230,7 @@ def b200_linear(
     if not x.is_cuda:
         N.require_cuda(x, op="linear")
     tracked = torch.is_grad_enabled() and (
-        x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+        weight.requires_grad or x.requires_grad or (bias is not None and bias.requires_grad)
         or (scale is not None and scale.requires_grad) or (residual is not None and residual.requires_grad))
     if out is not None:
         if tracked or out.requires_grad:
@@ -272,15 +278,17 @@ def b200_linear_backward(
 def _gated_ffn(x, w_gate, w_up, act, out):
     if out is None:
         out = x.new_empty((*x.shape[:-1], w_gate.shape[0]))
-    if x.numel() == 0:
-        return out
-    pack = N.pack_matrix
-    plain = x.dim() == 2
-    dx, dg, du, do = pack(x) if plain else _mat(x), pack(w_gate), pack(w_up), pack(out) if plain else _mat(out)
+    if x.dim() == 2:
+        dx, do = pack_matrix(x), pack_matrix(out)
+    else:
+        if x.numel() == 0:
+            return out
+        dx, do = _mat(x), _mat(out)
+    dg, du = pack_matrix(w_gate), pack_matrix(w_up)
     lib = N.lib()
     index = x.get_device()
     rc = N.ERR_WORKSPACE
-    if index == _current_device():  # (as in _linear)
+    if index == _current_device() and (x.dtype is not torch.float32 or x.numel() <= 8 * x.shape[-1]):  # (as in _linear)
         rc = lib.maba_gated_ffn(dx, dg, du, act, do, None, 0, _raw_stream(index))
     if rc:
         if rc != N.ERR_WORKSPACE:
