@@ -11,7 +11,7 @@
 // contraction indices: a sum over K loses about K 5.6e-10 of itself toward zero (measured
 // 6e-7 relative at K = 640, 4.4e-6 at 4,096).  That is far below a 16-bit result's rounding,
 // but not below a float32 result's, so sums that end in float32 (MODE 1 and 2) leave TMEM
-// every 512 (256) indices and are added, rounded to nearest, in the epilogue's registers.
+// every 640 (320) indices and are added, rounded to nearest, in the epilogue's registers.
 //
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
@@ -639,15 +639,26 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 __syncwarp();
             }
         };
-        // ---- scale and bias of a unit's columns, one unit ahead in registers
-        float ps[NV], pb[NV];
+        // ---- scale and bias of a unit's columns, one unit ahead in registers, as they are in
+        // memory (a conversion here would wait for each load in turn)
+        uint32_t ps[NV], pb[NV];
+        auto bits_at = [&](const Side& v, int col) {
+            const int64_t i = col * v.sc;
+            return sizeof(T) == 4 || v.f32 ? static_cast<const uint32_t*>(v.p)[i] : (uint32_t)static_cast<const uint16_t*>(v.p)[i];
+        };
+        auto value_of = [&](const Side& v, uint32_t bits) {
+            if constexpr (sizeof(T) == 2)
+                if (!v.f32) return unpack2<T>(bits).x;
+            return __uint_as_float(bits);
+        };
         auto fetch_vectors = [&](const Unit& t) {
 #pragma unroll
             for (int cc = 0; cc < (VECS ? NV : 0); ++cc) {
                 const int col = t.n0(a) + (h + CS * cc) * 32 + lane;
                 const bool in = (h + CS * cc) * 32 < width && col < a.N;
-                ps[cc] = in && e.scale.p ? side_at<T>(e.scale, 0, col) : 1.f;
-                pb[cc] = in && e.bias.p ? side_at<T>(e.bias, 0, col) : 0.f;
+                ps[cc] = pb[cc] = 0u;  // (columns past the last are not stored)
+                if (in && e.scale.p) ps[cc] = bits_at(e.scale, col);
+                if (in && e.bias.p) pb[cc] = bits_at(e.bias, col);
             }
         };
         // ---- accumulators
@@ -775,7 +786,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             if (VECS) {
                 __syncwarp();
 #pragma unroll
-                for (int cc = 0; cc < NV; ++cc) vscale[cc * 32 + lane] = ps[cc], vbias[cc * 32 + lane] = pb[cc];
+                for (int cc = 0; cc < NV; ++cc) {
+                    vscale[cc * 32 + lane] = value_of(e.scale, ps[cc]);
+                    vbias[cc * 32 + lane] = value_of(e.bias, pb[cc]);
+                }
                 __syncwarp();
                 if (after.u < a.units) fetch_vectors(after);
             }
@@ -864,7 +878,7 @@ inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
 }
 
 // How a product's sums are kept: 0 one accumulation (16-bit results), 1 added up in registers
-// every 512 indices (float32 results of 16-bit operands), 2 float32 operands, every 256.
+// every 640 indices (float32 results of 16-bit operands), 2 float32 operands, every 320.
 int mode_of(const Product& p, int dt) {
     if (dt == MABA_F32) return 2;
     return p.e.kind == E_LINEAR && p.e.out_f32 ? 1 : 0;
@@ -1000,7 +1014,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.d_col = workers / (a.splits * a.pairs) % a.tiles_n;
     a.d_row = workers / (a.splits * a.pairs) / a.tiles_n;
     const uint32_t bb = b_bytes_of(pl.cg, pl.bn, b_mn);
-    a.flush = mode == 0 ? a.kblocks : (mode == 1 ? 512 / BK : 256 / BK);
+    a.flush = mode == 0 ? a.kblocks : (mode == 1 ? 640 / BK : 320 / BK);
     a.b_at = planes * A_BYTES;
     a.b_bytes = (bb + 1023) / 1024 * 1024;
     a.stage_bytes = planes * (A_BYTES + a.b_bytes);
