@@ -4,8 +4,11 @@
 //
 // A call first lays its workspace out with a Scratch; the *_workspace_size entries run the
 // same code without launching, so size and use cannot differ.  Nothing is accumulated with
-// atomics: results do not depend on the order in which CTAs run.
+// atomics: results do not depend on the order in which CTAs run.  Every kernel here is launched
+// with programmatic dependence (pdl.cuh) and waits for its predecessor before its first access
+// of global memory; a chain of them is ordered, since each waits.
 #include "dense.cuh"
+#include "pdl.cuh"
 
 namespace maba {
 namespace dense {
@@ -48,8 +51,9 @@ __device__ __forceinline__ void split_planes(float x, __nv_bfloat16 (&v)[3]) {
 }
 
 // Operands made readable, up to three in one launch: dst [rows][ld] of a 16-bit type = src (that
-// type or float32, any strides), or the three planes of a float32 src.  Tiles of 32 x 64 pass
-// through shared memory, so that both sides run along their contiguous axis.
+// type or float32, any strides), or the three planes of a float32 src.  Tiles of 32 x 64; where
+// the source's columns are not contiguous they pass through shared memory, so that both sides
+// run along their contiguous axis.
 struct Job {
     Side src;
     int64_t rows = 0, cols = 0;
@@ -60,47 +64,53 @@ struct Jobs {
     Job j[3];
     int n = 0;
 };
+template <typename T> __device__ __forceinline__ void put_pair(const Job& b, int64_t at, float x, float y) {
+    if constexpr (sizeof(T) == 4) {
+        __nv_bfloat16 p[3], q[3];
+        split_planes(x, p), split_planes(y, q);
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(b.dst) + e * b.plane + at) =
+                __halves2bfloat162(p[e], q[e]);
+    } else {
+        const T v[2] = {Cvt<T>::from_f(x), Cvt<T>::from_f(y)};
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(b.dst) + at) = *reinterpret_cast<const uint32_t*>(v);
+    }
+}
 template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Jobs jobs) {
     __shared__ float tile[32][65];
+    griddep_launch_dependents();
+    griddep_wait();
     const Job& b = jobs.j[blockIdx.y];
     const unsigned tiles_c = (unsigned)((b.cols + 63) / 64);
     const int64_t tiles = (b.rows + 31) / 32 * tiles_c;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int64_t tr = tiles >> 32 ? t / tiles_c : (unsigned)t / tiles_c, r0 = tr * 32, c0 = (t - tr * tiles_c) * 64;
-        if (b.src.sc <= b.src.sr) {  // lanes along the columns
+        const int64_t c = c0 + lane * 2, rw = r0 + w * 4;
+        if (b.src.sc == 1) {
+            float x[4], y[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = w * 4 + (i >> 1), c = (i & 1) * 32 + lane;
-                if (r0 + r < b.rows && c0 + c < b.cols) tile[r][c] = side_at<T>(b.src, r0 + r, c0 + c);
+            for (int i = 0; i < 4; ++i) {
+                x[i] = rw + i < b.rows && c < b.cols ? side_at<T>(b.src, rw + i, c) : 0.f;
+                y[i] = rw + i < b.rows && c + 1 < b.cols ? side_at<T>(b.src, rw + i, c + 1) : 0.f;
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = lane, c = w * 8 + i;
-                if (r0 + r < b.rows && c0 + c < b.cols) tile[r][c] = side_at<T>(b.src, r0 + r, c0 + c);
-            }
+            for (int i = 0; i < 4; ++i)  // (ld is a multiple of 8: the pair fits)
+                if (rw + i < b.rows && c < b.cols) put_pair<T>(b, (rw + i) * b.ld + c, x[i], y[i]);
+            continue;
+        }
+        const bool along = b.src.sc <= b.src.sr;  // lanes along the columns
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = along ? w * 4 + (i >> 1) : lane, q = along ? (i & 1) * 32 + lane : w * 8 + i;
+            if (r0 + r < b.rows && c0 + q < b.cols) tile[r][q] = side_at<T>(b.src, r0 + r, c0 + q);
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = w * 4 + i, c = lane * 2;
-            if (r0 + r >= b.rows || c0 + c >= b.cols) continue;  // (ld is a multiple of 8: the pair fits)
-            const float x = tile[r][c], y = c0 + c + 1 < b.cols ? tile[r][c + 1] : 0.f;
-            const int64_t at = (r0 + r) * b.ld + c0 + c;
-            if constexpr (sizeof(T) == 4) {
-                __nv_bfloat16 p[3], q[3];
-                split_planes(x, p), split_planes(y, q);
-#pragma unroll
-                for (int e = 0; e < 3; ++e)
-                    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(b.dst) + e * b.plane + at) =
-                        __halves2bfloat162(p[e], q[e]);
-            } else {
-                T* d = static_cast<T*>(b.dst) + at;
-                const T v[2] = {Cvt<T>::from_f(x), Cvt<T>::from_f(y)};
-                *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(v);
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+            if (rw + i < b.rows && c < b.cols)
+                put_pair<T>(b, (rw + i) * b.ld + c, tile[w * 4 + i][lane * 2], c + 1 < b.cols ? tile[w * 4 + i][lane * 2 + 1] : 0.f);
         __syncthreads();
     }
 }
@@ -111,6 +121,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     sum_splits_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t rows, int64_t cols, T* out,
                       T* out2, int64_t half, int64_t ld) {
+    griddep_launch_dependents();
+    griddep_wait();
     const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 4;
     if (c >= cols) return;
     for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
@@ -133,6 +145,8 @@ __global__ void __launch_bounds__(256)
 constexpr int CS_ROWS = 128;
 template <typename T>
 __global__ void __launch_bounds__(256) colsum_kernel(Side g, int64_t rows, int64_t cols, float* part) {
+    griddep_launch_dependents();
+    griddep_wait();
     const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int w = threadIdx.x >> 5;
     __shared__ float red[8][32];
@@ -159,6 +173,8 @@ struct Columns {
 };
 template <typename T>
 __global__ void __launch_bounds__(1024) colsum_finish_kernel(const Columns v, int64_t blocks, int64_t cols) {
+    griddep_launch_dependents();
+    griddep_wait();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.y;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     __shared__ float red[32][33];
@@ -204,9 +220,9 @@ int run(Ctx& c, const Product& p) {
         MABA_TRY(tc_product<T>(p, plan, partial, ldp, c.s));
         if (plan.splits == 1) return (int)MABA_OK;
         const int64_t gy = ceil_div(rows, 8), cap = 32768;
-        sum_splits_kernel<T><<<dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), 256, 0, c.s>>>(
-            partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2), p.M, p.e.ldo);
-        return check_launch("dense(split sums)");
+        return launch_pdl(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), dim3(256),
+                          0, c.s, partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2),
+                          p.M, p.e.ldo);
     });
 }
 
@@ -225,8 +241,7 @@ int prepare(Ctx& c) {
     c.jobs.n = 0;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        prepare_kernel<T><<<grid, 256, 0, c.s>>>(jobs);
-        return check_launch("dense(operands)");
+        return launch_pdl(prepare_kernel<T>, grid, dim3(256), 0, c.s, jobs);
     });
 }
 
@@ -234,8 +249,7 @@ int column_sums(Ctx& c, const Side& g, int64_t rows, int64_t cols, float* part) 
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
         const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)ceil_div(rows, CS_ROWS));
-        colsum_kernel<T><<<grid, 256, 0, c.s>>>(g, rows, cols, part);
-        return check_launch("dense(column sums)");
+        return launch_pdl(colsum_kernel<T>, grid, dim3(256), 0, c.s, g, rows, cols, part);
     });
 }
 
@@ -251,8 +265,8 @@ int finish_columns(Ctx& c, const float* pb, const maba_tensor* db, const float* 
     }
     if (n == 0) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        colsum_finish_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), n), 1024, 0, c.s>>>(v, blocks, cols);
-        return check_launch("dense(column sums)");
+        return launch_pdl(colsum_finish_kernel<T>, dim3((unsigned)ceil_div(cols, 32), (unsigned)n), dim3(1024), 0, c.s, v, blocks,
+                          cols);
     });
 }
 

@@ -31,6 +31,7 @@
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
 // freed and the error word behind maba_device_error() is set.
 #include "dense.cuh"
+#include "pdl.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 
@@ -370,11 +371,13 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         if (CG == 2) tmem_alloc_pair<TMEM_COLS>(tmem_slot);
         else tmem_alloc<TMEM_COLS>(tmem_slot);
     }
+    griddep_launch_dependents();
     tc_fence_before();
     __syncthreads();
     if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    griddep_wait();  // all that precedes overlaps the previous kernel; every access of memory follows
 
     // A unit: splits innermost, then the pair index, then columns, then rows of tiles.  A worker
     // walks its units by adding (a division for each took the epilogue longer than a chunk).
@@ -1075,12 +1078,14 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)pl.cg;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)pl.cg;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pl.cg == 2 ? 1 : 0;
+    cfg.numAttrs = (unsigned)pl.cg;
     err = cudaLaunchKernelEx(&cfg, kern, a, m[0], m[1], m[2], m[3], m[4], m[5], m[6]);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
