@@ -141,6 +141,73 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// The epilogue on split sums, partial [splits][1 or 2][M][ldp]: a block has 32 columns of 32 rows
+template <typename T>
+__global__ void __launch_bounds__(256)
+    finish_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t M, int64_t N, const Epilogue e) {
+    griddep_launch_dependents();
+    griddep_wait();
+    __shared__ float red[2][8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+    const bool dual = e.kind == E_GLU || e.kind == E_GLU_BWD;
+    for (int64_t blk = blockIdx.y; blk * 32 < M; blk += gridDim.y) {
+        float sb = 0.f, ss = 0.f;
+        for (int64_t m = blk * 32 + w; m < M && m < blk * 32 + 32; m += 8) {
+            if (n >= N) break;
+            float z = 0.f, u = 0.f;
+            for (int q = 0; q < splits; ++q) {
+                const float* p = partial + ((int64_t)q * (dual ? 2 : 1) * M + m) * ldp + n;
+                z += p[0];
+                if (dual) u += p[M * ldp];
+            }
+            const int64_t at = m * e.ldo + n;
+            float r[2];
+            if (e.kind == E_LINEAR) {
+                if (e.bias.p) z += side_at<T>(e.bias, 0, n);
+                r[0] = act_f(z, e.act);
+                if (e.scale.p) r[0] *= side_at<T>(e.scale, 0, n);
+                if (e.res.p) r[0] += side_at<T>(e.res, m, n);
+            } else if (e.kind == E_GLU) {
+                r[0] = act_f(z, e.act) * u;
+            } else {
+                if (e.bias.p) z += side_at<T>(e.bias, 0, n);
+                const float g = side_at<T>(e.res, m, n);
+                float y, d;
+                act_grad_f(z, e.act, y, d);
+                r[0] = g * d * (dual ? u : (e.scale.p ? side_at<T>(e.scale, 0, n) : 1.f));
+                r[1] = g * y;
+                sb += r[0], ss += r[1];
+            }
+            const bool grad = e.kind == E_GLU_BWD || e.kind == E_LINEAR_BWD;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i == 1 && e.kind != E_GLU_BWD) break;
+                void* out = i ? e.out2 : e.out;
+                if (sizeof(T) == 4 && grad) {
+                    __nv_bfloat16 v[3];
+                    split_planes(r[i], v);
+                    for (int q = 0; q < 3; ++q) static_cast<__nv_bfloat16*>(out)[q * e.planes + at] = v[q];
+                } else if (e.out_f32) {
+                    static_cast<float*>(out)[at] = r[i];
+                } else {
+                    static_cast<T*>(out)[at] = Cvt<T>::from_f(r[i]);
+                }
+            }
+        }
+        if (e.kind != E_LINEAR_BWD || !(e.part_bias || e.part_scale)) continue;
+        red[0][w][lane] = sb, red[1][w][lane] = ss;
+        __syncthreads();
+        float* part = w == 0 ? e.part_bias : e.part_scale;
+        if (w < 2 && part && n < N) {
+            float t = 0.f;
+            for (int q = 0; q < 8; ++q) t += red[w][q][lane];
+            part[blk * N + n] = t;
+        }
+        __syncthreads();
+    }
+}
+
 // part[blk][n] = sum of g over rows [128 blk, 128 blk + 128), added in row order
 constexpr int CS_ROWS = 128;
 template <typename T>
@@ -200,6 +267,8 @@ struct Ctx {
     Scratch ws;
     cudaStream_t s;
     Jobs jobs;  // operand copies not launched yet
+    Plan plans[4];  // of the call's products, made by the workspace query and used in its order
+    int n_plans = 0, next_plan = 0;
 };
 
 // ---------------------------------------------------------------------------
@@ -212,14 +281,21 @@ int run(Ctx& c, const Product& p) {
     }
     // a plain product whose tiles do not fill the GPU splits its contraction; the partial
     // sums are float32 and added in split order
-    const Plan plan = tc_plan(p, c.dt);
-    const int64_t rows = p.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
+    const Plan plan = c.dry ? (c.plans[c.n_plans++] = tc_plan(p, c.dt)) : c.plans[c.next_plan++];
+    const Product sums = plan.finish ? split_sums(p) : p;
+    const int64_t rows = sums.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
     float* partial = plan.splits > 1 ? static_cast<float*>(c.ws.take((size_t)plan.splits * rows * ldp * 4)) : nullptr;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        MABA_TRY(tc_product<T>(p, plan, partial, ldp, c.s));
+        MABA_TRY(tc_product<T>(sums, plan, partial, ldp, c.s));
         if (plan.splits == 1) return (int)MABA_OK;
-        const int64_t gy = ceil_div(rows, 8), cap = 32768;
+        const int64_t cap = 32768;
+        if (plan.finish) {
+            const int64_t gy = ceil_div(p.M, 32);
+            return launch_pdl(finish_kernel<T>, dim3((unsigned)ceil_div(p.N, 32), (unsigned)(gy < cap ? gy : cap)), dim3(256), 0,
+                              c.s, partial, ldp, plan.splits, p.M, p.N, p.e);
+        }
+        const int64_t gy = ceil_div(rows, 8);
         return launch_pdl(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), dim3(256),
                           0, c.s, partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2),
                           p.M, p.e.ldo);
@@ -385,6 +461,7 @@ int dx_product(Ctx& c, int64_t M, int64_t N, int n, const Matrix* d, const Matri
     p.form = n == 2 ? F_SUM : F_SINGLE;
     p.M = M, p.N = dx->shape[1], p.K = N;
     for (int i = 0; i < n; ++i) p.a[i] = d[i], p.b[i] = transposed(w[i]);
+    p.b_mn = true;
     p.e.out = dx->data, p.e.ldo = dx->stride[0];
     return run(c, p);
 }
@@ -393,8 +470,8 @@ int dw_product(Ctx& c, int64_t M, int n, const Matrix* d, const Matrix& x, const
     p.form = n == 2 ? F_PAIR : F_SINGLE;
     p.M = dw[0]->shape[0], p.N = dw[0]->shape[1], p.K = M;
     for (int i = 0; i < n; ++i) p.a[i] = transposed(d[i]);
-    p.b[0] = transposed(x);
-    p.a_mn = true;
+    p.b[0] = p.b[1] = transposed(x);
+    p.a_mn = p.b_mn = true;
     p.e.out = dw[0]->data, p.e.ldo = dw[0]->stride[0];
     if (n == 2) p.e.out2 = dw[1]->data;
     return run(c, p);
@@ -529,17 +606,22 @@ int check_ffn(const FfnArgs& a, bool backward) {
     return MABA_OK;
 }
 
-template <typename Args, typename F> size_t query(const Args& a, F op) {
-    Ctx c{a.x->dtype, true, {}, nullptr, {}};
-    return op(c, a) == MABA_OK ? c.ws.used : 0;
+template <typename Args, typename F> Ctx query(const Args& a, F op) {
+    Ctx c{};
+    c.dt = a.x->dtype, c.dry = true;
+    if (op(c, a) != MABA_OK) c.ws.used = 0;
+    return c;
 }
 
 template <typename Args, typename F>
 int execute(const Args& a, F op, const char* name, void* workspace, size_t bytes, void* stream) {
-    const size_t need = query(a, op);
+    Ctx c = query(a, op);
+    const size_t need = c.ws.used;
     if (need > 0 && (workspace == nullptr || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
         return set_error(MABA_ERR_WORKSPACE, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu", name, need, bytes);
-    Ctx c{a.x->dtype, false, {static_cast<unsigned char*>(workspace), 0}, as_stream(stream), {}};
+    c.dry = false;
+    c.ws = Scratch{static_cast<unsigned char*>(workspace), 0};
+    c.s = as_stream(stream);
     return op(c, a);
 }
 
@@ -563,7 +645,7 @@ extern "C" size_t maba_linear_workspace_size(const maba_tensor* x, const maba_te
     LinearArgs a{};
     a.x = x, a.w = weight, a.out = out;
     if (check_linear(a, false) != MABA_OK) return 0;
-    return query(a, linear_forward);
+    return query(a, linear_forward).ws.used;
 }
 
 extern "C" int maba_linear_backward(const maba_tensor* grad, const maba_tensor* x, const maba_tensor* weight,
@@ -586,7 +668,7 @@ extern "C" size_t maba_linear_backward_workspace_size(const maba_tensor* grad, c
     a.g = grad, a.x = x, a.w = weight, a.bias = bias, a.scale = scale, a.act = activation;
     a.dx = dx, a.dw = dw, a.dbias = dbias, a.dscale = dscale;
     if (check_linear(a, true) != MABA_OK) return 0;
-    return query(a, linear_backward);
+    return query(a, linear_backward).ws.used;
 }
 
 extern "C" int maba_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up, int32_t activation,
@@ -602,7 +684,7 @@ extern "C" size_t maba_gated_ffn_workspace_size(const maba_tensor* x, const maba
     FfnArgs a{};
     a.x = x, a.wg = w_gate, a.wu = w_up, a.out = out, a.act = ACT_SILU;
     if (check_ffn(a, false) != MABA_OK) return 0;
-    return query(a, ffn_forward);
+    return query(a, ffn_forward).ws.used;
 }
 
 extern "C" int maba_gated_ffn_backward(const maba_tensor* grad, const maba_tensor* x, const maba_tensor* w_gate,
@@ -622,5 +704,5 @@ extern "C" size_t maba_gated_ffn_backward_workspace_size(const maba_tensor* grad
     FfnArgs a{};
     a.g = grad, a.x = x, a.wg = w_gate, a.wu = w_up, a.act = ACT_SILU, a.dx = dx, a.dwg = dw_gate, a.dwu = dw_up;
     if (check_ffn(a, true) != MABA_OK) return 0;
-    return query(a, ffn_backward);
+    return query(a, ffn_backward).ws.used;
 }

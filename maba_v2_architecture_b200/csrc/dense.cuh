@@ -21,7 +21,7 @@ enum Form {
     F_SINGLE = 0,  // C = A0 B0^T
     F_DUAL = 1,    // two products of one A: columns j of B0 and of B1 meet in the epilogue
     F_SUM = 2,     // C = A0 B0^T + A1 B1^T
-    F_PAIR = 3,    // C0 = A0 B0^T and C1 = A1 B0^T (epilogue E_STORE)
+    F_PAIR = 3,    // C0 = A0 B0^T and C1 = A1 B1^T (epilogue E_STORE)
 };
 
 enum EpiKind {
@@ -63,7 +63,7 @@ struct Product {
     int form = F_SINGLE;
     Matrix a[2], b[2];
     int64_t M = 0, N = 0, K = 0;
-    bool a_mn = false;  // E_STORE: A's rows (not its contraction) are contiguous; B's rows always are
+    bool a_mn = false, b_mn = false;  // E_STORE: an operand's rows, not its contraction, are contiguous
     Epilogue e;
 };
 
@@ -111,9 +111,11 @@ constexpr int TC_ROWS = 32;
 struct Plan {
     int cg = 1, bn = 32;  // CTAs per tile, columns of the MMA
     int splits = 1;       // of the contraction
+    bool finish = false;  // the splits' sums get the epilogue in a kernel of its own (split_sums)
 };
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
 Plan tc_plan(const Product& p, int dt);
+Product split_sums(const Product& p);  // the same sums as a plain product, two for F_DUAL
 template <typename T>
 int tc_product(const Product& p, const Plan& plan, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);

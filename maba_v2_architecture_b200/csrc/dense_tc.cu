@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                                 load(sb + a.bn / 2 * 128, &tb1, k0, n0, pl);
                             }
                         } else {
-                            const CUtensorMap* mb = seg ? &tb1 : &tb0;
+                            const CUtensorMap* mb = (a.pairs == 2 ? pair : seg) ? &tb1 : &tb0;
                             const int y = n0 + (int)rank * a.b_rows;
                             if (B_MN) {
                                 for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0, pl);
@@ -892,8 +892,8 @@ int mode_of(const Product& p, int dt) {
 // a unit that is not hidden under another adds its fill and epilogue.  The registers that
 // hold a unit's sums bound bn in modes 1 and 2.  Splits also bound what one accumulation
 // truncates: at most 16,384 indices.
-Plan plan_of(const Product& p, int mode) {
-    const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE, b_mn = store;
+Plan plan_of(const Product& p, int mode, double* time) {
+    const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE;
     const int kblocks = (int)ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
     const int pairs = p.form == F_PAIR ? 2 : 1;
     const int planes = mode == 2 ? 3 : 1, terms = mode == 2 ? 6 : 1;
@@ -903,10 +903,12 @@ Plan plan_of(const Product& p, int mode) {
     double least = 1e300;
     for (int cg = 1; cg <= 2; ++cg) {
         const int most = mode == 2 ? 128 : (cg == 2 ? 256 : 192), slots = sm_count() / cg;
-        const double rows = (double)ceil_div(p.M, 128 * cg) * pairs;
+        const int m = (int)((p.M + 128 * cg - 1) / (128 * cg)), n = (int)p.N;
+        const double rows = (double)m * pairs;
         for (int bn = dual ? 64 : 32; bn <= most; bn += dual ? 64 : 32) {
-            const double tiles = rows * (double)ceil_div(p.N, dual ? bn / 2 : bn);
-            const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, b_mn)) / 60.0;
+            const int cols = dual ? bn / 2 : bn;
+            const double tiles = rows * (n / cols + (n % cols != 0));
+            const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, p.b_mn)) / 60.0;
             const double kcost = mma > load ? mma : load;
             for (int i = 0; i < (store ? 16 : 1); ++i) {
                 const int kb = (kblocks + fewest + i - 1) / (fewest + i);  // blocks of a split
@@ -914,11 +916,12 @@ Plan plan_of(const Product& p, int mode) {
                 const double waves = std::ceil(tiles * splits / slots);
                 // (a bit more for the partial sums: a second kernel)
                 const double t = waves * kb * kcost + 2000.0 + 12.0 * bn + (splits > 1 ? 2000.0 + splits * out : 0.0);
-                if (t < least) least = t, best = Plan{cg, bn, splits};
+                if (t < least) least = t, best.cg = cg, best.bn = bn, best.splits = splits;
                 if (waves * kb * kcost < 2000.0 || kb == 1) break;  // (more splits cannot pay)
             }
         }
     }
+    *time = least;
     return best;
 }
 
@@ -977,7 +980,9 @@ template <typename T, int CG> int kernel_of(Kernel* k, const Product& p, int mod
         case E_LINEAR_BWD: return ready<T, CG, false, false, E_LINEAR_BWD, M>(k, device);
         case E_GLU: return ready<T, CG, false, false, E_GLU, M>(k, device);
         case E_GLU_BWD: return ready<T, CG, false, false, E_GLU_BWD, M>(k, device);
-        default: return p.a_mn ? ready<T, CG, true, true, E_STORE, M>(k, device) : ready<T, CG, false, true, E_STORE, M>(k, device);
+        default:
+            if (p.a_mn) return ready<T, CG, true, true, E_STORE, M>(k, device);
+            return p.b_mn ? ready<T, CG, false, true, E_STORE, M>(k, device) : ready<T, CG, false, false, E_STORE, M>(k, device);
     }
 }
 
@@ -989,7 +994,32 @@ bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t 
     return rows == 1 || (ld % 8 == 0 && ld >= cols);
 }
 
-Plan tc_plan(const Product& p, int dt) { return plan_of(p, mode_of(p, dt)); }
+Product split_sums(const Product& p) {
+    Product q = p;
+    q.form = p.form == F_DUAL ? F_PAIR : p.form;
+    if (p.form == F_DUAL) q.a[1] = p.a[0];
+    q.e = Epilogue{};
+    return q;
+}
+
+// A product with an epilogue whose few tiles have a long contraction: its sums by splits,
+// then the epilogue, where the model says that this is sooner.  (24 x 3,776 -> 2 x 120 float32,
+// one tile of 59 blocks: forward and gradients 66 us, 139 without.)  A float32 result of 16-bit
+// operands keeps its bound on one accumulation, 640 indices.
+Plan tc_plan(const Product& p, int dt) {
+    const int mode = mode_of(p, dt);
+    double whole, split;
+    const Plan plan = plan_of(p, mode, &whole);
+    if (p.e.kind == E_STORE || p.K < 16 * BK) return plan;
+    const int64_t tiles = ceil_div(p.M, 128 * plan.cg) * ceil_div(p.N, p.form == F_DUAL ? plan.bn / 2 : plan.bn);
+    if (2 * tiles * plan.cg > sm_count()) return plan;
+    Plan parts = plan_of(split_sums(p), mode == 1 ? 0 : mode, &split);
+    // (the two more launches cost about 3 us)
+    if (parts.splits == 1 || split + 6000.0 >= 0.7 * whole) return plan;
+    if (mode == 1 && ceil_div(ceil_div(p.K, BK), parts.splits) > 640 / BK) return plan;
+    parts.finish = true;
+    return parts;
+}
 
 template <typename T>
 int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cudaStream_t s) {
@@ -997,7 +1027,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     constexpr int dt = sizeof(T) == 4 ? MABA_F32 : (std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16);
     constexpr int planes = dt == MABA_F32 ? 3 : 1, odt = dt == MABA_F16 ? MABA_F16 : MABA_BF16;
     const int mode = mode_of(p, dt);
-    const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE, a_mn = p.a_mn, b_mn = store;
+    const bool dual = p.form == F_DUAL, a_mn = p.a_mn, b_mn = p.b_mn;
     TcArgs a{};
     a.M = p.M, a.N = p.N;
     a.kseg = (int)ceil_div(p.K, BK);
@@ -1052,7 +1082,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     Kernel kern = nullptr;
     MABA_TRY((pl.cg == 2 ? kernel_of<T, 2>(&kern, p, mode, device) : kernel_of<T, 1>(&kern, p, mode, device)));
     CUtensorMap m[7];
-    const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = p.form == F_SUM || dual ? 2 : 1;
+    const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = na == 2 || dual ? 2 : 1;
     const int box = dual ? pl.bn / 2 : a.b_rows;
     bool ok = true;
     for (int i = 0; i < na; ++i) ok = ok && operand_map(&m[i], odt, p.a[i], planes, p.M, p.K, a_mn, 128);

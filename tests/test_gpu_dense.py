@@ -47,8 +47,11 @@ EPILOGUES = [("none", "none", "none", "none", None), ("silu", "f32", "none", "no
              ("gelu", "same", "f32", "same", None), ("relu", "none", "same", "f32", F32), ("none", "none", "f32", "f32", F32)]
 
 
+LONG = [(100, 4000, 40), (24, 3776, 120), (257, 1300, 33)]  # few tiles, a long contraction: split sums
+
+
 @pytest.mark.parametrize("dt", [BF, HF, F32])
-@pytest.mark.parametrize("m,k,n", SHAPES + LARGE)
+@pytest.mark.parametrize("m,k,n", SHAPES + LARGE + LONG)
 def test_linear(m, k, n, dt):
     for i, (act, bias, scale, residual, out_dtype) in enumerate(EPILOGUES):
         t = linear_case(m, k, n, dt, bias, scale, residual, seed=i)
@@ -60,7 +63,7 @@ def test_linear(m, k, n, dt):
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 64, 64), (3, 7, 5), (40, 136, 72), (65, 130, 72), (129, 641, 257),
-                                   (300, 96, 1003), (2100, 200, 136)] + LARGE)
+                                   (300, 96, 1003), (2100, 200, 136)] + LARGE + LONG)
 def test_linear_backward(m, k, n, dt):
     for i, (act, bias, scale, _, out_dtype) in enumerate(EPILOGUES + [("none", "f32", "none", "none", F32)]):
         t = linear_case(m, k, n, dt, bias, scale, "none", seed=i, grad=out_dtype or dt)
@@ -73,7 +76,7 @@ def test_linear_backward(m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
-@pytest.mark.parametrize("m,k,n", SHAPES + LARGE)
+@pytest.mark.parametrize("m,k,n", SHAPES + LARGE + LONG)
 def test_gated_ffn(m, k, n, dt):
     g = gen(5)
     x, wg, wu = randn(g, m, k, dt=dt), randn(g, n, k, dt=dt, std=k ** -0.5), randn(g, n, k, dt=dt, std=k ** -0.5)
@@ -83,7 +86,7 @@ def test_gated_ffn(m, k, n, dt):
 
 @pytest.mark.parametrize("dt", [BF, HF, F32])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 64, 64), (3, 7, 5), (40, 136, 72), (65, 130, 72), (129, 641, 257),
-                                   (300, 96, 1003), (2100, 200, 136)] + LARGE)
+                                   (300, 96, 1003), (2100, 200, 136)] + LARGE + LONG)
 def test_gated_ffn_backward(m, k, n, dt):
     g = gen(6)
     x, wg, wu = randn(g, m, k, dt=dt), randn(g, n, k, dt=dt, std=k ** -0.5), randn(g, n, k, dt=dt, std=k ** -0.5)
