@@ -386,3 +386,121 @@ def test_swiglu_module_trains():
     before = wg.clone()
     torch.optim.SGD(ffn.parameters(), lr=0.1).step()
     assert not torch.equal(ffn.w_gate.weight.detach(), before)
+
+
+# ---------------------------------------------------------------------------
+# extremes
+# ---------------------------------------------------------------------------
+def test_offsets_past_32_bits():
+    """More than 2^31 elements of output and of gradient (4.5 GB): the last rows, and a gradient
+    that sums over all of them."""
+    m, k, n = 1_100_003, 64, 2048
+    w = randn(gen(1), n, k, dt=BF, std=0.1)
+    x = randn(gen(2), m, k, dt=BF)
+    y = mb.b200_linear(x, w, activation="relu")
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 40), slice(m - 300, m)):
+        O.assert_within(y[rows], O.linear(x[rows], w, act="relu"), "rows")
+    a = mb.b200_gated_ffn(x, w, w, out=y)
+    O.assert_within(a[m - 300:], O.gated(x[m - 300:], w, w, "silu"), "last rows")
+    # a gradient that is 1 in the last row and 0 before: dw is that row's outer product
+    y.zero_()
+    y[m - 1] = 1
+    dx, dw, _, _ = mb.b200_linear_backward(y, x, w, activation="relu")
+    want = O.linear_backward(y[m - 1:], x[m - 1:], w, act="relu")
+    O.assert_within(dw, want["dw"], "dw")
+    O.assert_within(dx[m - 1:], want["dx"], "dx")
+    assert not dx[:m - 1].any()
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e30, 3e38])
+def test_float32_magnitudes(scale):
+    """Float32 operands at the ends of their range.  The tensor cores take a bf16 plane below 2^-126
+    for zero, so a small x is off by at most its second and third plane's loss, 2^-126 each: with one
+    nonzero w per sum, 2^-125 |w| beside 2^-22 of the value (at 1e-36 = 2^-120 with w = 1e36 that is
+    2 %; at 1e-30 and above nothing)."""
+    m, k, n = 70, 8, 40
+    g = gen(3)
+    x = (torch.rand(m, k, generator=g, device=DEV) * 0.5 + 0.5) * scale
+    w = torch.eye(k, device=DEV).repeat(n // k, 1) * (1.0 / scale if scale < 1 else 1e-3)
+    y = mb.b200_linear(x, w)
+    want = x.double() @ w.double().t()
+    tol = 2.0 ** -22 * want.abs() + 2.0 ** -125 * float(w.max())
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("m", [5, 70])
+def test_float16_subnormals(m):
+    """Float16 values below 2^-14 are operands like any other."""
+    x = torch.full((m, 64), 2.0 ** -20, dtype=HF, device=DEV)
+    x[:, 32:] = 3 * 2.0 ** -24
+    w = torch.full((40, 64), 512.0, dtype=HF, device=DEV)
+    want = 32 * 512 * (2.0 ** -20 + 3 * 2.0 ** -24)
+    assert bool((mb.b200_linear(x, w, out_dtype=F32) == want).all())
+
+
+def test_float32_infinities_as_in_float32():
+    """inf * w is the infinity of w's sign (its planes hold no inf * 0), inf * 0 and inf - inf are NaN."""
+    x = torch.ones(70, 8, device=DEV)
+    x[1, 2], x[2, 3], x[3, 0], x[3, 1] = float("inf"), float("-inf"), float("inf"), float("inf")
+    w = torch.full((40, 8), 0.3, device=DEV)
+    w[5, 2] = -0.7
+    w[6, 2] = 0.0
+    w[7, 0] = -1.0
+    y, want = mb.b200_linear(x, w), x.cpu() @ w.cpu().t()
+    assert torch.equal(y.isnan().cpu(), want.isnan()) and torch.equal(y.isinf().cpu(), want.isinf())
+    assert torch.equal(y[y.isinf()].cpu(), want[want.isinf()])
+    assert bool(y[10:].isfinite().all())
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing has to run before a call is captured: a fresh process captures its first calls."""
+    import subprocess
+    import sys
+    import os
+
+    code = """
+import torch, maba_v2_architecture_b200 as mb
+x = torch.randn(300, 96, device="cuda").bfloat16(); w = torch.randn(64, 96, device="cuda").bfloat16()
+f = torch.randn(300, 96, device="cuda"); v = torch.randn(64, 96, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = [mb.b200_linear(x, w), mb.b200_linear(x[:3], w), mb.b200_gated_ffn(f, v, v), mb.b200_linear(f[:2], v)]
+    outs += list(mb.b200_gated_ffn_backward(outs[0], x, w, w))
+g.replay(); torch.cuda.synchronize()
+again = [mb.b200_linear(x, w), mb.b200_linear(x[:3], w), mb.b200_gated_ffn(f, v, v), mb.b200_linear(f[:2], v)]
+again += list(mb.b200_gated_ffn_backward(again[0], x, w, w))
+assert all(torch.equal(a, b) for a, b in zip(outs, again))
+print("captured")
+"""
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=repo, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_threads_at_once():
+    """Calls from two host threads, each on its own stream."""
+    import threading
+
+    ts = [linear_case(m, 264, 200, BF, "f32", "f32", "none", seed=m, grad=BF) for m in (700, 1500)]
+    wu = randn(gen(9), 200, 264, dt=BF, std=0.06)
+    want = [train_calls(t, wu) for t in ts]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = train_calls(ts[i], wu)
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
