@@ -1066,7 +1066,7 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
         a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
         staging = epi * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
         a.stages = (int)((SMEM_MAX - fixed - staging) / a.stage_bytes);
-        if (a.stages >= (mode == 2 ? 2 : (mode == 1 ? 3 : 4))) break;
+        if (a.stages >= (mode == 2 ? 2 : 5)) break;
     }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     a.vec_at = a.stages * a.stage_bytes + staging;
