@@ -372,6 +372,8 @@ MABA_API size_t maba_decode_dgda_mix_workspace_size(int32_t n_heads);
  * (float32 or x's type, any strides, 0 included); outputs have unit column stride
  * and rows that do not overlap.  Optional tensors are NULL.  Sums are float32 and
  * each result is rounded once; nothing depends on the order in which CTAs run.
+ * float32 products run on the tensor cores as bf16 planes: float32's accuracy, but
+ * elements below 2^-102 are off by up to 2^-125.
  * Workspace: 256-byte aligned, of the size that the matching call reports for the
  * same tensors; one workspace serves one call at a time.
  *
@@ -387,7 +389,8 @@ MABA_API size_t maba_decode_dgda_mix_workspace_size(int32_t n_heads);
 MABA_API int maba_linear(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* bias, int32_t activation,
                          const maba_tensor* scale, const maba_tensor* residual, const maba_tensor* out,
                          void* workspace, size_t workspace_bytes, void* stream);
-MABA_API size_t maba_linear_workspace_size(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* out);
+MABA_API size_t maba_linear_workspace_size(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* residual,
+                                           const maba_tensor* out);
 MABA_API int maba_linear_backward(const maba_tensor* grad, const maba_tensor* x, const maba_tensor* weight,
                                   const maba_tensor* bias, int32_t activation, const maba_tensor* scale,
                                   const maba_tensor* dx, const maba_tensor* dw, const maba_tensor* dbias,

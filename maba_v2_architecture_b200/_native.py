@@ -63,7 +63,7 @@ SIGNATURES = {
     "maba_swiglu": (ctypes.c_int, [T_P, T_P, _vp]),
     # the dense entries take their descriptors as addresses of packed bytes (pack_matrix / pack_vector)
     "maba_linear": (ctypes.c_int, [_vp] * 3 + [_i32] + [_vp] * 3 + [_vp, _sz, _vp]),
-    "maba_linear_workspace_size": (_sz, [_vp] * 3),
+    "maba_linear_workspace_size": (_sz, [_vp] * 4),
     "maba_linear_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 5 + [_vp, _sz, _vp]),
     "maba_linear_backward_workspace_size": (_sz, [_vp] * 4 + [_i32] + [_vp] * 5),
     "maba_gated_ffn": (ctypes.c_int, [_vp] * 3 + [_i32, _vp, _vp, _sz, _vp]),

@@ -50,8 +50,10 @@ __device__ __forceinline__ void split_planes(float x, __nv_bfloat16 (&v)[3]) {
     }
 }
 
-// Operands made readable, up to three in one launch: dst [rows][ld] of a 16-bit type = src (that
-// type or float32, any strides), or the three planes of a float32 src.  Tiles of 32 x 64; where
+// Matrices made readable for the tensor-memory copies, up to four in one launch: dst [rows][ld] of
+// a 16-bit type = src (that type or float32, any strides), float32 = float32, or the three planes
+// of a float32 src (4,096 x 640 and 1,544 x 640:
+// 36 MB in and out, 13 us).  Tiles of 32 x 64; where
 // the source's columns are not contiguous they pass through shared memory, so that both sides
 // run along their contiguous axis.
 struct Job {
@@ -59,12 +61,17 @@ struct Job {
     int64_t rows = 0, cols = 0;
     void* dst = nullptr;
     int64_t ld = 0, plane = 0;
+    int f32 = 0;  // a float32 copy
 };
 struct Jobs {
-    Job j[3];
+    Job j[4];
     int n = 0;
 };
 template <typename T> __device__ __forceinline__ void put_pair(const Job& b, int64_t at, float x, float y) {
+    if (b.f32) {
+        *reinterpret_cast<float2*>(static_cast<float*>(b.dst) + at) = make_float2(x, y);
+        return;
+    }
     if constexpr (sizeof(T) == 4) {
         __nv_bfloat16 p[3], q[3];
         split_planes(x, p), split_planes(y, q);
@@ -415,7 +422,20 @@ void operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
     const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
     void* to = c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2);
     m = Matrix{to, ld, 1, plane};
-    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, plane};
+    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, plane, 0};
+}
+// A matrix that an epilogue of the tensor-core products reads: copied where its rows are not on
+// 16-byte boundaries (a broadcast one too).
+Side side_of(Ctx& c, const maba_tensor* t, bool as_is = false) {
+    const Side src = side2(t);
+    if (!given(t) || as_is) return src;
+    const int64_t rows = t->shape[0], cols = t->shape[1], per = src.f32 ? 4 : 8;
+    if (src.sc == 1 && (rows == 1 || (src.sr % per == 0 && src.sr >= cols)) && (reinterpret_cast<uintptr_t>(src.p) & 15u) == 0)
+        return src;
+    const int64_t ld = (cols + 7) / 8 * 8;
+    void* to = c.ws.take((size_t)rows * ld * (src.f32 ? 4 : 2));
+    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, 0, src.f32};
+    return Side{to, ld, 1, src.f32};
 }
 // A gradient that an epilogue writes as an operand of the next products.
 Matrix written_operand(Ctx& c, int64_t rows, int64_t cols) {
@@ -438,9 +458,10 @@ int linear_forward(Ctx& c, const LinearArgs& a) {
     const bool as_is = skinny_takes(p, c.dt);
     operand(c, a.x, p.a[0], as_is);
     operand(c, a.w, p.b[0], as_is);
+    p.e.res = side_of(c, a.res, as_is);
     MABA_TRY(prepare(c));
     p.e.act = a.act;
-    p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.res);
+    p.e.bias = side1(a.bias), p.e.scale = side1(a.scale);
     if (a.out) p.e.out = a.out->data, p.e.ldo = a.out->stride[0], p.e.out_f32 = a.out->dtype == MABA_F32;
     return run(c, p);
 }
@@ -495,6 +516,8 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
     if (!through || need_dx) operand(c, a.w, w);
     // (the products take one type: where dz = g, a float32 gradient is rounded to x's here)
     if (through && (need_dx || need_dw)) operand(c, a.g, d);
+    Side g;
+    if (!through) g = side_of(c, a.g);
     MABA_TRY(prepare(c));
     if (!through) {
         // z again, rather than a copy kept by the forward pass: a 16-bit z would add its own
@@ -505,7 +528,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         p.a[0] = x, p.b[0] = w;
         p.e.kind = E_LINEAR_BWD;
         p.e.act = a.act;
-        p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = side2(a.g);
+        p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = g;
         p.e.out = const_cast<void*>(d.p), p.e.ldo = d.sr, p.e.planes = d.sp;
         p.e.part_bias = pb, p.e.part_scale = ps;
         MABA_TRY(run(c, p));
@@ -534,6 +557,7 @@ int ffn_product(Ctx& c, const FfnArgs& a, Product& p) {
     operand(c, a.x, p.a[0], as_is);
     operand(c, a.wg, p.b[0], as_is);
     operand(c, a.wu, p.b[1], as_is);
+    p.e.res = side_of(c, a.g);
     return prepare(c);
 }
 
@@ -557,7 +581,6 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
     // the one rounding between the two passes
     const Matrix d[2] = {written_operand(c, M, p.N), written_operand(c, M, p.N)};
-    p.e.res = side2(a.g);
     p.e.out = const_cast<void*>(d[0].p), p.e.out2 = const_cast<void*>(d[1].p), p.e.ldo = d[0].sr, p.e.planes = d[0].sp;
     MABA_TRY(run(c, p));
     if (given(a.dx)) MABA_TRY(dx_product(c, M, p.N, 2, d, p.b, a.dx));
@@ -641,9 +664,10 @@ extern "C" int maba_linear(const maba_tensor* x, const maba_tensor* weight, cons
     return execute(a, linear_forward, "linear", workspace, workspace_bytes, stream);
 }
 
-extern "C" size_t maba_linear_workspace_size(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* out) {
+extern "C" size_t maba_linear_workspace_size(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* residual,
+                                             const maba_tensor* out) {
     LinearArgs a{};
-    a.x = x, a.w = weight, a.out = out;
+    a.x = x, a.w = weight, a.res = residual, a.out = out;
     if (check_linear(a, false) != MABA_OK) return 0;
     return query(a, linear_forward).ws.used;
 }

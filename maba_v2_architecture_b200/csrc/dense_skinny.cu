@@ -13,6 +13,11 @@
 // contraction, four elements per lane and step.
 //
 // Both read any strides (element by element where rows are not 16-byte aligned).
+//
+// On the device, bf16: one token through 640 -> 2 x 1248 3.3 us, through 1248 -> 640 3.6 us (3.2 MB
+// and 1.6 MB of weights: a quarter of the time is their bytes, the rest one chain of loads, the
+// exchange and the launch); 48 tokens through 640 -> 1544 5.4 us, where a tile of the tensor-core
+// kernel (128 rows, its set-up and its pipeline's fill) takes 7.
 #include "dense.cuh"
 #include "mma_util.cuh"
 

@@ -5,7 +5,9 @@
 // six down to 2^-16 are taken, x1 w1 into one accumulator, x1 w2 + x2 w1 + x2 w2 + x1 w3 +
 // x3 w1 into a second, and what is left out is below 2^-23 of |x w|: float32's own rounding,
 // at six tensor products instead of the CUDA cores' one (where main is an infinity or NaN the
-// second sum, which may hold inf * 0, is not added).
+// second sum, which may hold inf * 0, is not added).  The tensor cores take a bf16 below
+// 2^-126 for zero, so an x below 2^-102 is off by up to 2^-125.  4,096 x 640 -> 1544: 48 us,
+// 1.0 PFLOP/s of bf16 products, 170 TFLOP/s of float32; a CUDA-core kernel took 346 us.
 //
 // The tensor cores truncate when they add to their float32 accumulator, once per 16
 // contraction indices: a sum over K loses about K 5.6e-10 of itself toward zero (measured
@@ -16,16 +18,26 @@
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
 // A and one half of B, so a k-block costs an SM 32 KB for 128 x 256 x 64 products instead
-// of 48 KB, below what L2 delivers per SM) over one split of the contraction.  Twelve warps:
-//  * 0..7   epilogue: warp w reads TMEM lanes 32 (w & 3).. and every fourth 32-column
-//           chunk, applies the epilogue and stores whole rows' segments, staged through
-//           shared memory so that global accesses run along the rows;
-//  * 8      TMA producer: 64 contraction indices per stage, 128-byte swizzle, operands
-//           K-major or (for the transposed products of the backward pass) MN-major;
-//  * 9      allocates TMEM and issues the products.
+// of 48 KB, below what L2 delivers per SM: 199 -> 165 us for the gated block of 65,536 x 640
+// -> 2 x 1248) over one split of the contraction.  The warps:
+//  * epilogue (16, or 8 where they hold a unit's sums): warp w reads TMEM lanes 32 (w & 3)..
+//           and every fourth (second) 32-column chunk and applies the epilogue;
+//  * TMA producer: 64 contraction indices per stage, 128-byte swizzle, operands K-major or
+//           (for the transposed products of the backward pass) MN-major;
+//  * MMA:   allocates TMEM and issues the products, one thread (a warp-wide loop with an
+//           election for each took 560 cycles to issue a k-block of 512);
+//  * side:  brings the epilogue's residual or gradient, 128 rows x 32 columns a copy.
 // The float32 accumulator is double-buffered in TMEM (2 x 256 columns): a unit's epilogue
 // runs under the next unit's products.  The gated block's tile holds bn/2 rows of w_gate and
 // bn/2 of w_up, so a thread sees both projections of an element in its own row.
+//
+// What bounds it: the gated block the tensor cores (65,536 x 640 -> 2 x 1248, bf16: 146 us,
+// 1,433 TFLOP/s, 84 % of the 1,703 of an 8,192^3 library product; its two SFU operations per
+// element take 2,048 of a unit's 5,120 cycles); the linear map with a scale and a float32
+// residual (65,536 x 1248 -> 640) 118 us, 4.3 TB/s; with a bias, SiLU, scale and residual
+// (16,384 x 640 -> 2560) 66 us, by the epilogue's chains of shared-memory, barrier and copy
+// latencies, which the products' own use of shared memory stretches; its gradient pass, with
+// column sums, 84 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
@@ -80,7 +92,7 @@ struct TcArgs {
     int stages;
     uint32_t stage_bytes, b_at, b_bytes, load_bytes;  // B's place in a stage, one plane of it, bytes per stage
     uint32_t idesc;
-    int side_tma, out_tma;               // the epilogue's matrices move by copies
+    int out_tma;                         // the results leave by copies
     int n_in, n_out;                     // staging buffers per warp
     uint32_t in_bytes, out_bytes, vec_at, bar_at;  // of one buffer; places of the vectors and the barriers
     Epilogue e;
@@ -182,7 +194,8 @@ template <typename F> __device__ __forceinline__ void with_act(int act, F f) {
 // load/store unit's address stage).  A buffer has the copy's swizzle: rows of 128 bytes
 // (float32) or 64 (16 bits), 16-byte piece p of row r at p ^ (r & 7) or p ^ (r / 2 & 3), so
 // that a lane can read its row, or eight lanes a column of pieces, without bank conflicts.
-// What a copy cannot address (unaligned rows, strides) moves element by element, out of line.
+// A result that a copy cannot address (rows not on 16-byte boundaries) is stored element by
+// element, out of line; what is read has been made readable.
 // --------------------------------------------------------------------------
 __device__ __forceinline__ uint4* at32(unsigned char* st, int row, int piece) {
     return reinterpret_cast<uint4*>(st + row * 128 + ((piece ^ (row & 7)) << 4));
@@ -194,18 +207,7 @@ template <typename E> __device__ __forceinline__ E* element(unsigned char* st, i
     return sizeof(E) == 4 ? reinterpret_cast<E*>(at32(st, r, c >> 2)) + (c & 3)
                           : reinterpret_cast<E*>(at16(st, r, c >> 3)) + (c & 7);
 }
-// (src, dst: the chunk's first element)
-template <typename E>
-__device__ __noinline__ void stage_in(unsigned char* st, const E* src, int64_t sr, int64_t sc, int rows, int cols, int lane) {
-#pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += 16) {
-        E v[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = r0 + r < rows && lane < cols ? src[(r0 + r) * sr + lane * sc] : E(0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) *element<E>(st, r0 + r, lane) = v[r];
-    }
-}
+// (dst: the chunk's first element)
 template <typename E>
 __device__ __noinline__ void stage_out(unsigned char* st, E* dst, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll 8
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     } else if (warp == W_SIDE && KIND != E_STORE && KIND != E_GLU) {
         // ================= residual or gradient, chunk by chunk ================
         // One copy brings 32 columns of the CTA's 128 rows, a chunk of each of a group's warps.
-        if (a.side_tma && elect_one()) {
+        if (a.e.res.p != nullptr && elect_one()) {
             const int width = KIND == E_GLU_BWD ? a.bn / 2 : a.bn;
             uint32_t count[GROUPS] = {};
             bool ok = true;
@@ -596,25 +598,14 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         // ---- residual or gradient
         uint32_t used = 0;
         bool ok = true;
-        auto side_ready = [&](const Chunk& k) {
-            if (a.side_tma) {
-                const uint32_t slot = a.n_in == 2 ? used & 1 : 0, use = a.n_in == 2 ? used >> 1 : used;
-                ok = mbar_wait_warp(&bars[B_SFULL + 2 * h + slot], use & 1, abort_f);
-                return in_buf + slot * 4 * a.in_bytes;
-            }
-            __syncwarp();
-            if (side_f32)
-                stage_in<float>(in_buf, static_cast<const float*>(e.res.p) + k.row0 * e.res.sr + k.col0 * e.res.sc, e.res.sr,
-                                e.res.sc, k.rows, k.cols, lane);
-            else
-                stage_in<uint16_t>(in_buf, static_cast<const uint16_t*>(e.res.p) + k.row0 * e.res.sr + k.col0 * e.res.sc,
-                                   e.res.sr, e.res.sc, k.rows, k.cols, lane);
-            __syncwarp();
-            return in_buf;
+        auto side_ready = [&]() {
+            const uint32_t slot = a.n_in == 2 ? used & 1 : 0, use = a.n_in == 2 ? used >> 1 : used;
+            ok = mbar_wait_warp(&bars[B_SFULL + 2 * h + slot], use & 1, abort_f);
+            return in_buf + slot * 4 * a.in_bytes;
         };
         auto side_used = [&]() {
             __syncwarp();
-            if (a.side_tma && lane == 0) mbar_arrive(&bars[B_SEMPTY + 2 * h + (a.n_in == 2 ? used & 1 : 0)]);
+            if (lane == 0) mbar_arrive(&bars[B_SEMPTY + 2 * h + (a.n_in == 2 ? used & 1 : 0)]);
             ++used;
         };
         // ---- results
@@ -691,7 +682,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             const Chunk k = place(t, c);
             if (k.cols <= 0) return;
             if (k.rows <= 0) {  // (the group's copy still counts this warp)
-                if (has_side && a.side_tma) side_ready(k), side_used();
+                if (has_side) side_ready(), side_used();
                 return;
             }
             unsigned char* in = nullptr;
@@ -704,14 +695,14 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 });
                 if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
                 if (has_side) {
-                    in = side_ready(k);
+                    in = side_ready();
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) { add2(z[j], z[j + 1], g0, g1); });
                     side_used();
                 }
             } else if (KIND == E_LINEAR_BWD) {
                 float sb[8] = {}, ss[8] = {};  // this lane's part of its eight columns' sums
                 if (e.bias.p) with_vector<FRAG>(z, vb, lane, add2);
-                in = side_ready(k);
+                in = side_ready();
                 with_act(e.act, [&](auto A) {
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
                         float y0, y1, d0, d1;
@@ -747,7 +738,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                     }
                 });
             } else if (KIND == E_GLU_BWD) {
-                in = side_ready(k);
+                in = side_ready();
                 with_act(e.act, [&](auto A) {
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
                         float y0, y1, d0, d1;
@@ -1091,8 +1082,8 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     if (na == 1) m[1] = m[0];
     if (nb == 1) m[3] = m[2];
     m[4] = m[5] = m[6] = m[0];
-    a.side_tma = p.e.res.p && p.e.res.sc == 1 &&
-                 chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1, 128);
+    if (p.e.res.p && !chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1, 128))
+        return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     if (a.splits > 1) {
         a.out_tma = chunk_map(&m[5], MABA_F32, partial, p.M, p.N, ldp, a.splits * a.pairs);
     } else if (to_planes) {

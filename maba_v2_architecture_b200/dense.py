@@ -9,14 +9,15 @@ The reference computes these with torch modules and autograd: SwiGLUFFN (maba_sp
 
 Inputs are float32, float16 or bfloat16 CUDA tensors of one type with any strides; leading
 dimensions of ``x`` are rows.  Sums are float32 and a result is rounded once; results do not
-depend on the order in which the GPU runs the work.  Inputs are never written, except that
+depend on the order in which the GPU runs the work.  Float32 products have float32's accuracy (they
+run on the tensor cores as three bf16 planes each; elements below 2^-102 are off by up to 2^-125).  Inputs are never written, except that
 ``out`` may be ``residual``.  Work is enqueued on the current stream of the tensors' device.
 Scratch memory comes from torch's allocator for each call (not from the per-stream buffer that
 the other ops keep): two captured graphs, or a graph and an eager call, then never share it.
 
 With gradients enabled and an input that requires one, both functions record themselves for
-autograd; ``*_backward`` are the same gradients as plain calls, for training loops that are
-captured into a CUDA graph or keep their own tape.
+autograd (first derivatives); ``*_backward`` are the same gradients as plain calls, for training
+loops that are captured into a CUDA graph or keep their own tape.
 """
 from __future__ import annotations
 
@@ -163,7 +164,7 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
     if rc:
         if rc != N.ERR_WORKSPACE:
             N.check(rc, "maba_linear")
-        _call(lib.maba_linear, lib.maba_linear_workspace_size, x, (dx, dw, db, act, ds, dr, do), (dx, dw, do))
+        _call(lib.maba_linear, lib.maba_linear_workspace_size, x, (dx, dw, db, act, ds, dr, do), (dx, dw, dr, do))
     return out
 
 
