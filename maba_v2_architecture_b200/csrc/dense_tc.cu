@@ -93,6 +93,7 @@ struct TcArgs {
     uint32_t stage_bytes, b_at, b_bytes, load_bytes;  // B's place in a stage, one plane of it, bytes per stage
     uint32_t idesc;
     int out_tma;                         // the results leave by copies
+    int in_place;                        // from the buffer that brought the residual or gradient
     int n_in, n_out;                     // staging buffers per warp
     uint32_t in_bytes, out_bytes, vec_at, bar_at;  // of one buffer; places of the vectors and the barriers
     Epilogue e;
@@ -598,26 +599,42 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         // ---- residual or gradient
         uint32_t used = 0;
         bool ok = true;
+        // (in place: a chunk's result is put over what was read and leaves from there, so its
+        // buffer goes back to the side warp when the next chunk is asked for, its copy out read)
+        int leaving = -1;
         auto side_ready = [&]() {
+            if (leaving >= 0) {
+                if (lane == 0) {
+                    bulk_wait_read<0>();
+                    mbar_arrive(&bars[B_SEMPTY + 2 * h + leaving]);
+                }
+                leaving = -1;
+            }
             const uint32_t slot = a.n_in == 2 ? used & 1 : 0, use = a.n_in == 2 ? used >> 1 : used;
             ok = mbar_wait_warp(&bars[B_SFULL + 2 * h + slot], use & 1, abort_f);
             return in_buf + slot * 4 * a.in_bytes;
         };
-        auto side_used = [&]() {
+        auto side_used = [&](bool stays) {
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[B_SEMPTY + 2 * h + (a.n_in == 2 ? used & 1 : 0)]);
+            const int slot = a.n_in == 2 ? (int)(used & 1) : 0;
+            if (stays) leaving = slot;
+            else if (lane == 0) mbar_arrive(&bars[B_SEMPTY + 2 * h + slot]);
             ++used;
         };
         // ---- results
         uint32_t stored = 0;
-        auto store = [&](const Chunk& k, const float* z, const CUtensorMap* map, void* dst, int64_t ld, int plane) {
-            unsigned char* buf = out_buf + (a.n_out == 2 ? (stored & 1) * a.out_bytes : 0u);
-            ++stored;
-            if (lane == 0) {
-                if (a.n_out == 2) bulk_wait_read<1>();
-                else bulk_wait_read<0>();
+        auto store = [&](const Chunk& k, const float* z, const CUtensorMap* map, void* dst, int64_t ld, int plane,
+                         unsigned char* in) {
+            unsigned char* buf = in;
+            if (in == nullptr) {
+                buf = out_buf + (a.n_out == 2 ? (stored & 1) * a.out_bytes : 0u);
+                ++stored;
+                if (lane == 0) {
+                    if (a.n_out == 2) bulk_wait_read<1>();
+                    else bulk_wait_read<0>();
+                }
+                __syncwarp();
             }
-            __syncwarp();
             put_chunk<OT, FRAG>(z, out_f32, buf, lane);
             if (a.out_tma) {
                 fence_proxy_async_smem();
@@ -682,7 +699,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             const Chunk k = place(t, c);
             if (k.cols <= 0) return;
             if (k.rows <= 0) {  // (the group's copy still counts this warp)
-                if (has_side) side_ready(), side_used();
+                if (has_side) side_ready(), side_used(false);
                 return;
             }
             unsigned char* in = nullptr;
@@ -697,7 +714,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 if (has_side) {
                     in = side_ready();
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) { add2(z[j], z[j + 1], g0, g1); });
-                    side_used();
+                    side_used(a.in_place);
                 }
             } else if (KIND == E_LINEAR_BWD) {
                 float sb[8] = {}, ss[8] = {};  // this lane's part of its eight columns' sums
@@ -715,7 +732,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                         ss[c] = y0, ss[c + 1] = y1;
                     });
                 });
-                side_used();
+                side_used(a.in_place);
                 if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) add2(sb[((j >> 2) & 3) * 2], sb[((j >> 2) & 3) * 2 + 1], z[j], z[j + 1]);
@@ -750,7 +767,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                         mul2(z[j], z[j + 1], d0, d1);
                     });
                 });
-                side_used();
+                side_used(false);
             }
             if (TO_PLANES) {
 #pragma unroll
@@ -758,18 +775,18 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = next_plane(pl < 3 ? z[j] : w[j]);
-                    store(k, v, pl < 3 ? &tout : &tout2, nullptr, e.ldo, pl % 3);
+                    store(k, v, pl < 3 ? &tout : &tout2, nullptr, e.ldo, pl % 3, nullptr);
                 }
                 return;
             }
             if (KIND == E_STORE && a.splits > 1) {
                 const int part = t.split(a) * a.pairs + t.pair(a);
-                store(k, z, &tout, a.partial + (int64_t)part * a.M * a.ldp, a.ldp, part);
+                store(k, z, &tout, a.partial + (int64_t)part * a.M * a.ldp, a.ldp, part, nullptr);
             } else {
                 const bool second = t.pair(a) != 0;
-                store(k, z, second ? &tout2 : &tout, second ? e.out2 : e.out, e.ldo, 0);
+                store(k, z, second ? &tout2 : &tout, second ? e.out2 : e.out, e.ldo, 0, a.in_place ? in : nullptr);
             }
-            if (KIND == E_GLU_BWD) store(k, w, &tout2, e.out2, e.ldo, 0);
+            if (KIND == E_GLU_BWD) store(k, w, &tout2, e.out2, e.ldo, 0, nullptr);
         };
 
         Unit t = first_unit();
@@ -1053,11 +1070,13 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.out_bytes = out_f32 ? 4096 : 2048;
     const uint32_t fixed = 1024 + BAR_BYTES + vec_bytes;
     uint32_t staging = 0;
+    a.in_place = p.e.res.p && (p.e.kind == E_LINEAR || (p.e.kind == E_LINEAR_BWD && !to_planes)) && side_f32 == out_f32;
+    if (a.in_place) a.out_bytes = 0;
     for (int t = 0; t < 3; ++t) {
         a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
         staging = epi * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
         a.stages = (int)((SMEM_MAX - fixed - staging) / a.stage_bytes);
-        if (a.stages >= (mode == 2 ? 2 : 5)) break;
+        if (a.stages >= (mode == 2 ? 2 : (a.in_place ? 4 : 5))) break;
     }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     a.vec_at = a.stages * a.stage_bytes + staging;
