@@ -531,6 +531,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = g;
         p.e.out = const_cast<void*>(d.p), p.e.ldo = d.sr, p.e.planes = d.sp;
         p.e.part_bias = pb, p.e.part_scale = ps;
+        p.e.sums_f32 = (need_db && a.dbias->dtype == MABA_F32) || (need_ds && a.dscale->dtype == MABA_F32);
         MABA_TRY(run(c, p));
     } else if (need_db) {
         MABA_TRY(column_sums(c, side2(a.g), M, N, pb));

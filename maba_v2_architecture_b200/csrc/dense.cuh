@@ -57,6 +57,7 @@ struct Epilogue {
     Side bias, scale, res;
     float* part_bias = nullptr;   // E_LINEAR_BWD: [row blocks][N] column sums of dz
     float* part_scale = nullptr;  // and of g * act(z + bias)
+    int sums_f32 = 0;             // they end in a float32 gradient
 };
 
 struct Product {

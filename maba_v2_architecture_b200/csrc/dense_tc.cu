@@ -889,9 +889,11 @@ inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
 }
 
 // How a product's sums are kept: 0 one accumulation (16-bit results), 1 added up in registers
-// every 640 indices (float32 results of 16-bit operands), 2 float32 operands, every 320.
+// every 640 indices (16-bit operands whose results, or column sums, are float32), 2 float32
+// operands, every 320.
 int mode_of(const Product& p, int dt) {
     if (dt == MABA_F32) return 2;
+    if (p.e.kind == E_LINEAR_BWD) return p.e.sums_f32 && p.K > 640 ? 1 : 0;
     return p.e.kind == E_LINEAR && p.e.out_f32 ? 1 : 0;
 }
 
@@ -982,7 +984,9 @@ template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> int read
 template <typename T, int CG> int kernel_of(Kernel* k, const Product& p, int mode, int device) {
     constexpr int M = sizeof(T) == 4 ? 2 : 0;
     if constexpr (M == 0)
-        if (mode == 1) return ready<T, CG, false, false, E_LINEAR, 1>(k, device);
+        if (mode == 1)
+            return p.e.kind == E_LINEAR ? ready<T, CG, false, false, E_LINEAR, 1>(k, device)
+                                        : ready<T, CG, false, false, E_LINEAR_BWD, 1>(k, device);
     switch (p.e.kind) {
         case E_LINEAR: return ready<T, CG, false, false, E_LINEAR, M>(k, device);
         case E_LINEAR_BWD: return ready<T, CG, false, false, E_LINEAR_BWD, M>(k, device);

@@ -504,3 +504,21 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("m,k,n", [(900, 3000, 300), (64, 1500, 40)])
+def test_float32_results_of_long_sums(m, k, n, dt):
+    """What ends in float32 (a float32 result, the gradient of a float32 scale) does not lose what the
+    tensor cores truncate over a long contraction.  An accumulation of 640 random products loses 6e-7
+    of its own size; those of a sum add like its parts do, in quadrature, so the sum loses 6e-7 of its
+    norm whatever its length, and the rounding of the additions (2^-24 each) stays below 1e-7.  One
+    accumulation of 3,000 would lose 3e-6."""
+    t = linear_case(m, k, n, dt, "f32", "f32", "none", seed=2, grad=dt)
+    y = mb.b200_linear(t["x"], t["w"], t["bias"], "none", t["scale"], out_dtype=F32)
+    want = (t["x"].double() @ t["w"].double().t() + t["bias"].double()) * t["scale"].double()
+    assert float((y.double() - want).norm() / want.norm()) <= 1e-6
+    ds = mb.b200_linear_backward(t["g"], t["x"], t["w"], t["bias"], "none", t["scale"])[3]
+    z = t["x"].double() @ t["w"].double().t() + t["bias"].double()
+    want = (t["g"].double() * z).sum(0)
+    assert float((ds.double() - want).norm() / want.norm()) <= 1e-6
