@@ -163,10 +163,17 @@ __global__ void __launch_bounds__(256)
         for (int64_t m = blk * 32 + w; m < M && m < blk * 32 + 32; m += 8) {
             if (n >= N) break;
             float z = 0.f, u = 0.f;
-            for (int q = 0; q < splits; ++q) {
-                const float* p = partial + ((int64_t)q * (dual ? 2 : 1) * M + m) * ldp + n;
-                z += p[0];
-                if (dual) u += p[M * ldp];
+            const float* p = partial + m * ldp + n;
+            const int64_t one = M * ldp, step = dual ? 2 * one : one;
+            for (int q0 = 0; q0 < splits; q0 += 8) {  // eight loads in flight, added in order
+                float v[8], w[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    v[q] = q0 + q < splits ? p[(q0 + q) * step] : 0.f;
+                    w[q] = dual && q0 + q < splits ? p[(q0 + q) * step + one] : 0.f;
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) z += v[q], u += w[q];
             }
             const int64_t at = m * e.ldo + n;
             float r[2];

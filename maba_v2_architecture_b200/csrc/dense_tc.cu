@@ -920,14 +920,16 @@ Plan plan_of(const Product& p, int mode, double* time) {
             const double tiles = rows * (n / cols + (n % cols != 0));
             const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, p.b_mn)) / 60.0;
             const double kcost = mma > load ? mma : load;
-            for (int i = 0; i < (store ? 16 : 1); ++i) {
-                const int kb = (kblocks + fewest + i - 1) / (fewest + i);  // blocks of a split
-                const int splits = (kblocks + kb - 1) / kb;                // none of them empty
+            // as few splits as may be, or as many as fill the GPU once, twice (up to 15 more)
+            for (int i = 0; i < (store ? 3 : 1); ++i) {
+                const double fill = i * (slots / tiles);
+                const int ask = i == 0 || fill < fewest ? fewest : (fill > fewest + 15 ? fewest + 15 : (int)fill);
+                const int kb = (kblocks + ask - 1) / ask;    // blocks of a split
+                const int splits = (kblocks + kb - 1) / kb;  // none of them empty
                 const double waves = std::ceil(tiles * splits / slots);
                 // (a bit more for the partial sums: a second kernel)
                 const double t = waves * kb * kcost + 2000.0 + 12.0 * bn + (splits > 1 ? 2000.0 + splits * out : 0.0);
                 if (t < least) least = t, best.cg = cg, best.bn = bn, best.splits = splits;
-                if (waves * kb * kcost < 2000.0 || kb == 1) break;  // (more splits cannot pay)
             }
         }
     }

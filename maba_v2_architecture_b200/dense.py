@@ -122,7 +122,7 @@ def _call(fn, size, x: torch.Tensor, head, size_args) -> None:
         with torch.cuda.device(index):
             return _call(fn, size, x, head, size_args)
     nbytes = size(*size_args)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = fn(*head, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
     if rc != N.OK:
         N.check(rc, fn.__name__)
@@ -170,10 +170,10 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
 
 def _linear_backward(grad_out, x, weight, bias, act, scale, needs):
     need_x, need_w, need_b, need_s = needs
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if need_w else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if need_b else None
-    ds = torch.empty(scale.shape, dtype=scale.dtype, device=x.device) if need_s else None
+    dx = x.new_empty(x.shape) if need_x else None
+    dw = x.new_empty(weight.shape) if need_w else None
+    db = bias.new_empty(bias.shape) if need_b else None
+    ds = scale.new_empty(scale.shape) if need_s else None
     if need_x or need_w or need_b or need_s:
         lib = N.lib()
         args = (_mat(grad_out), _mat(x), _mat(weight), _vec(bias), act, _vec(scale), _mat(dx), _mat(dw), _vec(db), _vec(ds))
@@ -300,9 +300,9 @@ def _gated_ffn(x, w_gate, w_up, act, out):
 
 def _gated_ffn_backward(grad_out, x, w_gate, w_up, act, needs):
     need_x, need_g, need_u = needs
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    dg = torch.empty(w_gate.shape, dtype=x.dtype, device=x.device) if need_g else None
-    du = torch.empty(w_up.shape, dtype=x.dtype, device=x.device) if need_u else None
+    dx = x.new_empty(x.shape) if need_x else None
+    dg = x.new_empty(w_gate.shape) if need_g else None
+    du = x.new_empty(w_up.shape) if need_u else None
     if need_x or need_g or need_u:
         lib = N.lib()
         ins, outs = (_mat(grad_out), _mat(x), _mat(w_gate), _mat(w_up)), (_mat(dx), _mat(dg), _mat(du))
