@@ -4,11 +4,8 @@
 //
 // A call first lays its workspace out with a Scratch; the *_workspace_size entries run the
 // same code without launching, so size and use cannot differ.  Nothing is accumulated with
-// atomics: results do not depend on the order in which CTAs run.  Every kernel here is launched
-// with programmatic dependence (pdl.cuh) and waits for its predecessor before its first access
-// of global memory; a chain of them is ordered, since each waits.
+// atomics: results do not depend on the order in which CTAs run.
 #include "dense.cuh"
-#include "pdl.cuh"
 
 namespace maba {
 namespace dense {
@@ -33,6 +30,12 @@ struct Scratch {
         using T = __nv_bfloat16;                                                 \
         return __VA_ARGS__();                                                    \
     }()
+
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+    kern<<<grid, block, smem, s>>>(static_cast<KArgs>(args)...);
+    return check_launch("dense");
+}
 
 // ---------------------------------------------------------------------------
 // small kernels
@@ -86,8 +89,6 @@ template <typename T> __device__ __forceinline__ void put_pair(const Job& b, int
 }
 template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Jobs jobs) {
     __shared__ float tile[32][65];
-    griddep_launch_dependents();
-    griddep_wait();
     const Job& b = jobs.j[blockIdx.y];
     const unsigned tiles_c = (unsigned)((b.cols + 63) / 64);
     const int64_t tiles = (b.rows + 31) / 32 * tiles_c;
@@ -128,8 +129,6 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     sum_splits_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t rows, int64_t cols, T* out,
                       T* out2, int64_t half, int64_t ld) {
-    griddep_launch_dependents();
-    griddep_wait();
     const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 4;
     if (c >= cols) return;
     for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
@@ -152,8 +151,6 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 __global__ void __launch_bounds__(256)
     finish_kernel(const float* __restrict__ partial, int64_t ldp, int splits, int64_t M, int64_t N, const Epilogue e) {
-    griddep_launch_dependents();
-    griddep_wait();
     __shared__ float red[2][8][32];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t n = (int64_t)blockIdx.x * 32 + lane;
@@ -226,8 +223,6 @@ __global__ void __launch_bounds__(256)
 constexpr int CS_ROWS = 128;
 template <typename T>
 __global__ void __launch_bounds__(256) colsum_kernel(Side g, int64_t rows, int64_t cols, float* part) {
-    griddep_launch_dependents();
-    griddep_wait();
     const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int w = threadIdx.x >> 5;
     __shared__ float red[8][32];
@@ -254,8 +249,6 @@ struct Columns {
 };
 template <typename T>
 __global__ void __launch_bounds__(1024) colsum_finish_kernel(const Columns v, int64_t blocks, int64_t cols) {
-    griddep_launch_dependents();
-    griddep_wait();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.y;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     __shared__ float red[32][33];
@@ -306,11 +299,11 @@ int run(Ctx& c, const Product& p) {
         const int64_t cap = 32768;
         if (plan.finish) {
             const int64_t gy = ceil_div(p.M, 32);
-            return launch_pdl(finish_kernel<T>, dim3((unsigned)ceil_div(p.N, 32), (unsigned)(gy < cap ? gy : cap)), dim3(256), 0,
+            return launch(finish_kernel<T>, dim3((unsigned)ceil_div(p.N, 32), (unsigned)(gy < cap ? gy : cap)), dim3(256), 0,
                               c.s, partial, ldp, plan.splits, p.M, p.N, p.e);
         }
         const int64_t gy = ceil_div(rows, 8);
-        return launch_pdl(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), dim3(256),
+        return launch(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), dim3(256),
                           0, c.s, partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2),
                           p.M, p.e.ldo);
     });
@@ -331,7 +324,7 @@ int prepare(Ctx& c) {
     c.jobs.n = 0;
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        return launch_pdl(prepare_kernel<T>, grid, dim3(256), 0, c.s, jobs);
+        return launch(prepare_kernel<T>, grid, dim3(256), 0, c.s, jobs);
     });
 }
 
@@ -339,7 +332,7 @@ int column_sums(Ctx& c, const Side& g, int64_t rows, int64_t cols, float* part) 
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
         const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)ceil_div(rows, CS_ROWS));
-        return launch_pdl(colsum_kernel<T>, grid, dim3(256), 0, c.s, g, rows, cols, part);
+        return launch(colsum_kernel<T>, grid, dim3(256), 0, c.s, g, rows, cols, part);
     });
 }
 
@@ -355,7 +348,7 @@ int finish_columns(Ctx& c, const float* pb, const maba_tensor* db, const float* 
     }
     if (n == 0) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        return launch_pdl(colsum_finish_kernel<T>, dim3((unsigned)ceil_div(cols, 32), (unsigned)n), dim3(1024), 0, c.s, v, blocks,
+        return launch(colsum_finish_kernel<T>, dim3((unsigned)ceil_div(cols, 32), (unsigned)n), dim3(1024), 0, c.s, v, blocks,
                           cols);
     });
 }

@@ -43,7 +43,6 @@
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
 // freed and the error word behind maba_device_error() is set.
 #include "dense.cuh"
-#include "pdl.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 
@@ -374,13 +373,11 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         if (CG == 2) tmem_alloc_pair<TMEM_COLS>(tmem_slot);
         else tmem_alloc<TMEM_COLS>(tmem_slot);
     }
-    griddep_launch_dependents();
     tc_fence_before();
     __syncthreads();
     if (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    griddep_wait();  // all that precedes overlaps the previous kernel; every access of memory follows
 
     // A unit: splits innermost, then the pair index, then columns, then rows of tiles.  A worker
     // walks its units by adding (a division for each took the epilogue longer than a chunk).
@@ -470,10 +467,13 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 if (++st == a.stages) st = 0, phase ^= 1;
             }
         }
-        // every copy has landed before a CTA may exit (rank 0's barriers count the pair's)
-        if (rank == 0)
-            for (int s = 0; s < a.stages && s < it; ++s)
-                mbar_wait(&bars[B_FULL + s], (((it - 1 - s) / a.stages)) & 1, nullptr);
+        // every copy has landed (rank 0's barriers count the pair's), and every arrival that rank
+        // 0's products make on this CTA's barriers, before it may exit
+        for (int s = 0; s < a.stages && s < it; ++s) {
+            const uint32_t last = ((it - 1 - s) / a.stages) & 1;
+            if (rank == 0) mbar_wait(&bars[B_FULL + s], last, nullptr);
+            if (ok) ok = mbar_wait(&bars[B_EMPTY + s], last, abort_f);
+        }
         }
     } else if (warp == W_MMA) {
         // ============================ MMA issuer ==============================
@@ -532,6 +532,12 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             // every product has completed before TMEM is freed
             commit(&bars[B_DRAIN]);
             mbar_wait(&bars[B_DRAIN], 0, nullptr);
+            // and the epilogue's last arrivals, of both CTAs, have come in (buffers never used pass)
+            for (int i = 0; i < 2 && ok; ++i) {
+                ok = mbar_wait(&bars[B_TEMPTY + buf], tphase, abort_f);
+                buf ^= 1;
+                if (buf == 0) tphase ^= 1;
+            }
         }
     } else if (warp == W_SIDE && KIND != E_STORE && KIND != E_GLU) {
         // ================= residual or gradient, chunk by chunk ================
@@ -687,10 +693,12 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 if (CG == 2) mbar_arrive_cluster(cluster_addr(&bars[B_TEMPTY + buf], 0));
                 else mbar_arrive(&bars[B_TEMPTY + buf]);
             }
+            __syncwarp();
             buf ^= 1;
             if (buf == 0) phase ^= 1;
         };
         auto load_sums = [&](float* z, uint32_t at) {
+            __syncwarp();  // (a warp-wide instruction; one lane may come from issuing a copy)
             if (FRAG) tmem_ld_frag32(at, reinterpret_cast<uint32_t*>(z));
             else tmem_ld32(at, reinterpret_cast<uint32_t*>(z));
         };
@@ -876,6 +884,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         if (CG == 2) tmem_dealloc_pair<TMEM_COLS>(tmem);
         else tmem_dealloc<TMEM_COLS>(tmem);
     }
+    // the pair frees its TMEM together: neither CTA may be gone, or another in its place, before
+    if (CG == 2) cluster_sync();
     if (tid == 0 && *abort_f) atomicExch(&g_dense_error, 1);
 }
 
@@ -1124,14 +1134,12 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)pl.cg;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)pl.cg;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = (unsigned)pl.cg;
+    cfg.numAttrs = pl.cg == 2 ? 1 : 0;
     err = cudaLaunchKernelEx(&cfg, kern, a, m[0], m[1], m[2], m[3], m[4], m[5], m[6]);
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
