@@ -128,10 +128,14 @@ def _call(fn, size, x: torch.Tensor, head, size_args) -> None:
         N.check(rc, fn.__name__)
 
 
+def _rows(*ts: Optional[torch.Tensor]):
+    """Each tensor as a matrix of rows: a view where its strides allow one, else a copy, which the
+    caller holds until the launch (a descriptor keeps only its address)."""
+    return [t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1]) for t in ts]
+
+
 def _mat(t: Optional[torch.Tensor]) -> Optional[bytes]:
-    if t is None:
-        return None
-    return pack_matrix(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+    return None if t is None else pack_matrix(t)
 
 
 def _vec(t: Optional[torch.Tensor]) -> Optional[bytes]:
@@ -151,7 +155,8 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
     else:
         if x.numel() == 0:
             return out
-        dx, do, dr = _mat(x), _mat(out), _mat(residual)
+        held = _rows(x, out, residual)
+        dx, do, dr = map(_mat, held)
     dw = pack_matrix(weight)
     db = None if bias is None else pack_vector(bias)
     ds = None if scale is None else pack_vector(scale)
@@ -176,7 +181,9 @@ def _linear_backward(grad_out, x, weight, bias, act, scale, needs):
     ds = scale.new_empty(scale.shape) if need_s else None
     if need_x or need_w or need_b or need_s:
         lib = N.lib()
-        args = (_mat(grad_out), _mat(x), _mat(weight), _vec(bias), act, _vec(scale), _mat(dx), _mat(dw), _vec(db), _vec(ds))
+        held = _rows(grad_out, x, weight, dx, dw)
+        mg, mx, mw, mdx, mdw = map(_mat, held)
+        args = (mg, mx, mw, _vec(bias), act, _vec(scale), mdx, mdw, _vec(db), _vec(ds))
         _call(lib.maba_linear_backward, lib.maba_linear_backward_workspace_size, x, args, args)
     return dx, dw, db, ds
 
@@ -284,7 +291,8 @@ def _gated_ffn(x, w_gate, w_up, act, out):
     else:
         if x.numel() == 0:
             return out
-        dx, do = _mat(x), _mat(out)
+        held = _rows(x, out)
+        dx, do = map(_mat, held)
     dg, du = pack_matrix(w_gate), pack_matrix(w_up)
     lib = N.lib()
     index = x.get_device()
@@ -305,7 +313,9 @@ def _gated_ffn_backward(grad_out, x, w_gate, w_up, act, needs):
     du = x.new_empty(w_up.shape) if need_u else None
     if need_x or need_g or need_u:
         lib = N.lib()
-        ins, outs = (_mat(grad_out), _mat(x), _mat(w_gate), _mat(w_up)), (_mat(dx), _mat(dg), _mat(du))
+        held = _rows(grad_out, x, w_gate, w_up, dx, dg, du)
+        packed = [_mat(t) for t in held]
+        ins, outs = packed[:4], packed[4:]
         _call(lib.maba_gated_ffn_backward, lib.maba_gated_ffn_backward_workspace_size, x, (*ins, act, *outs),
               (*ins, *outs))
     return dx, dg, du

@@ -1,5 +1,6 @@
 """Refusals of the dense operators, without a GPU: shapes, types, devices, activations, out."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -162,3 +163,16 @@ def test_install_patches_the_ffn_only_when_asked(monkeypatch):
     assert SwiGLUFFN.forward is mb.SwiGLUFFN.forward
     uninstall(h)
     assert SwiGLUFFN.forward is before
+
+
+def test_copies_of_inputs_are_held_until_the_launch(monkeypatch):
+    """Inputs that no view turns into rows are copied: the copies are alive, so apart, at the launch."""
+    launches = []
+    monkeypatch.setattr(dense, "_call", lambda fn, size, x, head, size_args: launches.append(head))
+    x, g = (torch.zeros(6, 5, 32).transpose(0, 1) for _ in range(2))
+    w = torch.zeros(32, 32)
+    dense._linear_backward(g, x, w, None, 0, None, (True, True, False, False))
+    dense._gated_ffn_backward(g, x, w, w, 2, (True, True, True))
+    for head in launches:
+        places = [struct.unpack_from("Q", d)[0] for d in head if isinstance(d, bytes)]
+        assert len(set(places)) == len(places) - (head[2] == head[3])  # (one weight is given twice)

@@ -213,6 +213,22 @@ def test_rows_do_not_mix(dt, m):
 # ---------------------------------------------------------------------------
 # gradients: needs, differences, autograd
 # ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_inputs_without_a_view_as_rows(dt):
+    """Leading dimensions that only a copy makes rows of, for two inputs of the same size at once."""
+    x, g = (randn(gen(i), 60, 50, 128, dt=dt).transpose(0, 1) for i in (5, 6))
+    w, wu = (randn(gen(i), 128, 128, dt=dt, std=0.1) for i in (7, 8))
+    r = randn(gen(9), 60, 50, 128, dt=dt).transpose(0, 1)
+    xr, gr, rr = (t.reshape(-1, 128).clone() for t in (x, g, r))
+    same = lambda a, b: torch.equal(a.reshape(-1, a.shape[-1]), b)
+    assert same(mb.b200_linear(x, w, residual=r), mb.b200_linear(xr, w, residual=rr))
+    assert same(mb.b200_gated_ffn(x, w, wu), mb.b200_gated_ffn(xr, w, wu))
+    for got, want in ((mb.b200_linear_backward(g, x, w), mb.b200_linear_backward(gr, xr, w)),
+                      (mb.b200_gated_ffn_backward(g, x, w, wu), mb.b200_gated_ffn_backward(gr, xr, w, wu))):
+        for a, b in zip(got, want):
+            assert (a is None and b is None) or same(a, b)
+
+
 def test_needs_select_the_outputs():
     t = linear_case(70, 40, 24, BF, "f32", "f32", "none", seed=2, grad=BF)
     full = mb.b200_linear_backward(t["g"], t["x"], t["w"], t["bias"], "silu", t["scale"])
