@@ -372,8 +372,7 @@ MABA_API size_t maba_decode_dgda_mix_workspace_size(int32_t n_heads);
  * (float32 or x's type, any strides, 0 included); outputs have unit column stride
  * and rows that do not overlap.  Optional tensors are NULL.  Sums are float32 and
  * each result is rounded once; nothing depends on the order in which CTAs run.
- * float32 products run on the tensor cores as bf16 planes: float32's accuracy, but
- * elements below 2^-102 are off by up to 2^-125.
+ * 16-bit products run on the tensor cores, float32 ones on the CUDA cores.
  * Workspace: 256-byte aligned, of the size that the matching call reports for the
  * same tensors; one workspace serves one call at a time.
  *

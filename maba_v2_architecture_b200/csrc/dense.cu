@@ -23,6 +23,12 @@ struct Scratch {
 };
 
 
+#define DENSE_DISPATCH16(DT, ...)                                                \
+    [&]() -> int {                                                               \
+        if ((DT) == MABA_F16) { using T = __half; return __VA_ARGS__(); }        \
+        using T = __nv_bfloat16;                                                 \
+        return __VA_ARGS__();                                                    \
+    }()
 #define DENSE_DISPATCH(DT, ...)                                                  \
     [&]() -> int {                                                               \
         if ((DT) == MABA_F32) { using T = float; return __VA_ARGS__(); }         \
@@ -40,30 +46,15 @@ int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStrea
 // ---------------------------------------------------------------------------
 // small kernels
 // ---------------------------------------------------------------------------
-// x = x1 + x2 + x3: each the nearest bf16 of what the ones before left, so the three hold all
-// 24 bits of x (a finite x that would round to infinity is truncated).  An infinity or NaN is
-// x1 alone.
-__device__ __forceinline__ void split_planes(float x, __nv_bfloat16 (&v)[3]) {
-    v[0] = __float2bfloat16_rn(x), v[1] = v[2] = __float2bfloat16_rn(0.f);
-    if (isfinite(x)) {
-        if (!isfinite(__bfloat162float(v[0]))) v[0] = __float2bfloat16_rz(x);
-        const float r = x - __bfloat162float(v[0]);
-        v[1] = __float2bfloat16_rn(r);
-        v[2] = __float2bfloat16_rn(r - __bfloat162float(v[1]));
-    }
-}
-
 // Matrices made readable for the tensor-memory copies, up to four in one launch: dst [rows][ld] of
-// a 16-bit type = src (that type or float32, any strides), float32 = float32, or the three planes
-// of a float32 src (4,096 x 640 and 1,544 x 640:
-// 36 MB in and out, 13 us).  Tiles of 32 x 64; where
-// the source's columns are not contiguous they pass through shared memory, so that both sides
-// run along their contiguous axis.
+// a 16-bit type = src (that type or float32, any strides), or float32 = float32.  Tiles of 32 x 64;
+// where the source's columns are not contiguous they pass through shared memory, so that both
+// sides run along their contiguous axis.
 struct Job {
     Side src;
     int64_t rows = 0, cols = 0;
     void* dst = nullptr;
-    int64_t ld = 0, plane = 0;
+    int64_t ld = 0;
     int f32 = 0;  // a float32 copy
 };
 struct Jobs {
@@ -75,17 +66,8 @@ template <typename T> __device__ __forceinline__ void put_pair(const Job& b, int
         *reinterpret_cast<float2*>(static_cast<float*>(b.dst) + at) = make_float2(x, y);
         return;
     }
-    if constexpr (sizeof(T) == 4) {
-        __nv_bfloat16 p[3], q[3];
-        split_planes(x, p), split_planes(y, q);
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-            *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(b.dst) + e * b.plane + at) =
-                __halves2bfloat162(p[e], q[e]);
-    } else {
-        const T v[2] = {Cvt<T>::from_f(x), Cvt<T>::from_f(y)};
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(b.dst) + at) = *reinterpret_cast<const uint32_t*>(v);
-    }
+    const T v[2] = {Cvt<T>::from_f(x), Cvt<T>::from_f(y)};
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(b.dst) + at) = *reinterpret_cast<const uint32_t*>(v);
 }
 template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Jobs jobs) {
     __shared__ float tile[32][65];
@@ -190,16 +172,11 @@ __global__ void __launch_bounds__(256)
                 r[1] = g * y;
                 sb += r[0], ss += r[1];
             }
-            const bool grad = e.kind == E_GLU_BWD || e.kind == E_LINEAR_BWD;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (i == 1 && e.kind != E_GLU_BWD) break;
                 void* out = i ? e.out2 : e.out;
-                if (sizeof(T) == 4 && grad) {
-                    __nv_bfloat16 v[3];
-                    split_planes(r[i], v);
-                    for (int q = 0; q < 3; ++q) static_cast<__nv_bfloat16*>(out)[q * e.planes + at] = v[q];
-                } else if (e.out_f32) {
+                if (e.out_f32) {
                     static_cast<float*>(out)[at] = r[i];
                 } else {
                     static_cast<T*>(out)[at] = Cvt<T>::from_f(r[i]);
@@ -288,14 +265,15 @@ int run(Ctx& c, const Product& p) {
     }
     // a plain product whose tiles do not fill the GPU splits its contraction; the partial
     // sums are float32 and added in split order
-    const Plan plan = c.dry ? (c.plans[c.n_plans++] = tc_plan(p, c.dt)) : c.plans[c.next_plan++];
+    const Plan plan = c.dry ? (c.plans[c.n_plans++] = c.dt == MABA_F32 ? simt_plan(p) : tc_plan(p)) : c.plans[c.next_plan++];
     const Product sums = plan.finish ? split_sums(p) : p;
     const int64_t rows = sums.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
     float* partial = plan.splits > 1 ? static_cast<float*>(c.ws.take((size_t)plan.splits * rows * ldp * 4)) : nullptr;
     if (c.dry) return MABA_OK;
+    if (c.dt == MABA_F32) MABA_TRY(simt_product(sums, plan.splits, partial, ldp, c.s));
+    else MABA_TRY(DENSE_DISPATCH16(c.dt, [&] { return tc_product<T>(sums, plan, partial, ldp, c.s); }));
+    if (plan.splits == 1) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        MABA_TRY(tc_product<T>(sums, plan, partial, ldp, c.s));
-        if (plan.splits == 1) return (int)MABA_OK;
         const int64_t cap = 32768;
         if (plan.finish) {
             const int64_t gy = ceil_div(p.M, 32);
@@ -323,7 +301,7 @@ int prepare(Ctx& c) {
     const Jobs jobs = c.jobs;
     c.jobs.n = 0;
     if (c.dry) return MABA_OK;
-    return DENSE_DISPATCH(c.dt, [&] {
+    return DENSE_DISPATCH16(c.dt, [&] {
         return launch(prepare_kernel<T>, grid, dim3(256), 0, c.s, jobs);
     });
 }
@@ -412,37 +390,37 @@ Side side1(const maba_tensor* t) { return given(t) ? Side{t->data, 0, t->stride[
 // ---------------------------------------------------------------------------
 // A matrix as an operand.  The tensor-memory loads of the 16-bit products want rows on
 // 16-byte boundaries; what is not laid out so is copied once per call (noted here, launched by
-// prepare()), and a float32 matrix is split into its planes.  One copy serves both directions
-// of a matrix: K-major along its rows, MN-major across them.
+// prepare()).  One copy serves both directions of a matrix: K-major along its rows, MN-major
+// across them.  The float32 products read the caller's matrix.
 void operand(Ctx& c, const maba_tensor* t, Matrix& m, bool as_is = false) {
     const Side src = side2(t);
     const int64_t rows = t->shape[0], cols = t->shape[1];
-    m = Matrix{src.p, src.sr, src.sc, 0};
-    if (as_is || (!src.f32 && tc_readable(src.p, rows, cols, src.sr, src.sc))) return;
-    const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
-    void* to = c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2);
-    m = Matrix{to, ld, 1, plane};
-    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, plane, 0};
+    m = Matrix{src.p, src.sr, src.sc};
+    if (as_is || c.dt == MABA_F32 || (!src.f32 && tc_readable(src.p, rows, cols, src.sr, src.sc))) return;
+    const int64_t ld = (cols + 7) / 8 * 8;
+    void* to = c.ws.take((size_t)rows * ld * 2);
+    m = Matrix{to, ld, 1};
+    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, 0};
 }
 // A matrix that an epilogue of the tensor-core products reads: copied where its rows are not on
 // 16-byte boundaries (a broadcast one too).
 Side side_of(Ctx& c, const maba_tensor* t, bool as_is = false) {
     const Side src = side2(t);
-    if (!given(t) || as_is) return src;
+    if (!given(t) || as_is || c.dt == MABA_F32) return src;
     const int64_t rows = t->shape[0], cols = t->shape[1], per = src.f32 ? 4 : 8;
     if (src.sc == 1 && (rows == 1 || (src.sr % per == 0 && src.sr >= cols)) && (reinterpret_cast<uintptr_t>(src.p) & 15u) == 0)
         return src;
     const int64_t ld = (cols + 7) / 8 * 8;
     void* to = c.ws.take((size_t)rows * ld * (src.f32 ? 4 : 2));
-    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, 0, src.f32};
+    c.jobs.j[c.jobs.n++] = Job{src, rows, cols, to, ld, src.f32};
     return Side{to, ld, 1, src.f32};
 }
 // A gradient that an epilogue writes as an operand of the next products.
 Matrix written_operand(Ctx& c, int64_t rows, int64_t cols) {
-    const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
-    return Matrix{c.ws.take((size_t)(c.dt == MABA_F32 ? 3 : 1) * plane * 2), ld, 1, plane};
+    const int64_t ld = (cols + 7) / 8 * 8;
+    return Matrix{c.ws.take((size_t)rows * ld * (c.dt == MABA_F32 ? 4 : 2)), ld, 1};
 }
-Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr, m.sp}; }
+Matrix transposed(const Matrix& m) { return Matrix{m.p, m.sk, m.sr}; }
 
 struct LinearArgs {
     const maba_tensor *x, *w, *bias, *scale, *res, *out;              // forward
@@ -508,7 +486,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
     }
     if (!need_dx && !need_dw && !need_db && !need_ds) return MABA_OK;
     const bool through = a.act == ACT_NONE && !given(a.scale);  // dz = g
-    const int64_t blocks = ceil_div(M, through ? CS_ROWS : TC_ROWS);
+    const int64_t blocks = ceil_div(M, through ? CS_ROWS : (c.dt == MABA_F32 ? SIMT_ROWS : TC_ROWS));
     float* pb = need_db ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     float* ps = need_ds ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     Matrix x, w, d;
@@ -529,7 +507,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
         p.e.kind = E_LINEAR_BWD;
         p.e.act = a.act;
         p.e.bias = side1(a.bias), p.e.scale = side1(a.scale), p.e.res = g;
-        p.e.out = const_cast<void*>(d.p), p.e.ldo = d.sr, p.e.planes = d.sp;
+        p.e.out = const_cast<void*>(d.p), p.e.ldo = d.sr;
         p.e.part_bias = pb, p.e.part_scale = ps;
         p.e.sums_f32 = (need_db && a.dbias->dtype == MABA_F32) || (need_ds && a.dscale->dtype == MABA_F32);
         MABA_TRY(run(c, p));
@@ -582,7 +560,7 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
     // the one rounding between the two passes
     const Matrix d[2] = {written_operand(c, M, p.N), written_operand(c, M, p.N)};
-    p.e.out = const_cast<void*>(d[0].p), p.e.out2 = const_cast<void*>(d[1].p), p.e.ldo = d[0].sr, p.e.planes = d[0].sp;
+    p.e.out = const_cast<void*>(d[0].p), p.e.out2 = const_cast<void*>(d[1].p), p.e.ldo = d[0].sr;
     MABA_TRY(run(c, p));
     if (given(a.dx)) MABA_TRY(dx_product(c, M, p.N, 2, d, p.b, a.dx));
     const maba_tensor* dw[2] = {a.dwg, a.dwu};

@@ -32,13 +32,10 @@ enum EpiKind {
     E_STORE = 4,       // out = z, or float32 partial sums [split][M (2 M of F_PAIR)][N]
 };
 
-// An operand of a Product: 16-bit elements, or a float32 matrix as three bf16 planes
-// x = x1 + x2 + x3 (dense_tc.cu) that lie sp elements apart.  The few-row kernels read the
-// caller's float32 matrix itself.
+// An operand of a Product, of the operands' type.
 struct Matrix {
     const void* p = nullptr;
     int64_t sr = 0, sk = 0;  // element strides along the rows and along the contraction
-    int64_t sp = 0;
 };
 
 // A vector or a matrix that an epilogue reads: float32 or the operands' type, any strides.
@@ -53,7 +50,6 @@ struct Epilogue {
     void* out = nullptr;   // row-major, unit column stride
     void* out2 = nullptr;  // laid out like out: du of E_GLU_BWD, C1 of F_PAIR
     int64_t ldo = 0;
-    int64_t planes = 0;    // float32, E_LINEAR_BWD and E_GLU_BWD: out (out2) receives bf16 planes, this far apart
     Side bias, scale, res;
     float* part_bias = nullptr;   // E_LINEAR_BWD: [row blocks][N] column sums of dz
     float* part_scale = nullptr;  // and of g * act(z + bias)
@@ -106,8 +102,8 @@ template <typename T> __device__ __forceinline__ float side_at(const Side& s, in
 bool skinny_takes(const Product& p, int dt);
 template <typename T> int skinny_product(const Product& p, cudaStream_t s);
 
-// dense_tc.cu: tensor cores.  Operands as tc_readable() accepts them (float32: as planes);
-// column sums per TC_ROWS rows; T is the type of what the epilogue reads and writes.
+// dense_tc.cu: 16-bit operands on the tensor cores, laid out as tc_readable() accepts them;
+// column sums per TC_ROWS rows; T is their type.
 constexpr int TC_ROWS = 32;
 struct Plan {
     int cg = 1, bn = 32;  // CTAs per tile, columns of the MMA
@@ -115,11 +111,16 @@ struct Plan {
     bool finish = false;  // the splits' sums get the epilogue in a kernel of its own (split_sums)
 };
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
-Plan tc_plan(const Product& p, int dt);
+Plan tc_plan(const Product& p);
 Product split_sums(const Product& p);  // the same sums as a plain product, two for F_DUAL
 template <typename T>
 int tc_product(const Product& p, const Plan& plan, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);
+
+// dense_simt.cu: float32 operands, any strides; column sums per SIMT_ROWS rows.
+constexpr int SIMT_ROWS = 128;
+Plan simt_plan(const Product& p);
+int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s);
 
 }  // namespace dense
 }  // namespace maba

@@ -1,0 +1,238 @@
+// Float32 products on the CUDA cores: any strides, float32 sums.
+//
+// A CTA computes a 128 x 128 tile of C (of a pair of projections 128 x 64 of each: the tile's
+// columns 0..63 belong to B0, 64..127 to B1) over its share of the contraction, 16 indices at a
+// time.  Both operand tiles lie contraction-major in two shared-memory buffers; the next tile is
+// on its way into registers under the current one's arithmetic.  A thread owns rows and columns
+// {4 t, 64 + 4 t} + 0..3, so gate and up of a pair sit in one thread, and multiplies two columns
+// by one instruction (fma.f32x2).  What bounds it is the rate of float32 multiply-adds.
+#include "dense.cuh"
+
+namespace maba {
+namespace dense {
+namespace {
+
+constexpr int BM = SIMT_ROWS, BN = 128, BK = 16, LD = BM + 4, NTHR = 256;
+
+__device__ __forceinline__ unsigned long long both(float a) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(a));
+    return r;
+}
+__device__ __forceinline__ void fma_pair(unsigned long long& c, unsigned long long a, unsigned long long b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+
+// One operand's 128 x 16 tile: half i (64 rows) is this thread's piece i, four elements along the
+// contraction (KFAST) or along the rows, whichever is the shorter stride.  A piece that is whole,
+// contiguous and on 16 bytes is one load; elements out of range are 0.
+struct Half {
+    const float* p;
+    int64_t sr, sk;
+    bool kfast, vec;
+};
+__device__ __forceinline__ Half half_of(const Matrix& m) {
+    Half h{static_cast<const float*>(m.p), m.sr, m.sk, m.sk <= m.sr, false};
+    h.vec = (h.kfast ? h.sk == 1 && (h.sr & 3) == 0 : h.sr == 1 && (h.sk & 3) == 0) &&
+            (reinterpret_cast<uintptr_t>(m.p) & 15u) == 0;
+    return h;
+}
+__device__ __forceinline__ float4 load_piece(const Half& h, int64_t r0, int64_t rows, int64_t k0, int64_t K, int tid) {
+    const int64_t r = r0 + (h.kfast ? tid >> 2 : (tid & 15) * 4), k = k0 + (h.kfast ? (tid & 3) * 4 : tid >> 4);
+    const int64_t n = h.kfast ? K - k : rows - r;  // elements left along the piece
+    const bool in = h.kfast ? r < rows : k < K;
+    const float* p = h.p + r * h.sr + k * h.sk;
+    if (in && h.vec && n >= 4) return *reinterpret_cast<const float4*>(p);
+    const int64_t step = h.kfast ? h.sk : h.sr;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = in && j < n ? p[j * step] : 0.f;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_piece(const float4& v, bool kfast, float* s, int half, int tid) {
+    if (kfast) {
+        float* t = s + (tid & 3) * 4 * LD + half * 64 + (tid >> 2);
+        t[0] = v.x, t[LD] = v.y, t[2 * LD] = v.z, t[3 * LD] = v.w;
+    } else {
+        *reinterpret_cast<float4*>(s + (tid >> 4) * LD + half * 64 + (tid & 15) * 4) = v;
+    }
+}
+// four results of a row: one store where they are whole and on 16 bytes
+__device__ __forceinline__ void put4(float* p, const float* v, int64_t n) {
+    if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) p[j] = v[j];
+    }
+}
+
+template <bool DUAL>
+__global__ void __launch_bounds__(NTHR, 2)
+    simt_kernel(const Product p, int tiles_n, int splits, float* partial, int64_t ldp) {
+    __shared__ __align__(16) float As[2][BK * LD], Bs[2][BK * LD];
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int64_t tm = blockIdx.x / tiles_n, m0 = tm * BM, n0 = (int64_t)(blockIdx.x % tiles_n) * (DUAL ? 64 : BN);
+    const int pair = p.form == F_PAIR ? blockIdx.z : 0;
+    const int64_t nk = (p.K + BK - 1) / BK, total = nk * (p.form == F_SUM ? 2 : 1);
+    const int64_t k_lo = total * blockIdx.y / splits, k_hi = total * (blockIdx.y + 1) / splits;
+
+    float4 ra[2], rb[2];
+    auto halves = [&](int64_t it, Half& a, Half& b0, Half& b1) {
+        const int sg = it >= nk ? 1 : 0;
+        a = half_of(p.a[p.form == F_PAIR ? pair : sg]);
+        b0 = half_of(p.b[p.form == F_PAIR ? pair : sg]);
+        b1 = DUAL ? half_of(p.b[1]) : b0;
+        return (it - sg * nk) * BK;
+    };
+    auto load = [&](int64_t it) {
+        Half a, b0, b1;
+        const int64_t k0 = halves(it, a, b0, b1);
+        ra[0] = load_piece(a, m0, p.M, k0, p.K, tid);
+        ra[1] = load_piece(a, m0 + 64, p.M, k0, p.K, tid);
+        rb[0] = load_piece(b0, n0, p.N, k0, p.K, tid);
+        rb[1] = load_piece(b1, DUAL ? n0 : n0 + 64, p.N, k0, p.K, tid);
+    };
+    auto store = [&](int64_t it, int buf) {
+        Half a, b0, b1;
+        halves(it, a, b0, b1);
+        store_piece(ra[0], a.kfast, As[buf], 0, tid), store_piece(ra[1], a.kfast, As[buf], 1, tid);
+        store_piece(rb[0], b0.kfast, Bs[buf], 0, tid), store_piece(rb[1], b1.kfast, Bs[buf], 1, tid);
+    };
+    unsigned long long acc[8][4] = {};
+    if (k_lo < k_hi) {
+        load(k_lo);
+        store(k_lo, 0);
+    }
+    __syncthreads();
+    for (int64_t it = k_lo; it < k_hi; ++it) {
+        const int buf = (int)(it - k_lo) & 1;
+        if (it + 1 < k_hi) load(it + 1);
+#pragma unroll
+        for (int k = 0; k < BK; ++k) {
+            float a[8];
+            *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(&As[buf][k * LD + ty * 4]);
+            *reinterpret_cast<float4*>(a + 4) = *reinterpret_cast<const float4*>(&As[buf][k * LD + 64 + ty * 4]);
+            const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(&Bs[buf][k * LD + tx * 4]);
+            const ulonglong2 b1 = *reinterpret_cast<const ulonglong2*>(&Bs[buf][k * LD + 64 + tx * 4]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned long long x = both(a[i]);
+                fma_pair(acc[i][0], x, b0.x), fma_pair(acc[i][1], x, b0.y);
+                fma_pair(acc[i][2], x, b1.x), fma_pair(acc[i][3], x, b1.y);
+            }
+        }
+        if (it + 1 < k_hi) store(it + 1, buf ^ 1);  // (its last readers passed the barrier before this step)
+        __syncthreads();
+    }
+
+    const Epilogue& e = p.e;
+    const int64_t rows_out = p.form == F_PAIR ? 2 * p.M : p.M;
+    float sum_b[8] = {}, sum_s[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
+        if (m >= p.M) continue;
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 v = *reinterpret_cast<const float2*>(&acc[i][j]);
+            z[2 * j] = v.x, z[2 * j + 1] = v.y;
+        }
+        if (DUAL) {
+            const int64_t n = n0 + tx * 4;
+            if (n >= p.N) continue;
+            float first[4], second[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (e.kind == E_GLU) {
+                    first[j] = act_f(z[j], e.act) * z[j + 4];
+                } else {
+                    const float g = n + j < p.N ? side_at<float>(e.res, m, n + j) : 0.f;
+                    float y, d;
+                    act_grad_f(z[j], e.act, y, d);
+                    first[j] = g * z[j + 4] * d, second[j] = g * y;
+                }
+            }
+            put4(static_cast<float*>(e.out) + m * e.ldo + n, first, p.N - n);
+            if (e.kind == E_GLU_BWD) put4(static_cast<float*>(e.out2) + m * e.ldo + n, second, p.N - n);
+            continue;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t n = n0 + h * 64 + tx * 4;
+            if (n >= p.N) continue;
+            float* v = z + 4 * h;
+            if (e.kind != E_STORE) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (n + j >= p.N) continue;
+                    if (e.bias.p) v[j] += side_at<float>(e.bias, 0, n + j);
+                    const float s = e.scale.p ? side_at<float>(e.scale, 0, n + j) : 1.f;
+                    const float g = e.res.p ? side_at<float>(e.res, m, n + j) : 0.f;
+                    if (e.kind == E_LINEAR) {
+                        v[j] = act_f(v[j], e.act);
+                        if (e.scale.p) v[j] *= s;
+                        if (e.res.p) v[j] += g;
+                    } else {
+                        float y, d;
+                        act_grad_f(v[j], e.act, y, d);
+                        v[j] = g * d;
+                        if (e.scale.p) v[j] *= s;
+                        sum_b[4 * h + j] += v[j], sum_s[4 * h + j] += g * y;
+                    }
+                }
+            }
+            float* out = splits > 1 ? partial + ((int64_t)blockIdx.y * rows_out + m + pair * p.M) * ldp
+                                    : static_cast<float*>(pair ? e.out2 : e.out) + m * e.ldo;
+            put4(out + n, v, p.N - n);
+        }
+    }
+    if (e.kind != E_LINEAR_BWD || !(e.part_bias || e.part_scale)) return;
+    // column sums of the tile: thread rows first, then the 16 of them, in order
+    float* red = As[0];  // [16][128], free after the last barrier
+    for (int which = 0; which < 2; ++which) {
+        float* dst = which ? e.part_scale : e.part_bias;
+        if (!dst) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) red[ty * 128 + (j >> 2) * 64 + tx * 4 + (j & 3)] = which ? sum_s[j] : sum_b[j];
+        __syncthreads();
+        if (tid < 128 && n0 + tid < p.N) {
+            float s = 0.f;
+            for (int q = 0; q < 16; ++q) s += red[q * 128 + tid];
+            dst[tm * p.N + n0 + tid] = s;
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+// A plain product whose tiles do not fill the GPU (two CTAs on each SM) splits its contraction,
+// into parts of at least 128 indices; so does an epilogue's with few tiles and a long one, and
+// the epilogue follows.  (Not with column sums: those are the tiles'.)
+Plan simt_plan(const Product& p) {
+    Plan plan;
+    const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, p.form == F_DUAL ? 64 : BN) * (p.form == F_PAIR ? 2 : 1);
+    const int64_t k = p.K * (p.form == F_SUM ? 2 : 1), slots = 2 * (int64_t)sm_count();
+    if (p.e.kind != E_STORE && (p.e.kind == E_LINEAR_BWD || p.K < 1024 || 4 * tiles > slots)) return plan;
+    int64_t n = slots / tiles;
+    if (n > k / 128) n = k / 128;
+    if (n > 16) n = 16;
+    plan.splits = n > 1 ? (int)n : 1;
+    plan.finish = p.e.kind != E_STORE && plan.splits > 1;
+    return plan;
+}
+
+int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s) {
+    const int64_t tn = ceil_div(p.N, p.form == F_DUAL ? 64 : BN), tm = ceil_div(p.M, BM);
+    if (tm * tn > 0x7fffffff) return set_error(MABA_ERR_UNSUPPORTED, "dense: %lld tiles", (long long)(tm * tn));
+    const dim3 grid((unsigned)(tm * tn), (unsigned)splits, p.form == F_PAIR ? 2 : 1);
+    if (p.form == F_DUAL) simt_kernel<true><<<grid, NTHR, 0, s>>>(p, (int)tn, splits, partial, ldp);
+    else simt_kernel<false><<<grid, NTHR, 0, s>>>(p, (int)tn, splits, partial, ldp);
+    return check_launch("dense(simt)");
+}
+
+}  // namespace dense
+}  // namespace maba

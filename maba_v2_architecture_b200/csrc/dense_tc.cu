@@ -1,19 +1,10 @@
-// Products on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
-//
-// 16-bit operands are multiplied as they are.  A float32 operand is three bf16 planes,
-// x = x1 + x2 + x3 exactly, |x2| <= 2^-8 |x|, |x3| <= 2^-16 |x|; of the nine products the
-// six down to 2^-16 are taken, x1 w1 into one accumulator, x1 w2 + x2 w1 + x2 w2 + x1 w3 +
-// x3 w1 into a second, and what is left out is below 2^-23 of |x w|: float32's own rounding,
-// at six tensor products instead of the CUDA cores' one (where main is an infinity or NaN the
-// second sum, which may hold inf * 0, is not added).  The tensor cores take a bf16 below
-// 2^-126 for zero, so an x below 2^-102 is off by up to 2^-125.  4,096 x 640 -> 1544: 48 us,
-// 1.0 PFLOP/s of bf16 products, 170 TFLOP/s of float32; a CUDA-core kernel took 346 us.
+// Products of 16-bit operands on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
 // The tensor cores truncate when they add to their float32 accumulator, once per 16
 // contraction indices: a sum over K loses about K 5.6e-10 of itself toward zero (measured
 // 6e-7 relative at K = 640, 4.4e-6 at 4,096).  That is far below a 16-bit result's rounding,
-// but not below a float32 result's, so sums that end in float32 (MODE 1 and 2) leave TMEM
-// every 640 (320) indices and are added, rounded to nearest, in the epilogue's registers.
+// but not below a float32 result's, so sums that end in float32 (MODE 1) leave TMEM every
+// 640 indices and are added, rounded to nearest, in the epilogue's registers.
 //
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
@@ -75,7 +66,7 @@ constexpr uint32_t A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8;
 constexpr uint32_t BAR_BYTES = 512;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
-constexpr int TMEM_COLS = 512, ACC_COLS = 256, MINOR = 128;  // MINOR: the second accumulator of float32 products
+constexpr int TMEM_COLS = 512, ACC_COLS = 256;
 
 enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_TFULL = 2 * MAX_STAGES, B_TEMPTY = B_TFULL + 2, B_DRAIN = B_TEMPTY + 2,
        B_SFULL = B_DRAIN + 1, B_SEMPTY = B_SFULL + 8, N_BARS = B_SEMPTY + 8 };  // [group][slot]
@@ -89,7 +80,7 @@ struct TcArgs {
     int bn, b_rows;  // columns of the MMA, rows of B per CTA
     int flush;       // contraction blocks between two readings of the accumulator
     int stages;
-    uint32_t stage_bytes, b_at, b_bytes, load_bytes;  // B's place in a stage, one plane of it, bytes per stage
+    uint32_t stage_bytes, load_bytes;  // of shared memory, and of the copies (of both CTAs)
     uint32_t idesc;
     int out_tma;                         // the results leave by copies
     int in_place;                        // from the buffer that brought the residual or gradient
@@ -157,9 +148,9 @@ __device__ __forceinline__ void sigmoid2(float z0, float z1, float& s0, float& s
     add2(s0, s1, 1.f, 1.f);
     s0 = rcp_sfu(s0), s1 = rcp_sfu(s1);
 }
-// phi and phi' of a pair; of float32 operands (EXACT) as dense.cuh has them.
-template <int ACT, bool EXACT> __device__ __forceinline__ void act2(float& z0, float& z1) {
-    if (ACT == ACT_SILU && !EXACT) {
+// phi and phi' of a pair.
+template <int ACT> __device__ __forceinline__ void act2(float& z0, float& z1) {
+    if (ACT == ACT_SILU) {
         float s0, s1;
         sigmoid2(z0, z1, s0, s1);
         mul2(z0, z1, s0, s1);
@@ -167,9 +158,9 @@ template <int ACT, bool EXACT> __device__ __forceinline__ void act2(float& z0, f
         z0 = act_f(z0, ACT), z1 = act_f(z1, ACT);
     }
 }
-template <int ACT, bool EXACT>
+template <int ACT>
 __device__ __forceinline__ void act_grad2(float z0, float z1, float& y0, float& y1, float& d0, float& d1) {
-    if (ACT == ACT_SILU && !EXACT) {
+    if (ACT == ACT_SILU) {
         float s0, s1;
         sigmoid2(z0, z1, s0, s1);
         y0 = z0, y1 = z1;
@@ -224,7 +215,7 @@ __device__ __forceinline__ int frag_col(int j, int lane) { return ((j >> 2) & 3)
 // f(j, value, next value) for the 32 elements of a staged chunk, in pairs
 template <typename T, bool FRAG, typename F>
 __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane, F f) {
-    if (sizeof(T) == 4 || f32) {
+    if (f32) {
         if (FRAG) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -238,7 +229,7 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
                 f(4 * i, x.x, x.y), f(4 * i + 2, x.z, x.w);
             }
         }
-    } else if constexpr (sizeof(T) == 2) {
+    } else {
         if (FRAG) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -260,22 +251,8 @@ __device__ __forceinline__ void with_chunk(bool f32, unsigned char* st, int lane
         }
     }
 }
-// The next of a float32 value's three bf16 planes (dense.cu's split_planes); what it leaves
-// stays in z.
-__device__ __forceinline__ float next_plane(float& z) {
-    float v = __bfloat162float(__float2bfloat16_rn(z));
-    if (!isfinite(v)) {
-        if (!isfinite(z)) {  // the first plane alone
-            v = z, z = 0.f;
-            return v;
-        }
-        v = __bfloat162float(__float2bfloat16_rz(z));
-    }
-    z -= v;
-    return v;
-}
 template <typename T, bool FRAG> __device__ __forceinline__ void put_chunk(const float* z, bool f32, unsigned char* st, int lane) {
-    if (sizeof(T) == 4 || f32) {
+    if (f32) {
         if (FRAG) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2)
@@ -285,7 +262,7 @@ template <typename T, bool FRAG> __device__ __forceinline__ void put_chunk(const
             for (int i = 0; i < 8; ++i)
                 *reinterpret_cast<float4*>(at32(st, lane, i)) = make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
         }
-    } else if constexpr (sizeof(T) == 2) {
+    } else {
         if (FRAG) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2)
@@ -352,7 +329,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* abort_f = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    constexpr int PLANES = MODE == 2 ? 3 : 1;
     constexpr int EPI_WARPS = Warps<MODE>::EPI, W_TMA = Warps<MODE>::TMA, W_MMA = Warps<MODE>::MMA;
     constexpr int W_SIDE = Warps<MODE>::SIDE, GROUPS = Warps<MODE>::GROUPS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -432,34 +408,33 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 {
                     uint64_t* full = &bars[B_FULL + st];
                     const uint32_t full0 = CG == 2 ? cluster_addr(full, 0) : 0u;
-                    auto load = [&](unsigned char* dst, const CUtensorMap* m, int x, int y, int plane) {
-                        if (CG == 2) tma_load_3d_pair(dst, m, full0, x, y, plane);
-                        else tma_load_3d(dst, m, full, x, y, plane);
+                    auto load = [&](unsigned char* dst, const CUtensorMap* m, int x, int y) {
+                        if (CG == 2) tma_load_3d_pair(dst, m, full0, x, y, 0);
+                        else tma_load_3d(dst, m, full, x, y, 0);
                     };
                     if (rank == 0) mbar_arrive_expect_tx(full, a.load_bytes);
-#pragma unroll
-                    for (int pl = 0; pl < PLANES; ++pl, sa += A_BYTES) {
-                        unsigned char* sb = base + st * a.stage_bytes + a.b_at + pl * a.b_bytes;
+                    {
+                        unsigned char* sb = sa + A_BYTES;
                         if (A_MN) {
-                            load(sa, ma, m0, k0, pl);
-                            load(sa + A_BYTES / 2, ma, m0 + 64, k0, pl);
+                            load(sa, ma, m0, k0);
+                            load(sa + A_BYTES / 2, ma, m0 + 64, k0);
                         } else {
-                            load(sa, ma, k0, m0, pl);
+                            load(sa, ma, k0, m0);
                         }
                         if (KIND == E_GLU || KIND == E_GLU_BWD) {
                             if (CG == 2) {
-                                load(sb, rank ? &tb1 : &tb0, k0, n0, pl);
+                                load(sb, rank ? &tb1 : &tb0, k0, n0);
                             } else {
-                                load(sb, &tb0, k0, n0, pl);
-                                load(sb + a.bn / 2 * 128, &tb1, k0, n0, pl);
+                                load(sb, &tb0, k0, n0);
+                                load(sb + a.bn / 2 * 128, &tb1, k0, n0);
                             }
                         } else {
                             const CUtensorMap* mb = (a.pairs == 2 ? pair : seg) ? &tb1 : &tb0;
                             const int y = n0 + (int)rank * a.b_rows;
                             if (B_MN) {
-                                for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0, pl);
+                                for (int i = 0; i < a.b_rows; i += 64) load(sb + i * 128, mb, y + i, k0);
                             } else {
-                                load(sb, mb, k0, y, pl);
+                                load(sb, mb, k0, y);
                             }
                         }
                     }
@@ -479,7 +454,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         // ============================ MMA issuer ==============================
         if (rank == 0 && elect_one()) {
             const uint64_t ad0 = sdesc_sw128(smem_addr(base), A_MN ? A_BYTES / 2 : 16, 1024);
-            const uint64_t bd0 = sdesc_sw128(smem_addr(base + a.b_at), B_MN ? 8192 : 16, 1024);
+            const uint64_t bd0 = sdesc_sw128(smem_addr(base + A_BYTES), B_MN ? 8192 : 16, 1024);
             constexpr uint32_t ak = A_MN ? 2048 >> 4 : 32 >> 4, bk = B_MN ? 2048 >> 4 : 32 >> 4;
             auto mma = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t acc) {
                 if (CG == 2) umma_f16_ss_pair(d, ad, bd, a.idesc, acc);
@@ -506,19 +481,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                         tc_fence_after();
                         const uint64_t so = (uint64_t)(st * (a.stage_bytes >> 4));
                         const uint64_t ad = ad0 + so, bd = bd0 + so;
-                        const uint64_t bp = a.b_bytes >> 4;  // from one plane of B to the next
-                        constexpr uint64_t ap = A_BYTES >> 4;
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k) {
                             const uint32_t acc = kb > f0 || k > 0 ? 1u : 0u;
                             mma(d, ad + k * ak, bd + k * bk, acc);
-                            if (PLANES == 3) {
-                                mma(d + MINOR, ad + k * ak, bd + k * bk + 2 * bp, acc);
-                                mma(d + MINOR, ad + k * ak + 2 * ap, bd + k * bk, 1u);
-                                mma(d + MINOR, ad + k * ak + ap, bd + k * bk + bp, 1u);
-                                mma(d + MINOR, ad + k * ak, bd + k * bk + bp, 1u);
-                                mma(d + MINOR, ad + k * ak + ap, bd + k * bk, 1u);
-                            }
                         }
                         commit(&bars[B_EMPTY + st]);
                         if (++st == a.stages) st = 0, phase ^= 1;
@@ -573,11 +539,11 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Warps<MODE>::REG_EPI));
         // ============================== epilogue ==============================
-        constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD, EXACT = MODE == 2;
+        constexpr bool DUAL = KIND == E_GLU || KIND == E_GLU_BWD;
         constexpr bool FRAG = KIND == E_LINEAR_BWD, VECS = KIND == E_LINEAR || KIND == E_LINEAR_BWD;
         constexpr bool SIDE = KIND != E_STORE && KIND != E_GLU;
-        // MODE 1, 2: chunks (of a pair of projections: one) whose sums a warp holds
-        constexpr int CH = MODE == 0 || DUAL ? 1 : (MODE == 1 ? 4 : 2);
+        constexpr int CH = MODE == 0 ? 1 : 4;  // MODE 1: chunks whose sums a warp holds
+        static_assert(MODE == 0 || VECS, "the linear map's kinds alone");
         constexpr int CS = GROUPS, NV = Warps<MODE>::CHUNKS;
         const int q = warp & 3, h = warp >> 2;
         unsigned char* in_buf = staging + (h * a.n_in * 4 + q) * a.in_bytes;  // slots 4 in_bytes apart
@@ -587,11 +553,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         const Epilogue& e = a.e;
         const int width = DUAL ? a.bn / 2 : a.bn;
         const bool has_side = SIDE && e.res.p != nullptr;
-        const bool side_f32 = sizeof(T) == 4 || e.res.f32;
-        // (the gradients of float32 operands leave as planes)
-        constexpr bool TO_PLANES = MODE == 2 && (KIND == E_LINEAR_BWD || KIND == E_GLU_BWD);
-        const bool out_f32 = !TO_PLANES && (sizeof(T) == 4 || e.out_f32 || (KIND == E_STORE && a.splits > 1));
-        using OT = typename std::conditional<TO_PLANES, __nv_bfloat16, T>::type;
+        const bool side_f32 = e.res.f32;
+        const bool out_f32 = e.out_f32 || (KIND == E_STORE && a.splits > 1);
         struct Chunk {
             int row0, col0, rows, cols;  // rows, cols: of 32, inside the matrix
         };
@@ -641,7 +604,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 }
                 __syncwarp();
             }
-            put_chunk<OT, FRAG>(z, out_f32, buf, lane);
+            put_chunk<T, FRAG>(z, out_f32, buf, lane);
             if (a.out_tma) {
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -661,11 +624,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         uint32_t ps[NV], pb[NV];
         auto bits_at = [&](const Side& v, int col) {
             const int64_t i = col * v.sc;
-            return sizeof(T) == 4 || v.f32 ? static_cast<const uint32_t*>(v.p)[i] : (uint32_t)static_cast<const uint16_t*>(v.p)[i];
+            return v.f32 ? static_cast<const uint32_t*>(v.p)[i] : (uint32_t)static_cast<const uint16_t*>(v.p)[i];
         };
         auto value_of = [&](const Side& v, uint32_t bits) {
-            if constexpr (sizeof(T) == 2)
-                if (!v.f32) return unpack2<T>(bits).x;
+            if (!v.f32) return unpack2<T>(bits).x;
             return __uint_as_float(bits);
         };
         auto fetch_vectors = [&](const Unit& t) {
@@ -716,7 +678,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 if (e.bias.p) with_vector<FRAG>(z, vb, lane, add2);
                 with_act(e.act, [&](auto A) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) act2<A.value, EXACT>(z[j], z[j + 1]);
+                    for (int j = 0; j < 32; j += 2) act2<A.value>(z[j], z[j + 1]);
                 });
                 if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
                 if (has_side) {
@@ -731,7 +693,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 with_act(e.act, [&](auto A) {
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
                         float y0, y1, d0, d1;
-                        act_grad2<A.value, EXACT>(z[j], z[j + 1], y0, y1, d0, d1);
+                        act_grad2<A.value>(z[j], z[j + 1], y0, y1, d0, d1);
                         if (k.rows < 32 && frag_row(j, lane) >= k.rows) y0 = y1 = d0 = d1 = 0.f;  // whatever the bias is
                         const int c = ((j >> 2) & 3) * 2;
                         z[j] = g0, z[j + 1] = g1;
@@ -758,7 +720,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 with_act(e.act, [&](auto A) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        act2<A.value, EXACT>(z[j], z[j + 1]);
+                        act2<A.value>(z[j], z[j + 1]);
                         mul2(z[j], z[j + 1], w[j], w[j + 1]);
                     }
                 });
@@ -767,7 +729,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 with_act(e.act, [&](auto A) {
                     with_chunk<T, FRAG>(side_f32, in, lane, [&](int j, float g0, float g1) {
                         float y0, y1, d0, d1;
-                        act_grad2<A.value, EXACT>(z[j], z[j + 1], y0, y1, d0, d1);
+                        act_grad2<A.value>(z[j], z[j + 1], y0, y1, d0, d1);
                         mul2(d0, d1, w[j], w[j + 1]);
                         w[j] = g0, w[j + 1] = g1;
                         z[j] = g0, z[j + 1] = g1;
@@ -776,16 +738,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                     });
                 });
                 side_used(false);
-            }
-            if (TO_PLANES) {
-#pragma unroll
-                for (int pl = 0; pl < (KIND == E_GLU_BWD ? 6 : 3); ++pl) {
-                    float v[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = next_plane(pl < 3 ? z[j] : w[j]);
-                    store(k, v, pl < 3 ? &tout : &tout2, nullptr, e.ldo, pl % 3, nullptr);
-                }
-                return;
             }
             if (KIND == E_STORE && a.splits > 1) {
                 const int part = t.split(a) * a.pairs + t.pair(a);
@@ -813,44 +765,31 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 if (after.u < a.units) fetch_vectors(after);
             }
             if constexpr (MODE != 0) {
-                float sz[CH][32], sw[DUAL ? 32 : 1];  // the unit's accumulations, added up
+                float sz[CH][32], none[1];  // the unit's accumulations, added up
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = 0; j < 32; ++j)
 #pragma unroll
                     for (int cc = 0; cc < CH; ++cc) sz[cc][j] = 0.f;
-                    if (DUAL) sw[j] = 0.f;
-                }
                 const int kb1 = t.kb1(a);
                 for (int f0 = t.kb0(a); f0 < kb1; f0 += a.flush) {
                     if (!wait_full()) break;
                     const uint32_t acc = tmem + buf * ACC_COLS + ((uint32_t)(q * 32) << 16);
-                    auto add = [&](float* sum, int col) {
+#pragma unroll
+                    for (int cc = 0; cc < CH; ++cc) {
+                        if ((h + CS * cc) * 32 >= width) continue;
                         float z[32];
-                        load_sums(z, acc + col);
-                        if (MODE == 2) {
-                            float y[32];
-                            load_sums(y, acc + MINOR + col);
-                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
-                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(y));
+                        load_sums(z, acc + (h + CS * cc) * 32);
+                        tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[j] += isfinite(z[j]) ? z[j] + y[j] : z[j];
-                        } else {
-                            tmem_wait_ld_pin32(reinterpret_cast<uint32_t*>(z));
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[j] += z[j];
-                        }
-                    };
-#pragma unroll
-                    for (int cc = 0; cc < CH; ++cc)
-                        if ((h + CS * cc) * 32 < width) add(sz[cc], (h + CS * cc) * 32);
-                    if (DUAL && h * 32 < width) add(sw, width + h * 32);
+                        for (int j = 0; j < 32; ++j) sz[cc][j] += z[j];
+                    }
                     release();
                 }
                 if (!ok) break;
 #pragma unroll
                 for (int cc = 0; cc < CH; ++cc) {
                     const int c = h + CS * cc;
-                    if (c * 32 < width) chunk(t, c, sz[cc], sw);
+                    if (c * 32 < width) chunk(t, c, sz[cc], none);
                 }
             } else {
                 if (!wait_full()) break;
@@ -899,10 +838,8 @@ inline uint32_t b_bytes_of(int cg, int bn, bool mn) {
 }
 
 // How a product's sums are kept: 0 one accumulation (16-bit results), 1 added up in registers
-// every 640 indices (16-bit operands whose results, or column sums, are float32), 2 float32
-// operands, every 320.
-int mode_of(const Product& p, int dt) {
-    if (dt == MABA_F32) return 2;
+// every 640 indices (results, or column sums, that are float32).
+int mode_of(const Product& p) {
     if (p.e.kind == E_LINEAR_BWD) return p.e.sums_f32 && p.K > 640 ? 1 : 0;
     return p.e.kind == E_LINEAR && p.e.out_f32 ? 1 : 0;
 }
@@ -910,25 +847,24 @@ int mode_of(const Product& p, int dt) {
 // The tile and the splits with the least estimated time.  Per k-block and SM: the larger of
 // the products (128 x bn x 64 at 4,096 per cycle) and the loads (60 bytes per cycle from L2);
 // a unit that is not hidden under another adds its fill and epilogue.  The registers that
-// hold a unit's sums bound bn in modes 1 and 2.  Splits also bound what one accumulation
+// hold a unit's sums bound bn in mode 1.  Splits also bound what one accumulation
 // truncates: at most 16,384 indices.
 Plan plan_of(const Product& p, int mode, double* time) {
     const bool dual = p.form == F_DUAL, store = p.e.kind == E_STORE;
     const int kblocks = (int)ceil_div(p.K, BK) * (p.form == F_SUM ? 2 : 1);
     const int pairs = p.form == F_PAIR ? 2 : 1;
-    const int planes = mode == 2 ? 3 : 1, terms = mode == 2 ? 6 : 1;
     const int fewest = store && mode == 0 ? (kblocks + 255) / 256 : 1;
     const double out = 8.0 * pairs * (double)p.M * (double)p.N / 3500.0;  // one split's sums, written and read
     Plan best;
     double least = 1e300;
     for (int cg = 1; cg <= 2; ++cg) {
-        const int most = mode == 2 ? 128 : (cg == 2 ? 256 : 192), slots = sm_count() / cg;
+        const int most = cg == 2 ? 256 : 192, slots = sm_count() / cg;
         const int m = (int)((p.M + 128 * cg - 1) / (128 * cg)), n = (int)p.N;
         const double rows = (double)m * pairs;
         for (int bn = dual ? 64 : 32; bn <= most; bn += dual ? 64 : 32) {
             const int cols = dual ? bn / 2 : bn;
             const double tiles = rows * (n / cols + (n % cols != 0));
-            const double mma = 2.0 * bn * terms, load = planes * (A_BYTES + b_bytes_of(cg, bn, p.b_mn)) / 60.0;
+            const double mma = 2.0 * bn, load = (A_BYTES + b_bytes_of(cg, bn, p.b_mn)) / 60.0;
             const double kcost = mma > load ? mma : load;
             // as few splits as may be, or as many as fill the GPU once, twice (up to 15 more)
             for (int i = 0; i < (store ? 3 : 1); ++i) {
@@ -947,23 +883,23 @@ Plan plan_of(const Product& p, int mode, double* time) {
     return best;
 }
 
-// One operand's map: rows x contraction (x planes), read K-major (contraction contiguous) or
+// One operand's map: rows x contraction, read K-major (contraction contiguous) or
 // MN-major.
-bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int planes, int64_t rows, int64_t k, bool mn, int box_rows) {
-    const int64_t dims[3] = {mn ? rows : k, mn ? k : rows, planes};
+bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int64_t rows, int64_t k, bool mn, int box_rows) {
+    const int64_t dims[3] = {mn ? rows : k, mn ? k : rows, 1};
     const int64_t ld = dims[1] > 1 ? (mn ? x.sk : x.sr) : (dims[0] + 7) / 8 * 8;
-    const int64_t strides[2] = {ld, planes > 1 ? x.sp : ld};
+    const int64_t strides[2] = {ld, ld};
     const uint32_t box[3] = {(uint32_t)BK, (uint32_t)(mn ? BK : box_rows), 1};
     return make_map(m, dt, x.p, 3, dims, strides, box);
 }
 
-// The map of a matrix that the epilogue reads or writes in chunks, rows x cols (x planes).
-bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t planes,
+// The map of a matrix that the epilogue reads or writes in chunks, rows x cols (x parts).
+bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t parts,
                uint32_t box_rows = 32) {
     const int el = dt == MABA_F32 ? 4 : 2;
     if (rows == 1) ld = (cols + 7) / 8 * 8;
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (ld * el) % 16 != 0 || ld < cols) return false;
-    const int64_t dims[3] = {cols, rows, planes}, strides[2] = {ld, planes > 1 ? rows * ld : ld};
+    const int64_t dims[3] = {cols, rows, parts}, strides[2] = {ld, parts > 1 ? rows * ld : ld};
     const uint32_t box[3] = {32, box_rows, 1};
     return make_map(m, dt, p, 3, dims, strides, box);
 }
@@ -994,19 +930,17 @@ template <typename T, int CG, bool A_MN, bool B_MN, int KIND, int MODE> int read
 }
 
 template <typename T, int CG> int kernel_of(Kernel* k, const Product& p, int mode, int device) {
-    constexpr int M = sizeof(T) == 4 ? 2 : 0;
-    if constexpr (M == 0)
-        if (mode == 1)
-            return p.e.kind == E_LINEAR ? ready<T, CG, false, false, E_LINEAR, 1>(k, device)
-                                        : ready<T, CG, false, false, E_LINEAR_BWD, 1>(k, device);
+    if (mode == 1)
+        return p.e.kind == E_LINEAR ? ready<T, CG, false, false, E_LINEAR, 1>(k, device)
+                                    : ready<T, CG, false, false, E_LINEAR_BWD, 1>(k, device);
     switch (p.e.kind) {
-        case E_LINEAR: return ready<T, CG, false, false, E_LINEAR, M>(k, device);
-        case E_LINEAR_BWD: return ready<T, CG, false, false, E_LINEAR_BWD, M>(k, device);
-        case E_GLU: return ready<T, CG, false, false, E_GLU, M>(k, device);
-        case E_GLU_BWD: return ready<T, CG, false, false, E_GLU_BWD, M>(k, device);
+        case E_LINEAR: return ready<T, CG, false, false, E_LINEAR, 0>(k, device);
+        case E_LINEAR_BWD: return ready<T, CG, false, false, E_LINEAR_BWD, 0>(k, device);
+        case E_GLU: return ready<T, CG, false, false, E_GLU, 0>(k, device);
+        case E_GLU_BWD: return ready<T, CG, false, false, E_GLU_BWD, 0>(k, device);
         default:
-            if (p.a_mn) return ready<T, CG, true, true, E_STORE, M>(k, device);
-            return p.b_mn ? ready<T, CG, false, true, E_STORE, M>(k, device) : ready<T, CG, false, false, E_STORE, M>(k, device);
+            if (p.a_mn) return ready<T, CG, true, true, E_STORE, 0>(k, device);
+            return p.b_mn ? ready<T, CG, false, true, E_STORE, 0>(k, device) : ready<T, CG, false, false, E_STORE, 0>(k, device);
     }
 }
 
@@ -1028,10 +962,10 @@ Product split_sums(const Product& p) {
 
 // A product with an epilogue whose few tiles have a long contraction: its sums by splits,
 // then the epilogue, where the model says that this is sooner.  (24 x 3,776 -> 2 x 120 float32,
-// one tile of 59 blocks: forward and gradients 66 us, 139 without.)  A float32 result of 16-bit
+// one tile of 59 blocks.)  A float32 result of 16-bit
 // operands keeps its bound on one accumulation, 640 indices.
-Plan tc_plan(const Product& p, int dt) {
-    const int mode = mode_of(p, dt);
+Plan tc_plan(const Product& p) {
+    const int mode = mode_of(p);
     double whole, split;
     const Plan plan = plan_of(p, mode, &whole);
     if (p.e.kind == E_STORE || p.K < 16 * BK) return plan;
@@ -1048,9 +982,8 @@ Plan tc_plan(const Product& p, int dt) {
 template <typename T>
 int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cudaStream_t s) {
     if (encode_fn() == nullptr) return set_error(MABA_ERR_CUDA, "dense: cuTensorMapEncodeTiled not found");
-    constexpr int dt = sizeof(T) == 4 ? MABA_F32 : (std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16);
-    constexpr int planes = dt == MABA_F32 ? 3 : 1, odt = dt == MABA_F16 ? MABA_F16 : MABA_BF16;
-    const int mode = mode_of(p, dt);
+    constexpr int dt = std::is_same<T, __nv_bfloat16>::value ? MABA_BF16 : MABA_F16;
+    const int mode = mode_of(p);
     const bool dual = p.form == F_DUAL, a_mn = p.a_mn, b_mn = p.b_mn;
     TcArgs a{};
     a.M = p.M, a.N = p.N;
@@ -1071,34 +1004,31 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.d_col = workers / (a.splits * a.pairs) % a.tiles_n;
     a.d_row = workers / (a.splits * a.pairs) / a.tiles_n;
     const uint32_t bb = b_bytes_of(pl.cg, pl.bn, b_mn);
-    a.flush = mode == 0 ? a.kblocks : (mode == 1 ? 640 / BK : 320 / BK);
-    a.b_at = planes * A_BYTES;
-    a.b_bytes = (bb + 1023) / 1024 * 1024;
-    a.stage_bytes = planes * (A_BYTES + a.b_bytes);
-    a.load_bytes = planes * (A_BYTES + bb) * pl.cg;
+    a.flush = mode == 0 ? a.kblocks : 640 / BK;
+    a.stage_bytes = A_BYTES + (bb + 1023) / 1024 * 1024;
+    a.load_bytes = (A_BYTES + bb) * pl.cg;
     // staging: two buffers each way where that leaves enough stages for the products, else fewer
     const int epi = mode == 0 ? Warps<0>::EPI : Warps<1>::EPI, threads = mode == 0 ? Warps<0>::THREADS : Warps<1>::THREADS;
     const bool vecs = p.e.kind == E_LINEAR || p.e.kind == E_LINEAR_BWD;
     const uint32_t vec_bytes = !vecs ? 0 : epi * (mode == 0 ? Warps<0>::VEC_BYTES : Warps<1>::VEC_BYTES);
-    const bool to_planes = planes == 3 && (p.e.kind == E_LINEAR_BWD || p.e.kind == E_GLU_BWD);
-    const bool out_f32 = !to_planes && (planes == 3 || p.e.out_f32 || a.splits > 1), side_f32 = planes == 3 || p.e.res.f32;
+    const bool out_f32 = p.e.out_f32 || a.splits > 1, side_f32 = p.e.res.f32;
     a.in_bytes = p.e.res.p ? (side_f32 ? 4096 : 2048) : 0;
     a.out_bytes = out_f32 ? 4096 : 2048;
     const uint32_t fixed = 1024 + BAR_BYTES + vec_bytes;
     uint32_t staging = 0;
-    a.in_place = p.e.res.p && (p.e.kind == E_LINEAR || (p.e.kind == E_LINEAR_BWD && !to_planes)) && side_f32 == out_f32;
+    a.in_place = p.e.res.p && vecs && side_f32 == out_f32;
     if (a.in_place) a.out_bytes = 0;
     for (int t = 0; t < 3; ++t) {
         a.n_in = t < 2 ? 2 : 1, a.n_out = t < 1 ? 2 : 1;
         staging = epi * (a.n_in * a.in_bytes + a.n_out * a.out_bytes);
         a.stages = (int)((SMEM_MAX - fixed - staging) / a.stage_bytes);
-        if (a.stages >= (mode == 2 ? 2 : (a.in_place ? 4 : 5))) break;
+        if (a.stages >= (a.in_place ? 4 : 5)) break;
     }
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     a.vec_at = a.stages * a.stage_bytes + staging;
     a.bar_at = a.vec_at + vec_bytes;
     const size_t smem = 1024 + a.bar_at + BAR_BYTES;
-    a.idesc = idesc_f16(128 * pl.cg, pl.bn, odt == MABA_BF16, a_mn, b_mn);
+    a.idesc = idesc_f16(128 * pl.cg, pl.bn, dt == MABA_BF16, a_mn, b_mn);
     a.e = p.e;
     a.partial = partial;
     a.ldp = ldp;
@@ -1111,23 +1041,19 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     const int na = p.form == F_SUM || p.form == F_PAIR ? 2 : 1, nb = na == 2 || dual ? 2 : 1;
     const int box = dual ? pl.bn / 2 : a.b_rows;
     bool ok = true;
-    for (int i = 0; i < na; ++i) ok = ok && operand_map(&m[i], odt, p.a[i], planes, p.M, p.K, a_mn, 128);
-    for (int i = 0; i < nb; ++i) ok = ok && operand_map(&m[2 + i], odt, p.b[i], planes, p.N, p.K, b_mn, box);
+    for (int i = 0; i < na; ++i) ok = ok && operand_map(&m[i], dt, p.a[i], p.M, p.K, a_mn, 128);
+    for (int i = 0; i < nb; ++i) ok = ok && operand_map(&m[2 + i], dt, p.b[i], p.N, p.K, b_mn, box);
     if (!ok) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     if (na == 1) m[1] = m[0];
     if (nb == 1) m[3] = m[2];
     m[4] = m[5] = m[6] = m[0];
-    if (p.e.res.p && !chunk_map(&m[4], side_f32 ? MABA_F32 : odt, p.e.res.p, p.M, p.N, p.e.res.sr, 1, 128))
+    if (p.e.res.p && !chunk_map(&m[4], side_f32 ? MABA_F32 : dt, p.e.res.p, p.M, p.N, p.e.res.sr, 1, 128))
         return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     if (a.splits > 1) {
         a.out_tma = chunk_map(&m[5], MABA_F32, partial, p.M, p.N, ldp, a.splits * a.pairs);
-    } else if (to_planes) {
-        a.out_tma = chunk_map(&m[5], MABA_BF16, p.e.out, p.M, p.N, p.e.ldo, 3) &&
-                    (!p.e.out2 || chunk_map(&m[6], MABA_BF16, p.e.out2, p.M, p.N, p.e.ldo, 3));
-        if (!a.out_tma) return set_error(MABA_ERR_CUDA, "dense: tensor map refused");
     } else {
-        a.out_tma = chunk_map(&m[5], out_f32 ? MABA_F32 : odt, p.e.out, p.M, p.N, p.e.ldo, 1) &&
-                    (!p.e.out2 || chunk_map(&m[6], out_f32 ? MABA_F32 : odt, p.e.out2, p.M, p.N, p.e.ldo, 1));
+        a.out_tma = chunk_map(&m[5], out_f32 ? MABA_F32 : dt, p.e.out, p.M, p.N, p.e.ldo, 1) &&
+                    (!p.e.out2 || chunk_map(&m[6], out_f32 ? MABA_F32 : dt, p.e.out2, p.M, p.N, p.e.ldo, 1));
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(workers * pl.cg));
@@ -1144,7 +1070,6 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     if (err != cudaSuccess) return set_error(MABA_ERR_CUDA, "dense(tcgen05): %s", cudaGetErrorString(err));
     return check_launch("dense(tcgen05)");
 }
-template int tc_product<float>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
 template int tc_product<__half>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
 template int tc_product<__nv_bfloat16>(const Product&, const Plan&, float*, int64_t, cudaStream_t);
 

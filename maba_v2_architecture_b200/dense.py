@@ -9,9 +9,8 @@ The reference computes these with torch modules and autograd: SwiGLUFFN (maba_sp
 
 Inputs are float32, float16 or bfloat16 CUDA tensors of one type with any strides; leading
 dimensions of ``x`` are rows.  Sums are float32 and a result is rounded once; results do not
-depend on the order in which the GPU runs the work.  Float32 products have float32's accuracy (they
-run on the tensor cores as three bf16 planes each; elements below 2^-102 are off by up to 2^-125).  Inputs are never written, except that
-``out`` may be ``residual``.  Work is enqueued on the current stream of the tensors' device.
+depend on the order in which the GPU runs the work.  16-bit products run on the tensor cores,
+float32 ones on the CUDA cores.  Inputs are never written, except that ``out`` may be ``residual``.  Work is enqueued on the current stream of the tensors' device.
 Scratch memory comes from torch's allocator for each call (not from the per-stream buffer that
 the other ops keep): two captured graphs, or a graph and an eager call, then never share it.
 
@@ -164,7 +163,7 @@ def _linear(x, weight, bias, act, scale, residual, out, out_dtype):
     index = x.get_device()
     rc = N.ERR_WORKSPACE
     # most calls need no scratch memory: tried without (refused before any launch)
-    if index == _current_device() and (x.dtype is not torch.float32 or x.numel() <= 8 * x.shape[-1]):
+    if index == _current_device():
         rc = lib.maba_linear(dx, dw, db, act, ds, dr, do, None, 0, _raw_stream(index))
     if rc:
         if rc != N.ERR_WORKSPACE:
@@ -297,7 +296,7 @@ def _gated_ffn(x, w_gate, w_up, act, out):
     lib = N.lib()
     index = x.get_device()
     rc = N.ERR_WORKSPACE
-    if index == _current_device() and (x.dtype is not torch.float32 or x.numel() <= 8 * x.shape[-1]):  # (as in _linear)
+    if index == _current_device():  # (as in _linear)
         rc = lib.maba_gated_ffn(dx, dg, du, act, do, None, 0, _raw_stream(index))
     if rc:
         if rc != N.ERR_WORKSPACE:
