@@ -486,7 +486,7 @@ int linear_backward(Ctx& c, const LinearArgs& a) {
     }
     if (!need_dx && !need_dw && !need_db && !need_ds) return MABA_OK;
     const bool through = a.act == ACT_NONE && !given(a.scale);  // dz = g
-    const int64_t blocks = ceil_div(M, through ? CS_ROWS : (c.dt == MABA_F32 ? SIMT_ROWS : TC_ROWS));
+    const int64_t blocks = ceil_div(M, through ? CS_ROWS : TC_ROWS);
     float* pb = need_db ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     float* ps = need_ds ? static_cast<float*>(c.ws.take((size_t)blocks * N * 4)) : nullptr;
     Matrix x, w, d;

@@ -117,8 +117,7 @@ template <typename T>
 int tc_product(const Product& p, const Plan& plan, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);
 
-// dense_simt.cu: float32 operands, any strides; column sums per SIMT_ROWS rows.
-constexpr int SIMT_ROWS = 128;
+// dense_simt.cu: float32 operands, any strides; column sums per TC_ROWS rows too.
 Plan simt_plan(const Product& p);
 int simt_product(const Product& p, int splits, float* partial, int64_t ldp, cudaStream_t s);
 
