@@ -22,13 +22,12 @@
 // runs under the next unit's products.  The gated block's tile holds bn/2 rows of w_gate and
 // bn/2 of w_up, so a thread sees both projections of an element in its own row.
 //
-// What bounds it: the gated block the tensor cores (65,536 x 640 -> 2 x 1248, bf16: 146 us,
-// 1,433 TFLOP/s, 84 % of the 1,703 of an 8,192^3 library product; its two SFU operations per
-// element take 2,048 of a unit's 5,120 cycles); the linear map with a scale and a float32
-// residual (65,536 x 1248 -> 640) 118 us, 4.3 TB/s; with a bias, SiLU, scale and residual
-// (16,384 x 640 -> 2560) 66 us, by the epilogue's chains of shared-memory, barrier and copy
-// latencies, which the products' own use of shared memory stretches; its gradient pass, with
-// column sums, 84 us.
+// What bounds it (single launches): the gated block the tensor cores (65,536 x 640 -> 2 x 1248,
+// bf16: 123 us; its two SFU operations per element take 2,048 of a unit's 5,120 cycles); the
+// linear map with a scale and a float32 residual (65,536 x 1248 -> 640) 108 us, 4.7 TB/s; with a
+// bias, SiLU, scale and residual (16,384 x 640 -> 2560) 57 us, by the epilogue's chains of
+// shared-memory, barrier and copy latencies, which the products' own use of shared memory
+// stretches; its gradient pass, with column sums, 77 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
