@@ -413,6 +413,12 @@ MABA_API size_t maba_gated_ffn_backward_workspace_size(const maba_tensor* grad, 
                                                        const maba_tensor* dx, const maba_tensor* dw_gate,
                                                        const maba_tensor* dw_up);
 
+/* Self-test, host only: the partial sums of a product whose contraction is split (pairs: products
+ * that share the split, 1 or 2), rows x cols each: the bytes that a call lays out for them, and
+ * where the last of its stores ends. */
+MABA_API int maba_selftest_split_layout(int64_t rows, int64_t cols, int32_t splits, int32_t pairs, int64_t* reserved,
+                                        int64_t* reached);
+
 #ifdef __cplusplus
 }
 #endif

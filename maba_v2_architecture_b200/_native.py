@@ -70,6 +70,7 @@ SIGNATURES = {
     "maba_gated_ffn_workspace_size": (_sz, [_vp] * 4),
     "maba_gated_ffn_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 3 + [_vp, _sz, _vp]),
     "maba_gated_ffn_backward_workspace_size": (_sz, [_vp] * 7),
+    "maba_selftest_split_layout": (ctypes.c_int, [_i64, _i64, _i32, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
     "maba_decode_gemv": (ctypes.c_int, [T_P, _i32, T_P, T_P, _f32, T_P, _i32, T_P, T_P, T_P, T_P, T_P, _i32, _i32,
                                         T_P, _vp, _vp, _sz, _vp]),
     "maba_decode_gemv_workspace_size": (_sz, [_i64]),

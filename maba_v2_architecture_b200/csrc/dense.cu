@@ -267,8 +267,8 @@ int run(Ctx& c, const Product& p) {
     // sums are float32 and added in split order
     const Plan plan = c.dry ? (c.plans[c.n_plans++] = c.dt == MABA_F32 ? simt_plan(p) : tc_plan(p)) : c.plans[c.next_plan++];
     const Product sums = plan.finish ? split_sums(p) : p;
-    const int64_t rows = sums.form == F_PAIR ? 2 * p.M : p.M, ldp = (p.N + 3) / 4 * 4;
-    float* partial = plan.splits > 1 ? static_cast<float*>(c.ws.take((size_t)plan.splits * rows * ldp * 4)) : nullptr;
+    const int64_t rows = sums.form == F_PAIR ? 2 * p.M : p.M, ldp = partials_ld(p.N);
+    float* partial = plan.splits > 1 ? static_cast<float*>(c.ws.take((size_t)partials_bytes(plan.splits, rows, p.N))) : nullptr;
     if (c.dry) return MABA_OK;
     if (c.dt == MABA_F32) MABA_TRY(simt_product(sums, plan.splits, partial, ldp, c.s));
     else MABA_TRY(DENSE_DISPATCH16(c.dt, [&] { return tc_product<T>(sums, plan, partial, ldp, c.s); }));
@@ -708,4 +708,13 @@ extern "C" size_t maba_gated_ffn_backward_workspace_size(const maba_tensor* grad
     a.g = grad, a.x = x, a.wg = w_gate, a.wu = w_up, a.act = ACT_SILU, a.dx = dx, a.dwg = dw_gate, a.dwu = dw_up;
     if (check_ffn(a, true) != MABA_OK) return 0;
     return query(a, ffn_backward).ws.used;
+}
+
+extern "C" int maba_selftest_split_layout(int64_t rows, int64_t cols, int32_t splits, int32_t pairs, int64_t* reserved,
+                                          int64_t* reached) {
+    if (rows < 1 || cols < 1 || splits < 1 || pairs < 1 || reserved == nullptr || reached == nullptr)
+        return set_error(MABA_ERR_INVALID, "selftest_split_layout: sizes must be positive");
+    *reserved = partials_bytes(splits, rows * pairs, cols);
+    *reached = 4 * partials_reach(rows, cols, partials_ld(cols), (int64_t)splits * pairs);
+    return MABA_OK;
 }

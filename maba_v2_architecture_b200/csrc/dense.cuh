@@ -97,6 +97,8 @@ template <typename T> __device__ __forceinline__ float side_at(const Side& s, in
 }
 
 // Partial sums of a split product: float32 [split][rows][ldp], rows = M (2 M of F_PAIR).
+inline int64_t partials_ld(int64_t cols) { return (cols + 3) / 4 * 4; }
+inline int64_t partials_bytes(int64_t splits, int64_t rows, int64_t cols) { return splits * rows * partials_ld(cols) * 4; }
 
 // dense_skinny.cu: forward products of few rows, any strides.
 bool skinny_takes(const Product& p, int dt);
@@ -113,6 +115,8 @@ struct Plan {
 bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t col_stride);
 Plan tc_plan(const Product& p);
 Product split_sums(const Product& p);  // the same sums as a plain product, two for F_DUAL
+// End, in elements, of the partial sums [parts][rows][ldp] where the tensor-memory copies store them.
+int64_t partials_reach(int64_t rows, int64_t cols, int64_t ldp, int64_t parts);
 template <typename T>
 int tc_product(const Product& p, const Plan& plan, float* partial, int64_t ldp, cudaStream_t s);
 int device_error_take(cudaStream_t s, int* out);

@@ -892,15 +892,23 @@ bool operand_map(CUtensorMap* m, int dt, const Matrix& x, int64_t rows, int64_t 
     return make_map(m, dt, x.p, 3, dims, strides, box);
 }
 
-// The map of a matrix that the epilogue reads or writes in chunks, rows x cols (x parts).
+// The place of a matrix that the epilogue reads or writes in chunks, rows x cols (x parts, one after
+// another), in elements of el bytes; false where copies cannot address it.
+struct ChunkLayout {
+    int64_t dims[3], strides[2];
+};
+bool chunk_layout(ChunkLayout* c, int el, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t parts) {
+    // one row's stride is never used, whatever the caller's is; parts lie rows * ld apart even so
+    if (rows == 1 && parts == 1) ld = (cols + 7) / 8 * 8;
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (ld * el) % 16 != 0 || ld < cols) return false;
+    *c = {{cols, rows, parts}, {ld, parts > 1 ? rows * ld : ld}};
+    return true;
+}
 bool chunk_map(CUtensorMap* m, int dt, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t parts,
                uint32_t box_rows = 32) {
-    const int el = dt == MABA_F32 ? 4 : 2;
-    if (rows == 1) ld = (cols + 7) / 8 * 8;
-    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (ld * el) % 16 != 0 || ld < cols) return false;
-    const int64_t dims[3] = {cols, rows, parts}, strides[2] = {ld, parts > 1 ? rows * ld : ld};
+    ChunkLayout c;
     const uint32_t box[3] = {32, box_rows, 1};
-    return make_map(m, dt, p, 3, dims, strides, box);
+    return chunk_layout(&c, dt == MABA_F32 ? 4 : 2, p, rows, cols, ld, parts) && make_map(m, dt, p, 3, c.dims, c.strides, box);
 }
 
 using Kernel = void (*)(const TcArgs, const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
@@ -949,6 +957,12 @@ bool tc_readable(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t 
     if (col_stride != 1 && cols > 1) return false;
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return false;
     return rows == 1 || (ld % 8 == 0 && ld >= cols);
+}
+
+int64_t partials_reach(int64_t rows, int64_t cols, int64_t ldp, int64_t parts) {
+    ChunkLayout c;
+    if (!chunk_layout(&c, 4, nullptr, rows, cols, ldp, parts)) return (parts * rows - 1) * ldp + cols;
+    return (parts - 1) * c.strides[1] + (rows - 1) * c.strides[0] + cols;
 }
 
 Product split_sums(const Product& p) {

@@ -1,0 +1,54 @@
+"""Edges of the dense operators: products of one row whose contraction is split, among others.
+Values and bounds from tests/dense_oracle.py."""
+import pytest
+import torch
+
+import dense_oracle as O
+import maba_v2_architecture_b200 as mb
+from maba_v2_architecture_b200 import _native as N
+from test_gpu_dense import BF, DEV, F32, HF, gen, linear_case, no_device_error, randn  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# Products of one row (dx, dz and the projections of one row; dW of one output feature) with a split
+# contraction, widths of 1 to 4 past a multiple of eight, and their neighbours
+ONE = [(4096, 300, 1), (8192, 100, 1), (1, 300, 2048), (1, 100, 2048), (1, 650, 1251), (1, 4000, 100), (1, 4000, 25),
+       (2, 4000, 100), (4096, 300, 2), (1, 104, 2048)]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("m,k,n", ONE)
+def test_split_sums_of_one_row(m, k, n, dt):
+    for i, (act, bias, scale) in enumerate([("none", "none", "none"), ("none", "f32", "f32"), ("silu", "same", "f32")]):
+        t = linear_case(m, k, n, dt, bias, scale, "none", seed=i, grad=dt)
+        want = O.linear_backward(t["g"], t["x"], t["w"], t["bias"], act, t["scale"])
+        for name, v in zip(("dx", "dw", "dbias", "dscale"),
+                           mb.b200_linear_backward(t["g"], t["x"], t["w"], t["bias"], act, t["scale"])):
+            if v is not None:
+                O.assert_within(v, want[name], f"{name} {(m, k, n)} {act}")
+    g = gen(6)
+    x, wg, wu = randn(g, m, k, dt=dt), randn(g, n, k, dt=dt, std=k ** -0.5), randn(g, n, k, dt=dt, std=k ** -0.5)
+    d = randn(g, m, n, dt=dt, std=0.3)
+    want = O.gated_backward(d, x, wg, wu, "silu")
+    for name, v in zip(("dx", "dw_gate", "dw_up"), mb.b200_gated_ffn_backward(d, x, wg, wu)):
+        O.assert_within(v, want[name], f"{name} {(m, k, n)}")
+
+
+@pytest.mark.parametrize("m,k,n", ONE)
+def test_nothing_is_written_behind_the_workspace(m, k, n):
+    """The C entries with a workspace of exactly the size they ask for, in a larger buffer whose other
+    bytes keep their values."""
+    t = linear_case(m, k, n, BF, "none", "none", "none", seed=3, grad=BF)
+    wu = randn(gen(4), n, k, dt=BF, std=k ** -0.5)
+    dx, dw, dwu = torch.empty_like(t["x"]), torch.empty_like(t["w"]), torch.empty_like(wu)
+    pg, px, pw, pwu, pdx, pdw, pdwu = map(N.pack_matrix, (t["g"], t["x"], t["w"], wu, dx, dw, dwu))
+    lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
+    linear = (pg, px, pw, None, 2, None, pdx, pdw, None, None)
+    ffn = (pg, px, pw, pwu, 2, pdx, pdw, pdwu)
+    for fn, args, need in ((lib.maba_linear_backward, linear, lib.maba_linear_backward_workspace_size(*linear)),
+                           (lib.maba_gated_ffn_backward, ffn, lib.maba_gated_ffn_backward_workspace_size(*ffn[:4], *ffn[5:]))):
+        buf = torch.full((need + 8192,), 0x5a, dtype=torch.uint8, device=DEV)
+        assert need and buf.data_ptr() % 256 == 0
+        N.check(fn(*args, buf.data_ptr(), need, stream), fn.__name__)
+        torch.cuda.synchronize()
+        assert bool((buf[need:] == 0x5a).all())
