@@ -704,7 +704,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
                 side_used(a.in_place);
                 if (e.scale.p) with_vector<FRAG>(z, vs, lane, mul2);
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) add2(sb[((j >> 2) & 3) * 2], sb[((j >> 2) & 3) * 2 + 1], z[j], z[j + 1]);
+                for (int j = 0; j < 32; j += 2) {
+                    if (k.rows < 32 && frag_row(j, lane) >= k.rows) continue;  // whatever the scale is
+                    add2(sb[((j >> 2) & 3) * 2], sb[((j >> 2) & 3) * 2 + 1], z[j], z[j + 1]);
+                }
                 const int col = frag_sum_col(lane);
                 const int64_t at = (int64_t)(k.row0 >> 5) * a.N + k.col0 + col;
                 if (e.part_bias) {

@@ -52,3 +52,20 @@ def test_nothing_is_written_behind_the_workspace(m, k, n):
         N.check(fn(*args, buf.data_ptr(), need, stream), fn.__name__)
         torch.cuda.synchronize()
         assert bool((buf[need:] == 0x5a).all())
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("m,k", [(70, 40), (200, 40), (1001, 700), (70, 4000)])
+def test_an_infinite_scale_stays_in_its_column(m, k, dt):
+    """dz = grad * scale is +inf in every row of that column, and so is its sum, however many rows the
+    last block of 32 lacks.  The other columns are what they are without it."""
+    n, col = 72, 5
+    t = linear_case(m, k, n, dt, "f32", "f32", "none", seed=7, grad=dt)
+    t["g"] = t["g"].abs() + 0.25
+    clean = mb.b200_linear_backward(t["g"], t["x"], t["w"], t["bias"], "none", t["scale"], needs=(False, False, True, True))
+    scale = t["scale"].clone()
+    scale[col] = float("inf")
+    db, ds = mb.b200_linear_backward(t["g"], t["x"], t["w"], t["bias"], "none", scale, needs=(False, False, True, True))[2:]
+    assert float(db[col]) == float("inf")
+    db[col] = clean[2][col]
+    assert torch.equal(db, clean[2]) and torch.equal(ds, clean[3])
