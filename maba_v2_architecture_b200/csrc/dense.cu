@@ -43,6 +43,9 @@ int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStrea
     return check_launch("dense");
 }
 
+// A grid's second dimension holds 65,535 blocks: the kernels that use it walk on by gridDim.y
+unsigned grid_y(int64_t blocks) { return (unsigned)(blocks < 32768 ? blocks : 32768); }
+
 // ---------------------------------------------------------------------------
 // small kernels
 // ---------------------------------------------------------------------------
@@ -196,23 +199,27 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// part[blk][n] = sum of g over rows [128 blk, 128 blk + 128), added in row order
+// part[blk][n] = sum of g over rows [128 blk, 128 blk + 128): eight warps take every eighth row each,
+// and their sums are added in turn
 constexpr int CS_ROWS = 128;
 template <typename T>
 __global__ void __launch_bounds__(256) colsum_kernel(Side g, int64_t rows, int64_t cols, float* part) {
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     __shared__ float red[8][32];
-    const int64_t r0 = (int64_t)blockIdx.y * CS_ROWS;
-    float s = 0.f;
-    if (c < cols)
-        for (int64_t r = r0 + w; r < rows && r < r0 + CS_ROWS; r += 8) s += side_at<T>(g, r, c);
-    red[w][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (w == 0 && c < cols) {
-        float t = 0.f;
-        for (int q = 0; q < 8; ++q) t += red[q][threadIdx.x];
-        part[(int64_t)blockIdx.y * cols + c] = t;
+    for (int64_t blk = blockIdx.y; blk * CS_ROWS < rows; blk += gridDim.y) {
+        const int64_t r0 = blk * CS_ROWS;
+        float s = 0.f;
+        if (c < cols)
+            for (int64_t r = r0 + w; r < rows && r < r0 + CS_ROWS; r += 8) s += side_at<T>(g, r, c);
+        red[w][lane] = s;
+        __syncthreads();
+        if (w == 0 && c < cols) {
+            float t = 0.f;
+            for (int q = 0; q < 8; ++q) t += red[q][lane];
+            part[blk * cols + c] = t;
+        }
+        __syncthreads();
     }
 }
 
@@ -274,16 +281,11 @@ int run(Ctx& c, const Product& p) {
     else MABA_TRY(DENSE_DISPATCH16(c.dt, [&] { return tc_product<T>(sums, plan, partial, ldp, c.s); }));
     if (plan.splits == 1) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        const int64_t cap = 32768;
-        if (plan.finish) {
-            const int64_t gy = ceil_div(p.M, 32);
-            return launch(finish_kernel<T>, dim3((unsigned)ceil_div(p.N, 32), (unsigned)(gy < cap ? gy : cap)), dim3(256), 0,
-                              c.s, partial, ldp, plan.splits, p.M, p.N, p.e);
-        }
-        const int64_t gy = ceil_div(rows, 8);
-        return launch(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), (unsigned)(gy < cap ? gy : cap)), dim3(256),
-                          0, c.s, partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2),
-                          p.M, p.e.ldo);
+        if (plan.finish)
+            return launch(finish_kernel<T>, dim3((unsigned)ceil_div(p.N, 32), grid_y(ceil_div(p.M, 32))), dim3(256), 0, c.s,
+                          partial, ldp, plan.splits, p.M, p.N, p.e);
+        return launch(sum_splits_kernel<T>, dim3((unsigned)ceil_div(p.N, 128), grid_y(ceil_div(rows, 8))), dim3(256), 0, c.s,
+                      partial, ldp, plan.splits, rows, p.N, static_cast<T*>(p.e.out), static_cast<T*>(p.e.out2), p.M, p.e.ldo);
     });
 }
 
@@ -309,7 +311,7 @@ int prepare(Ctx& c) {
 int column_sums(Ctx& c, const Side& g, int64_t rows, int64_t cols, float* part) {
     if (c.dry) return MABA_OK;
     return DENSE_DISPATCH(c.dt, [&] {
-        const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)ceil_div(rows, CS_ROWS));
+        const dim3 grid((unsigned)ceil_div(cols, 32), grid_y(ceil_div(rows, CS_ROWS)));
         return launch(colsum_kernel<T>, grid, dim3(256), 0, c.s, g, rows, cols, part);
     });
 }

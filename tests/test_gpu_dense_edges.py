@@ -69,3 +69,18 @@ def test_an_infinite_scale_stays_in_its_column(m, k, dt):
     assert float(db[col]) == float("inf")
     db[col] = clean[2][col]
     assert torch.equal(db, clean[2]) and torch.equal(ds, clean[3])
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_column_sums_of_many_rows(dt):
+    """More blocks of 128 rows than a grid's second dimension holds (65,535).  The gradient's elements
+    are 0 and 1, so every partial sum is a whole number below 2^24 and the sums are exact."""
+    m, k, n = 8_400_000, 8, 8
+    rows = torch.arange(m, device=DEV)
+    g = torch.stack([rows % 3 == c % 3 if c < 6 else rows >= 65535 * 128 + 40 * (c - 7) for c in range(n)], 1).to(dt)
+    x, w, b = randn(gen(1), m, k, dt=dt), randn(gen(2), n, k, dt=dt), torch.zeros(n, device=DEV)
+    dx, dw, db, _ = mb.b200_linear_backward(g, x, w, b)
+    assert torch.equal(db, g.sum(0, dtype=torch.float64).float())
+    want = O.linear_backward(g[-300:], x[-300:], w, b)
+    O.assert_within(dx[-300:], want["dx"], "dx")
+    assert dw.shape == w.shape and bool(dw.isfinite().all())
