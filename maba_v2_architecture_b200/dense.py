@@ -15,7 +15,7 @@ Scratch memory comes from torch's allocator for each call (not from the per-stre
 the other ops keep): two captured graphs, or a graph and an eager call, then never share it.
 
 With gradients enabled and an input that requires one, both functions record themselves for
-autograd (first derivatives); ``*_backward`` are the same gradients as plain calls, for training
+autograd (first derivatives, reverse mode; dual tensors are refused); ``*_backward`` are the same gradients as plain calls, for training
 loops that are captured into a CUDA graph or keep their own tape.
 """
 from __future__ import annotations
@@ -23,6 +23,7 @@ from __future__ import annotations
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -83,6 +84,13 @@ def _activation(name: str, plain: bool) -> int:
         names = [a for a, c in ACTIVATIONS.items() if plain or c]
         raise ValueError(f"Unknown activation {name!r}. Supported: {names}")
     return code
+
+
+def _no_tangents(op: str, *ts: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors, whose tangents the kernels would drop; called inside a dual level."""
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{op}: forward-mode derivatives are not supported")
 
 
 def _span(t: torch.Tensor) -> Tuple[int, int]:
@@ -198,6 +206,8 @@ class _LinearFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         x, weight, bias, scale = ctx.saved_tensors
+        if forward_ad._current_level >= 0:
+            _no_tangents("linear_backward", grad_out, x, weight, bias, scale)
         dx, dw, db, ds = _linear_backward(grad_out, x, weight, bias, ctx.act, scale, ctx.needs_input_grad[:4])
         dr = grad_out.to(ctx.res_dtype) if ctx.needs_input_grad[4] else None
         return dx, dw, db, ds, dr, None, None
@@ -234,6 +244,8 @@ def b200_linear(
         _check_side(residual, "residual", x, shape)
     if out_dtype is not None and out_dtype is not torch.float32 and out_dtype is not x.dtype:
         raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear", x, weight, bias, scale, residual, out)
     if not x.is_cuda:
         N.require_cuda(x, op="linear")
     tracked = torch.is_grad_enabled() and (
@@ -274,6 +286,8 @@ def b200_linear_backward(
     if scale is not None:
         _check_side(scale, "scale", x, (n,))
     _check_side(grad_out, "grad_out", x, (*x.shape[:-1], n))
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear_backward", grad_out, x, weight, bias, scale)
     N.require_cuda(x, op="linear_backward")
     needs = (bool(needs[0]), bool(needs[1]), bool(needs[2]) and bias is not None, bool(needs[3]) and scale is not None)
     return _linear_backward(grad_out, x, weight, bias, act, scale, needs)
@@ -330,7 +344,10 @@ class _GatedFFNFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        return (*_gated_ffn_backward(grad_out, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad[:3]), None)
+        x, w_gate, w_up = ctx.saved_tensors
+        if forward_ad._current_level >= 0:
+            _no_tangents("gated_ffn_backward", grad_out, x, w_gate, w_up)
+        return (*_gated_ffn_backward(grad_out, x, w_gate, w_up, ctx.act, ctx.needs_input_grad[:3]), None)
 
 
 def b200_gated_ffn(
@@ -350,6 +367,8 @@ def b200_gated_ffn(
     act = _activation(activation, False)
     n, k = _check_x(x, w_gate, "w_gate")
     _check_weight(w_up, "w_up", x, n, k)
+    if forward_ad._current_level >= 0:
+        _no_tangents("gated_ffn", x, w_gate, w_up, out)
     if not x.is_cuda:
         N.require_cuda(x, op="gated_ffn")
     tracked = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
@@ -378,6 +397,8 @@ def b200_gated_ffn_backward(
     n, k = _check_x(x, w_gate, "w_gate")
     _check_weight(w_up, "w_up", x, n, k)
     _check_side(grad_out, "grad_out", x, (*x.shape[:-1], n), f32=False)
+    if forward_ad._current_level >= 0:
+        _no_tangents("gated_ffn_backward", grad_out, x, w_gate, w_up)
     N.require_cuda(x, op="gated_ffn_backward")
     return _gated_ffn_backward(grad_out, x, w_gate, w_up, act, tuple(bool(n) for n in needs))
 

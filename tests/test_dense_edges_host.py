@@ -1,8 +1,10 @@
-"""Edges of the dense operators that need no GPU: the layout of split sums."""
+"""Edges of the dense operators that need no GPU: the layout of split sums, refusals."""
 import ctypes
 
 import pytest
+import torch
 
+import maba_v2_architecture_b200 as mb
 from maba_v2_architecture_b200 import _native as N
 
 
@@ -25,3 +27,30 @@ def test_split_layout_refusals():
     for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
         assert N.lib().maba_selftest_split_layout(*bad, ctypes.byref(v), ctypes.byref(v)) == N.ERR_INVALID
     assert N.lib().maba_selftest_split_layout(1, 1, 1, 1, None, ctypes.byref(v)) == N.ERR_INVALID
+
+
+# ---------------------------------------------------------------------------
+# forward-mode derivatives
+# ---------------------------------------------------------------------------
+def test_dual_tensors_are_refused():
+    """A tangent is not dropped in silence, whichever input carries it."""
+    fw = torch.autograd.forward_ad
+    t = {"x": torch.zeros(4, 16), "w": torch.zeros(8, 16), "wu": torch.zeros(8, 16), "bias": torch.zeros(8),
+         "scale": torch.zeros(8), "residual": torch.zeros(4, 8), "g": torch.zeros(4, 8)}
+    calls = {
+        ("x", "w", "bias", "scale", "residual"): lambda a: mb.b200_linear(a["x"], a["w"], a["bias"], "silu", a["scale"],
+                                                                          a["residual"]),
+        ("x", "w", "bias", "scale", "g"): lambda a: mb.b200_linear_backward(a["g"], a["x"], a["w"], a["bias"], "silu",
+                                                                            a["scale"]),
+        ("x", "w", "wu"): lambda a: mb.b200_gated_ffn(a["x"], a["w"], a["wu"]),
+        ("x", "w", "wu", "g"): lambda a: mb.b200_gated_ffn_backward(a["g"], a["x"], a["w"], a["wu"]),
+    }
+    with fw.dual_level():
+        for names, call in calls.items():
+            for name in names:
+                for grad in (False, True):
+                    dual = fw.make_dual(t[name].clone().requires_grad_(grad), torch.ones_like(t[name]))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call({**t, name: dual})
+            with pytest.raises(RuntimeError, match="no CPU path"):  # a level without duals changes nothing
+                call(t)

@@ -84,3 +84,13 @@ def test_column_sums_of_many_rows(dt):
     want = O.linear_backward(g[-300:], x[-300:], w, b)
     O.assert_within(dx[-300:], want["dx"], "dx")
     assert dw.shape == w.shape and bool(dw.isfinite().all())
+
+
+def test_a_dual_gradient_is_refused_in_the_backward_pass():
+    x, w = randn(gen(1), 70, 40, dt=F32), randn(gen(2), 24, 40, dt=F32).requires_grad_(True)
+    fw = torch.autograd.forward_ad
+    for y in (mb.b200_linear(x, w), mb.b200_gated_ffn(x, w, w)):
+        with fw.dual_level():
+            g = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(y, w, g)
