@@ -25,6 +25,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version  # what a kernel writes in place, autograd cannot see
 
 from . import _native as N
 from ._native import pack_matrix, pack_vector
@@ -259,7 +260,10 @@ def b200_linear(
         _check_out(out, x, shape, (("x", x), ("weight", weight), ("bias", bias), ("scale", scale)), residual)
     if tracked:
         return _LinearFunction.apply(x, weight, bias, scale, residual, act, out_dtype)
-    return _linear(x, weight, bias, act, scale, residual, out, out_dtype)
+    y = _linear(x, weight, bias, act, scale, residual, out, out_dtype)
+    if out is not None:
+        increment_version(out)
+    return y
 
 
 def b200_linear_backward(
@@ -379,7 +383,10 @@ def b200_gated_ffn(
         _check_out(out, x, out.shape, (("x", x), ("w_gate", w_gate), ("w_up", w_up)), None)
     if tracked:
         return _GatedFFNFunction.apply(x, w_gate, w_up, act)
-    return _gated_ffn(x, w_gate, w_up, act, out)
+    y = _gated_ffn(x, w_gate, w_up, act, out)
+    if out is not None:
+        increment_version(out)
+    return y
 
 
 def b200_gated_ffn_backward(

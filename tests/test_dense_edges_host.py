@@ -6,6 +6,7 @@ import torch
 
 import maba_v2_architecture_b200 as mb
 from maba_v2_architecture_b200 import _native as N
+from maba_v2_architecture_b200 import dense
 
 
 @pytest.mark.parametrize("splits,pairs", [(2, 1), (16, 1), (10, 2)])
@@ -54,3 +55,17 @@ def test_dual_tensors_are_refused():
                         call({**t, name: dual})
             with pytest.raises(RuntimeError, match="no CPU path"):  # a level without duals changes nothing
                 call(t)
+
+
+def test_out_counts_as_modified(monkeypatch):
+    """With the launch left out: a write through out= raises the version that autograd checks."""
+    monkeypatch.setattr(dense.N, "require_cuda", lambda *a, **k: None)
+    monkeypatch.setattr(dense, "_linear", lambda *a: a[6])
+    monkeypatch.setattr(dense, "_gated_ffn", lambda *a: a[4])
+    x, w, out = torch.zeros(4, 16), torch.zeros(8, 16), torch.zeros(4, 8)
+    for call in (lambda: mb.b200_linear(x, w, out=out), lambda: mb.b200_linear(x, w, residual=out, out=out),
+                 lambda: mb.b200_gated_ffn(x, w, w, out=out)):
+        y = torch.ones(8, requires_grad=True) * out
+        assert call() is out
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()

@@ -94,3 +94,22 @@ def test_a_dual_gradient_is_refused_in_the_backward_pass():
             g = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
             with pytest.raises(RuntimeError):
                 torch.autograd.grad(y, w, g)
+
+
+@pytest.mark.parametrize("op", ["linear", "gated_ffn"])
+def test_out_counts_as_modified(op):
+    """A tensor that another operation saved for its backward pass and out= then overwrote is noticed."""
+    x, w = randn(gen(1), 70, 40, dt=BF), randn(gen(2), 24, 40, dt=BF)
+    stream, p = randn(gen(3), 70, 24, dt=BF), torch.ones(24, dtype=BF, device=DEV, requires_grad=True)
+    y = p * stream
+    version = stream._version
+    if op == "linear":
+        mb.b200_linear(x, w, residual=stream, out=stream)
+    else:
+        mb.b200_gated_ffn(x, w, w, out=stream)
+    assert stream._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():  # (tensors without a version)
+        out = torch.empty(70, 24, dtype=BF, device=DEV)
+        O.assert_within(mb.b200_linear(x, w, out=out), O.linear(x, w), "inference mode")
