@@ -369,11 +369,22 @@ class MabaSparseAttention(nn.Module):
 MABASALayer = MabaSparseAttention
 
 
+def _plain_weight(m: nn.Module, name: str) -> torch.Tensor:
+    """The weight of a projection that the kernels compute without calling its module, which must
+    therefore do nothing but multiply: a plain nn.Linear without bias, hooks or a wrapper."""
+    if (getattr(type(m), "forward", None) is not nn.Linear.forward or "forward" in m.__dict__ or m.bias is not None
+            or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks):
+        raise RuntimeError(f"SwiGLUFFN: {name} must be a plain nn.Linear without bias and hooks: its weight is read, "
+                           f"the module is not called ({type(m).__name__})")
+    return m.weight
+
+
 class SwiGLUFFN(nn.Module):
     """SwiGLU feed-forward block w_down(silu(w_gate x) * w_up x) (maba_sparse/model.py:28-37).
 
-    Two kernels forward: the gated block, whose projections are never stored, and the down
-    projection; differentiable.  With ``residual`` and ``gate`` ([dim], sigmoid(res_gate)) the down
+    Two operators forward: the gated block, whose projections are never stored, and the down
+    projection; differentiable.  They read the projections' weights and do not call their modules:
+    hooks, a bias or another module in their place (an adapter) are refused.  With ``residual`` and ``gate`` ([dim], sigmoid(res_gate)) the down
     projection returns residual + gate * ffn(x), the block's gated residual add
     (maba_sparse/model.py:107-108); a float32 residual makes the result float32."""
 
@@ -388,6 +399,7 @@ class SwiGLUFFN(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 gate: Optional[torch.Tensor] = None) -> torch.Tensor:
-        a = b200_gated_ffn(x, self.w_gate.weight, self.w_up.weight)
+        w_gate, w_up, w_down = (_plain_weight(getattr(self, n), n) for n in ("w_gate", "w_up", "w_down"))
+        a = b200_gated_ffn(x, w_gate, w_up)
         out_dtype = residual.dtype if residual is not None else None
-        return b200_linear(a, self.w_down.weight, scale=gate, residual=residual, out_dtype=out_dtype)
+        return b200_linear(a, w_down, scale=gate, residual=residual, out_dtype=out_dtype)

@@ -69,3 +69,84 @@ def test_out_counts_as_modified(monkeypatch):
         assert call() is out
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+# ---------------------------------------------------------------------------
+# the module
+# ---------------------------------------------------------------------------
+def recorded(monkeypatch):
+    """The module's two calls replaced by ones that note their operands' types and compute with torch."""
+    from maba_v2_architecture_b200 import layers
+
+    calls = []
+
+    def gated(x, wg, wu):
+        calls.append((x.dtype, wg.dtype, wu.dtype))
+        return torch.nn.functional.silu(x @ wg.t()) * (x @ wu.t())
+
+    def linear(x, w, scale=None, residual=None, out_dtype=None):
+        calls.append((x.dtype, w.dtype))
+        y = x @ w.t()
+        y = y if scale is None else y * scale
+        return (y if residual is None else y + residual).to(out_dtype or x.dtype)
+
+    monkeypatch.setattr(layers, "b200_gated_ffn", gated)
+    monkeypatch.setattr(layers, "b200_linear", linear)
+    return calls
+
+
+class Adapter(torch.nn.Module):
+    def __init__(self, base):
+        super().__init__()
+        self.base, self.weight, self.bias = base, base.weight, None
+
+    def forward(self, x):
+        return 2 * self.base(x)
+
+
+class Scaled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+@pytest.mark.parametrize("name", ["w_gate", "w_up", "w_down"])
+@pytest.mark.parametrize("change", ["wrapper", "subclass", "own forward", "bias", "forward hook", "pre-hook", "backward hook",
+                                    "backward pre-hook"])
+def test_projections_that_do_more_are_refused(monkeypatch, name, change):
+    """The module reads its projections' weights; what a projection's module would do beside the product
+    is not passed by in silence."""
+    calls = recorded(monkeypatch)
+    ffn = mb.SwiGLUFFN(dim=16, intermediate_size=24)
+    lin = getattr(ffn, name)
+    if change == "wrapper":
+        setattr(ffn, name, Adapter(lin))
+    elif change == "subclass":
+        setattr(ffn, name, Scaled(lin.in_features, lin.out_features, bias=False))
+    elif change == "own forward":
+        lin.forward = lambda x: 2 * x
+    elif change == "bias":
+        setattr(ffn, name, torch.nn.Linear(lin.in_features, lin.out_features))
+    else:
+        add = {"forward hook": lin.register_forward_hook, "pre-hook": lin.register_forward_pre_hook,
+               "backward hook": lin.register_full_backward_hook, "backward pre-hook": lin.register_full_backward_pre_hook}
+        handle = add[change](lambda *a: None)
+    with pytest.raises(RuntimeError, match=f"{name} must be a plain nn.Linear"):
+        ffn(torch.zeros(3, 16))
+    assert not calls
+    if "hook" in change:
+        handle.remove()
+        assert ffn(torch.zeros(3, 16)).shape == (3, 16)
+
+
+def test_a_parametrized_weight_is_read_as_it_is_computed(monkeypatch):
+    recorded(monkeypatch)
+    ffn = mb.SwiGLUFFN(dim=16, intermediate_size=24)
+    x = torch.ones(3, 16)
+    want = ffn(x)
+
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    torch.nn.utils.parametrize.register_parametrization(ffn.w_down, "weight", Twice())
+    assert torch.equal(ffn(x), 2 * want)
