@@ -379,12 +379,23 @@ def _plain_weight(m: nn.Module, name: str) -> torch.Tensor:
     return m.weight
 
 
+def _autocast_operands(*ts: torch.Tensor):
+    """The operands of a product in the type that torch's own modules multiply them in: autocast's,
+    where it is on (float64 keeps its type)."""
+    device = ts[0].device.type
+    if not torch.is_autocast_enabled(device):
+        return ts
+    dt = torch.get_autocast_dtype(device)
+    return tuple(t if t.dtype is torch.float64 else t.to(dt) for t in ts)
+
+
 class SwiGLUFFN(nn.Module):
     """SwiGLU feed-forward block w_down(silu(w_gate x) * w_up x) (maba_sparse/model.py:28-37).
 
     Two operators forward: the gated block, whose projections are never stored, and the down
     projection; differentiable.  They read the projections' weights and do not call their modules:
-    hooks, a bias or another module in their place (an adapter) are refused.  With ``residual`` and ``gate`` ([dim], sigmoid(res_gate)) the down
+    hooks, a bias or another module in their place (an adapter) are refused.  Under autocast x and the
+    weights are taken in its type, as nn.Linear takes them.  With ``residual`` and ``gate`` ([dim], sigmoid(res_gate)) the down
     projection returns residual + gate * ffn(x), the block's gated residual add
     (maba_sparse/model.py:107-108); a float32 residual makes the result float32."""
 
@@ -400,6 +411,7 @@ class SwiGLUFFN(nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 gate: Optional[torch.Tensor] = None) -> torch.Tensor:
         w_gate, w_up, w_down = (_plain_weight(getattr(self, n), n) for n in ("w_gate", "w_up", "w_down"))
+        x, w_gate, w_up, w_down = _autocast_operands(x, w_gate, w_up, w_down)
         a = b200_gated_ffn(x, w_gate, w_up)
         out_dtype = residual.dtype if residual is not None else None
         return b200_linear(a, w_down, scale=gate, residual=residual, out_dtype=out_dtype)

@@ -150,3 +150,23 @@ def test_a_parametrized_weight_is_read_as_it_is_computed(monkeypatch):
 
     torch.nn.utils.parametrize.register_parametrization(ffn.w_down, "weight", Twice())
     assert torch.equal(ffn(x), 2 * want)
+
+
+@pytest.mark.parametrize("x_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_autocast_reaches_the_module(monkeypatch, x_dtype):
+    """float32 weights under autocast, whatever x's type: the operators get autocast's, as nn.Linear does;
+    outside, and for float64, types are left alone."""
+    calls = recorded(monkeypatch)
+    ffn = mb.SwiGLUFFN(dim=16, intermediate_size=24)
+    x, r = torch.randn(3, 16).to(x_dtype), torch.zeros(3, 16)
+    bf = torch.bfloat16
+    with torch.autocast("cpu", dtype=bf):
+        assert ffn(x).dtype is bf and ffn(x, residual=r).dtype is torch.float32
+    assert calls == [(bf, bf, bf), (bf, bf)] * 2
+    calls.clear()
+    if x_dtype is torch.float32:
+        ffn(x)
+        with torch.autocast("cpu", dtype=bf):
+            ffn.double()(x.double())
+        f32, f64 = torch.float32, torch.float64
+        assert calls == [(f32, f32, f32), (f32, f32), (f64, f64, f64), (f64, f64)]

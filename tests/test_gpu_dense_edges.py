@@ -113,3 +113,24 @@ def test_out_counts_as_modified(op):
     with torch.inference_mode():  # (tensors without a version)
         out = torch.empty(70, 24, dtype=BF, device=DEV)
         O.assert_within(mb.b200_linear(x, w, out=out), O.linear(x, w), "inference mode")
+
+
+@pytest.mark.parametrize("x_dtype", [F32, BF])
+def test_module_under_autocast(x_dtype):
+    """A training step in mixed precision: float32 weights, their gradients float32; values and gradients
+    are those of the calls on operands cast to autocast's type."""
+    torch.manual_seed(4)
+    ffn = mb.SwiGLUFFN(dim=96, intermediate_size=200).to(DEV)
+    x = randn(gen(1), 70, 96, dt=x_dtype).requires_grad_(True)
+    d = randn(gen(2), 70, 96, dt=BF)
+    with torch.autocast("cuda", dtype=BF):
+        y = ffn(x)
+    assert y.dtype is BF
+    y.backward(d)
+    xb, wg, wu, wd = (t.detach().to(BF) for t in (x, ffn.w_gate.weight, ffn.w_up.weight, ffn.w_down.weight))
+    a = mb.b200_gated_ffn(xb, wg, wu)
+    assert torch.equal(y, mb.b200_linear(a, wd))
+    da, dwd, _, _ = mb.b200_linear_backward(d, a, wd)
+    dx, dwg, dwu = mb.b200_gated_ffn_backward(da, xb, wg, wu)
+    for p, want in ((ffn.w_down.weight, dwd), (ffn.w_gate.weight, dwg), (ffn.w_up.weight, dwu), (x, dx)):
+        assert p.grad.dtype is p.dtype and torch.equal(p.grad, want.to(p.dtype))
