@@ -138,8 +138,9 @@ __device__ __forceinline__ float rcp_sfu(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 1 / (1 + e^-z): the SFU's exponential and reciprocal, a few float32 ulp (e^-z past float32
-// gives 1 / inf = 0)
+// 1 / (1 + e^-z): the SFU's exponential and reciprocal.  The exponential's argument is rounded twice,
+// so the result is off by up to (4 + |z|) 2^-23 of itself; below z = -87, where it leaves float32's
+// normal range, it is 0
 __device__ __forceinline__ void sigmoid2(float z0, float z1, float& s0, float& s1) {
     s0 = z0, s1 = z1;
     mul2(s0, s1, -1.4426950408889634f, -1.4426950408889634f);

@@ -134,3 +134,41 @@ def test_module_under_autocast(x_dtype):
     dx, dwg, dwu = mb.b200_gated_ffn_backward(da, xb, wg, wu)
     for p, want in ((ffn.w_down.weight, dwd), (ffn.w_gate.weight, dwg), (ffn.w_up.weight, dwu), (x, dx)):
         assert p.grad.dtype is p.dtype and torch.equal(p.grad, want.to(p.dtype))
+
+
+@pytest.mark.parametrize("m,k", [(4, 300), (40, 300), (300, 300), (70, 4000)])
+def test_silu_far_below_zero(m, k):
+    """z in [-60, -5], exact (one nonzero product per sum), float32: silu and its slope keep their relative
+    accuracy.  In units of 2^-23: exp 2, 1 + exp 0.5, the quotient 0.5: 3 for silu, and 1 more for the
+    product with the up projection's value.  The slope s (1 + z (1 - s)): s 3, z (1 - s) 1, which the sum
+    with 1 stretches by at most 5/4 and rounds by 0.5, the product 0.5: 5.25."""
+    n = 240
+    z = -torch.randint(20, 241, (m, n), generator=gen(1), device=DEV) / 4.0
+    x, w = torch.zeros(m, k, device=DEV), torch.eye(n, k, device=DEV)
+    x[:, :n] = z
+    zd = z.double()
+    s = torch.sigmoid(zd)
+    unit = 2.0 ** -23
+    off = lambda got, want: float(((got.double() - want) / want).abs().max()) / unit
+    assert off(mb.b200_linear(x, w, activation="silu"), zd * s) <= 3
+    assert off(mb.b200_gated_ffn(x, w, w), zd * s * zd) <= 4
+    # w's columns 0..239 are a unit matrix, so dx there is dz, or dg and du added: grad z s' + grad silu
+    one = torch.ones(m, n, device=DEV)
+    slope = s * (1 + zd * (1 - s))
+    assert off(mb.b200_linear_backward(one, x, w, None, "silu")[0][:, :n], slope) <= 5.25
+    dx = mb.b200_gated_ffn_backward(one, x, w, 2 * w)[0][:, :n]  # up: 2 z
+    assert off(dx, 2 * zd * slope + 2 * zd * s) <= 8
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("m", [40, 300])
+def test_silu_far_below_zero_from_16_bit_operands(m, dt):
+    """The same with 16-bit operands and a float32 result.  On the tensor cores' path, in units of 2^-23: the
+    exponential's argument is rounded twice, |z|; the SFU's exponential 2, the sum 0.5, the SFU's
+    reciprocal 1, the product 0.5."""
+    k = n = 240
+    z = -torch.randint(20, 241, (m, n), generator=gen(1), device=DEV) / 4.0
+    zd = z.double()
+    got = mb.b200_linear(z.to(dt), torch.eye(n, k, dtype=dt, device=DEV), activation="silu", out_dtype=F32).double()
+    want = zd * torch.sigmoid(zd)
+    assert bool(((got - want).abs() <= (4 + zd.abs()) * 2.0 ** -23 * want.abs()).all())
