@@ -559,8 +559,8 @@ int ffn_backward(Ctx& c, const FfnArgs& a) {
     if (!given(a.dx) && !given(a.dwg) && !given(a.dwu)) return MABA_OK;
     Product p;
     MABA_TRY(ffn_product(c, a, p));
-    // dg and du in the operands' type: the matrix units multiply 16-bit operands, so this is
-    // the one rounding between the two passes
+    // dg and du in the operands' type: the one rounding between the two passes where that has 16 bits,
+    // which is what the tensor cores multiply; none in float32
     const Matrix d[2] = {written_operand(c, M, p.N), written_operand(c, M, p.N)};
     p.e.out = const_cast<void*>(d[0].p), p.e.out2 = const_cast<void*>(d[1].p), p.e.ldo = d[0].sr;
     MABA_TRY(run(c, p));

@@ -7,11 +7,14 @@
 // {4 t, 64 + 4 t} + 0..3, so gate and up of a pair sit in one thread, and multiplies two columns
 // by one instruction (fma.f32x2).
 //
-// What bounds it: issue.  A k index costs a thread 32 packed multiply-adds, 8 moves that repeat a
-// row's value and 4 shared-memory loads; 4,096 x 640 -> 1,544 takes 284 us, 28.5 TFLOP/s, forward
-// and gradients of the gated block of 2,048 x 640 -> 2 x 1,248 867 us.  Library products in float32
-// with separate activations take 212 and 602.  A 64 x 128 tile, four CTAs to an SM, 8 indices at a
-// time, took 319 and 863.
+// What bounds it: whole tiles on 296 places, and issue.  4,096 x 640 -> 1,544 takes 286 us, 28.3
+// TFLOP/s, forward and gradients of the gated block of 2,048 x 640 -> 2 x 1,248 866 us; library
+// products in float32 with separate activations take 212 and 602.  The first has 416 tiles, of
+// which the last column's 32 hold 8 of 128 columns; a k index costs a thread 32 packed multiply-adds,
+// 8 moves that repeat a row's value and 4 shared-memory loads.  A contraction below 1,024 is not split
+// under an epilogue, so few rows leave most SMs idle: 16, 64 and 256 rows of 640 -> 1,544 take 111,
+// 112 and 131 us (13 and 26 CTAs), library products 16, 17 and 24.  A 64 x 128 tile, four CTAs to an
+// SM, 8 indices at a time, took 319 and 863.
 #include "dense.cuh"
 
 namespace maba {

@@ -1,7 +1,7 @@
 // Products of 16-bit operands on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
 // The tensor cores truncate when they add to their float32 accumulator, once per 16
-// contraction indices: a sum over K loses about K 5.6e-10 of itself toward zero (measured
+// contraction indices: a sum over K loses about K 1e-9 of itself toward zero (measured
 // 6e-7 relative at K = 640, 4.4e-6 at 4,096).  That is far below a 16-bit result's rounding,
 // but not below a float32 result's, so sums that end in float32 (MODE 1) leave TMEM every
 // 640 indices and are added, rounded to nearest, in the epilogue's registers.
@@ -9,8 +9,8 @@
 // Persistent, one CTA per SM.  A work unit is a tile of C (128 rows of A by bn rows of B;
 // with CG = 2 a cluster's two CTAs share a tile of 256 rows: each loads its own 128 rows of
 // A and one half of B, so a k-block costs an SM 32 KB for 128 x 256 x 64 products instead
-// of 48 KB, below what L2 delivers per SM: 199 -> 165 us for the gated block of 65,536 x 640
-// -> 2 x 1248) over one split of the contraction.  The warps:
+// of 48 KB, below what L2 delivers per SM; with this step the gated block of 65,536 x 640 -> 2 x
+// 1248 went from 199 to 165 us in a row of calls) over one split of the contraction.  The warps:
 //  * epilogue (16, or 8 where they hold a unit's sums): warp w reads TMEM lanes 32 (w & 3)..
 //           and every fourth (second) 32-column chunk and applies the epilogue;
 //  * TMA producer: 64 contraction indices per stage, 128-byte swizzle, operands K-major or
@@ -22,12 +22,13 @@
 // runs under the next unit's products.  The gated block's tile holds bn/2 rows of w_gate and
 // bn/2 of w_up, so a thread sees both projections of an element in its own row.
 //
-// What bounds it (single launches): the gated block the tensor cores (65,536 x 640 -> 2 x 1248,
-// bf16: 123 us; its two SFU operations per element take 2,048 of a unit's 5,120 cycles); the
-// linear map with a scale and a float32 residual (65,536 x 1248 -> 640) 108 us, 4.7 TB/s; with a
-// bias, SiLU, scale and residual (16,384 x 640 -> 2560) 57 us, by the epilogue's chains of
-// shared-memory, barrier and copy latencies, which the products' own use of shared memory
-// stretches; its gradient pass, with column sums, 77 us.
+// What bounds it (bf16; one launch, counters and time of a capture): the gated block of 65,536 x
+// 640 -> 2 x 1248 takes 137 us, the tensor pipe active 92 % of it; in a row of calls the power limit
+// holds the clock near 1.2 GHz and a call takes 174 us.  The linear map with a scale and a float32
+// residual, 65,536 x 1248 -> 640, takes 108 us (140 in a row, for the same reason): tensor pipe 57 %,
+// DRAM 52 % of its peak, so neither, but the epilogue's chain of TMEM, copy and barrier latencies.
+// The gradient pass of a map with a bias, SiLU and scale, 16,384 x 640 -> 2560 with column sums,
+// takes 82 us: an instruction issued in 57 % of the cycles, the ALU 47 % busy, the tensor pipe 36 %.
 //
 // Every mbarrier wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and products in flight are drained (bounded), TMEM is
@@ -74,7 +75,7 @@ static_assert(N_BARS * 8 + 8 <= BAR_BYTES, "barrier area");
 struct TcArgs {
     int64_t M, N;
     int kblocks, kseg, kb_split;  // contraction blocks over all segments, of one segment, of one split
-    int tiles_n, splits, pairs, units, dual;
+    int tiles_n, splits, pairs, units;
     int d_inner, d_col, d_row;  // from a worker's unit to its next
     int bn, b_rows;  // columns of the MMA, rows of B per CTA
     int flush;       // contraction blocks between two readings of the accumulator
@@ -978,9 +979,10 @@ Product split_sums(const Product& p) {
 }
 
 // A product with an epilogue whose few tiles have a long contraction: its sums by splits,
-// then the epilogue, where the model says that this is sooner.  (24 x 3,776 -> 2 x 120 float32,
-// one tile of 59 blocks.)  A float32 result of 16-bit
-// operands keeps its bound on one accumulation, 640 indices.
+// then the epilogue, where the model says that this is sooner (bf16, whole and split: 100 x 4,000 ->
+// 40 16.1 and 11.9 us, -> 640 16.3 and 11.3; the gated block -> 2 x 640 15.7 and 10.9; the gradient
+// pass of 24 x 3,776 -> 120 18.4 and 13.6).  A float32 result keeps its bound on one accumulation,
+// 640 indices.
 Plan tc_plan(const Product& p) {
     const int mode = mode_of(p);
     double whole, split;
@@ -1007,7 +1009,6 @@ int tc_product(const Product& p, const Plan& pl, float* partial, int64_t ldp, cu
     a.kseg = (int)ceil_div(p.K, BK);
     a.kblocks = a.kseg * (p.form == F_SUM ? 2 : 1);
     a.pairs = p.form == F_PAIR ? 2 : 1;
-    a.dual = dual;
     a.kb_split = (int)ceil_div(a.kblocks, pl.splits);
     a.splits = (int)ceil_div(a.kblocks, a.kb_split);
     a.bn = pl.bn;

@@ -10,13 +10,19 @@ The reference computes these with torch modules and autograd: SwiGLUFFN (maba_sp
 Inputs are float32, float16 or bfloat16 CUDA tensors of one type with any strides; leading
 dimensions of ``x`` are rows.  Sums are float32 and a result is rounded once; results do not
 depend on the order in which the GPU runs the work.  16-bit products run on the tensor cores,
-float32 ones on the CUDA cores.  Inputs are never written, except that ``out`` may be ``residual``.  Work is enqueued on the current stream of the tensors' device.
-Scratch memory comes from torch's allocator for each call (not from the per-stream buffer that
-the other ops keep): two captured graphs, or a graph and an eager call, then never share it.
+float32 ones on the CUDA cores.  Inputs are never written, except that ``out`` may be ``residual``.
+Autocast does not reach these functions: operands are multiplied in the type they have
+(``layers.SwiGLUFFN`` casts its own).
+
+Work is enqueued on the current stream of the tensors' device.  Scratch memory comes from torch's
+allocator for each call (not from the per-stream buffer that the other ops keep): two captured
+graphs, or a graph and an eager call, then never share it.
 
 With gradients enabled and an input that requires one, both functions record themselves for
-autograd (first derivatives, reverse mode; dual tensors are refused); ``*_backward`` are the same gradients as plain calls, for training
-loops that are captured into a CUDA graph or keep their own tape.
+autograd (first derivatives, reverse mode; dual tensors are refused).  ``*_backward`` are the same
+gradients as plain calls, for training loops that keep their own tape or are captured into a CUDA
+graph.  (Autograd's own backward pass is to be captured only while no eager graph of the same
+leaves lives: torch accumulates their gradients on the eager graph's stream.)
 """
 from __future__ import annotations
 
@@ -224,7 +230,9 @@ def b200_linear(
     out: Optional[torch.Tensor] = None,
     out_dtype: Optional[torch.dtype] = None,
 ) -> torch.Tensor:
-    """``residual + scale * act(x weight^T + bias)`` in one kernel.
+    """``residual + scale * act(x weight^T + bias)``, the epilogue applied to the float32 sums.
+    One launch, and one more each where 16-bit inputs have rows off 16-byte boundaries (they are
+    copied first) and where few outputs with a long contraction split it.
 
     x [..., K], weight [N, K] (nn.Linear's layout), bias and scale [N] and residual [..., N] in x's
     dtype or float32; ``activation`` one of ``none``, ``relu``, ``silu``, ``gelu`` (the erf form).
@@ -279,8 +287,8 @@ def b200_linear_backward(
     ``grad_out`` [..., N] (x's dtype or float32); the residual's is grad_out itself.  ``needs``
     says which are computed (dbias / dscale only where bias / scale are given); the rest are None.
 
-    z = x weight^T + bias is computed again where act' or dscale needs it, so the forward pass
-    keeps nothing but its inputs.  grad_out * scale * act'(z) is rounded to x's dtype between the
+    z = x weight^T + bias is computed again where an activation or a scale is given, so the forward
+    pass keeps nothing but its inputs.  grad_out * scale * act'(z) is rounded to x's dtype between the
     products; the column sums of dbias and dscale are taken before that rounding.
     """
     act = _activation(activation, True)
@@ -361,8 +369,9 @@ def b200_gated_ffn(
     activation: str = "silu",
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """``act(x w_gate^T) * (x w_up^T)``: both projections, the activation and the product in one
-    kernel; the two projections are never stored.
+    """``act(x w_gate^T) * (x w_up^T)``: both projections, the activation and the product; the
+    projections are never stored, but for float32 partial sums where few outputs with a long
+    contraction split it.  Launches as for ``b200_linear``.
 
     x [..., K], w_gate and w_up [I, K]; ``activation`` one of ``silu``, ``gelu`` (the erf form),
     ``relu``.  The result is [..., I] in x's dtype.  Reference: maba_sparse/model.py:28-37

@@ -228,7 +228,9 @@ class MabaEngine:
     ``fused_dense`` runs the blocks' projections of a prefill on this library's dense operators:
     the gated feed-forward block as one kernel, and every output projection adding its gated result
     to the residual stream in its epilogue (``b200_gated_ffn``, ``b200_linear``), in place of matrix
-    products with separate SwiGLU and residual kernels.  Same function; sums are ordered differently."""
+    products with separate SwiGLU and residual kernels.  Same function; sums are ordered differently.
+    It pays in 16 bits (8 x 8,192 tokens, the last 256 positions' logits: 39.5 -> 36.4 ms), not in
+    float32 (8 x 2,048 tokens: 241 -> 269 ms)."""
 
     def __init__(self, config, state_dict: Dict[str, torch.Tensor], device="cuda", dtype=torch.bfloat16,
                  ablation_mode: Optional[str] = None, fused_dense: bool = False):
