@@ -364,6 +364,11 @@ int want_vector(const maba_tensor* t, const char* name, int64_t n, int dt) {
     if (t->stride[0] < 0) return set_error(MABA_ERR_INVALID, "%s: negative stride", name);
     return MABA_OK;
 }
+// a gradient: its elements lie apart
+int want_vector_out(const maba_tensor* t, const char* name, int64_t n, int dt) {
+    MABA_TRY(want_vector(t, name, n, dt));
+    return n > 1 && t->stride[0] < 1 ? set_error(MABA_ERR_INVALID, "%s: elements must not overlap", name) : MABA_OK;
+}
 
 int want_operands(const maba_tensor* x, const maba_tensor* w, const char* wname, int act, int act_min) {
     if (!given(x)) return set_error(MABA_ERR_INVALID, "x: tensor is required");
@@ -587,11 +592,11 @@ int check_linear(const LinearArgs& a, bool backward) {
     if (given(a.dx)) MABA_TRY(want_matrix(a.dx, "dx", M, K, dt, false, true));
     if (given(a.dw)) MABA_TRY(want_matrix(a.dw, "dw", N, K, dt, false, true));
     if (given(a.dbias)) {
-        MABA_TRY(want_vector(a.dbias, "dbias", N, dt));
+        MABA_TRY(want_vector_out(a.dbias, "dbias", N, dt));
         if (!given(a.bias)) return set_error(MABA_ERR_INVALID, "dbias without bias");
     }
     if (given(a.dscale)) {
-        MABA_TRY(want_vector(a.dscale, "dscale", N, dt));
+        MABA_TRY(want_vector_out(a.dscale, "dscale", N, dt));
         if (!given(a.scale)) return set_error(MABA_ERR_INVALID, "dscale without scale");
     }
     return MABA_OK;

@@ -170,3 +170,27 @@ def test_autocast_reaches_the_module(monkeypatch, x_dtype):
             ffn.double()(x.double())
         f32, f64 = torch.float32, torch.float64
         assert calls == [(f32, f32, f32), (f32, f32), (f64, f64, f64), (f64, f64)]
+
+
+# ---------------------------------------------------------------------------
+# refusals of the C entries (nothing is launched: the workspace is missing)
+# ---------------------------------------------------------------------------
+def descriptor(shape, stride=None):
+    t = N.MabaTensor(1 << 20, 0, len(shape))
+    run = 1
+    for i in reversed(range(len(shape))):
+        t.shape[i], t.stride[i] = shape[i], run if stride is None else stride[i]
+        run *= shape[i]
+    return ctypes.byref(t)
+
+
+def test_gradient_vectors_that_overlap_themselves_are_refused():
+    d = descriptor
+    x, w, g, v, same = d((4, 16)), d((8, 16)), d((4, 8)), d((8,)), d((8,), (0,))
+    lib = N.lib()
+    run = lambda *vec: lib.maba_linear_backward(g, x, w, v, 0, v, None, None, *vec, None, 0, None)
+    assert run(v, v) == N.ERR_WORKSPACE  # accepted
+    assert run(same, v) == N.ERR_INVALID and b"dbias" in lib.maba_last_error()
+    assert run(v, same) == N.ERR_INVALID and b"dscale" in lib.maba_last_error()
+    one = d((1,), (0,))  # (a single element does not)
+    assert lib.maba_linear_backward(d((4, 1)), x, d((1, 16)), one, 0, None, None, None, one, None, None, 0, None) == N.ERR_WORKSPACE
