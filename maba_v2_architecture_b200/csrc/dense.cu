@@ -341,6 +341,7 @@ bool given(const maba_tensor* t) { return t != nullptr && t->ndim > 0; }
 int want_matrix(const maba_tensor* t, const char* name, int64_t rows, int64_t cols, int dt, bool f32_ok, bool dense_rows) {
     if (!given(t)) return set_error(MABA_ERR_INVALID, "%s: tensor is required", name);
     if (t->ndim != 2) return set_error(MABA_ERR_INVALID, "%s: expected 2 dims, got %d", name, t->ndim);
+    if (t->shape[0] < 0 || t->shape[1] < 0) return set_error(MABA_ERR_INVALID, "%s: negative size", name);
     if ((rows >= 0 && t->shape[0] != rows) || (cols >= 0 && t->shape[1] != cols))
         return set_error(MABA_ERR_INVALID, "%s: shape [%lld, %lld], expected [%lld, %lld]", name, (long long)t->shape[0],
                          (long long)t->shape[1], (long long)rows, (long long)cols);

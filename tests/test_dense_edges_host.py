@@ -194,3 +194,12 @@ def test_gradient_vectors_that_overlap_themselves_are_refused():
     assert run(v, same) == N.ERR_INVALID and b"dscale" in lib.maba_last_error()
     one = d((1,), (0,))  # (a single element does not)
     assert lib.maba_linear_backward(d((4, 1)), x, d((1, 16)), one, 0, None, None, None, one, None, None, 0, None) == N.ERR_WORKSPACE
+
+
+def test_negative_sizes_are_refused():
+    """Also where every tensor agrees on them."""
+    d, lib = descriptor, N.lib()
+    assert lib.maba_linear_backward(d((-4, 8)), d((-4, 16)), d((8, 16)), None, 1, None, d((-4, 16)), None, None, None, None, 0,
+                                    None) == N.ERR_INVALID
+    assert lib.maba_gated_ffn_workspace_size(d((-4, 16)), d((8, 16)), d((8, 16)), d((-4, 8))) == 0
+    assert b"negative size" in lib.maba_last_error()
